@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -111,6 +112,20 @@ SIGNATURES = {
                             c_i64, c_void_p, c_size_t, c_void_p], c_int),
     "lifb_leaky_fwd": ([c_void_p, c_void_p, c_i64, c_i64, c_float, c_void_p], c_int),
     "lifb_leaky_bwd": ([c_void_p, c_void_p, c_i64, c_i64, c_float, c_void_p], c_int),
+    "lifb_embed_fwd": ([c_void_p, c_int, c_void_p, c_void_p, c_i64, c_i64, c_i64, c_i64, c_float, c_int, c_void_p],
+                       c_int),
+    "lifb_embed_bwd_workspace_bytes": ([c_i64, c_i64, c_i64], c_size_t),
+    "lifb_embed_bwd": ([c_void_p, c_int, c_void_p, c_void_p, c_i64, c_i64, c_i64, c_i64, c_float, c_int, c_void_p,
+                        c_size_t, c_void_p], c_int),
+    "lifb_norm_gate_fwd": ([c_void_p, c_void_p, c_void_p, c_void_p], c_int),
+    "lifb_norm_gate_bwd_workspace_bytes": ([c_i64, c_i64, c_int], c_size_t),
+    "lifb_norm_gate_bwd": ([c_void_p, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p,
+                            c_void_p, c_void_p, c_size_t, c_void_p], c_int),
+    "lifb_leaky_attn_workspace_bytes": ([c_void_p, c_int], c_size_t),
+    "lifb_leaky_attn_fwd": ([c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p], c_int),
+    "lifb_leaky_attn_bwd": ([c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                             c_void_p, c_size_t, c_void_p], c_int),
+    "lifb_leaky_attn_step": ([c_void_p, c_void_p, c_void_p, c_void_p], c_int),
     "lifb_spike_mask_stride": ([c_i64], c_i64),
     "lifb_spike_mask": ([c_void_p, c_void_p, c_i64, c_i64, c_void_p], c_int),
     "lifb_spike_linear_lif_fwd": ([c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -147,7 +162,7 @@ class LifbError(RuntimeError):
     """A nonzero status returned by liblifb.  `status` is the library's
     status code; for a device-side error (LIFB_ERR_DEVICE) `device_code` is
     the code a kernel recorded (101: a bounded wait for an asynchronous copy
-    expired), else None."""
+    expired; 102: a token id past the embedding table), else None."""
 
     def __init__(self, msg, status=None, device_code=None):
         super().__init__(msg)
@@ -230,6 +245,52 @@ def ptr(t):
 
 def stream_of(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+# Element types of the sequence-model operators (LIFB_F32, LIFB_BF16, LIFB_F16).
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+# Argument blocks of the sequence-model operators, packed in one call in the
+# C layout of lifb_norm_gate, lifb_leaky_attn and lifb_leaky_attn_step_args.
+NORM_GATE = struct.Struct("@6P6q2f3i")
+LEAKY_ATTN = struct.Struct("@6P15qfi")
+LEAKY_ATTN_STEP = struct.Struct("@5P14qfi")
+
+
+def addr(t) -> int:
+    """The tensor's address; 0 (NULL) for None."""
+    return 0 if t is None else t.data_ptr()
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def on_device(t: torch.Tensor):
+    """torch.cuda.device(t.device) where that is not the current device already."""
+    return _here if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def need_cuda(what: str, **tensors) -> None:
+    """Raises unless every tensor given (None: absent) is on one CUDA device."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: {name} must be a CUDA tensor")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, not {dev}")
 
 
 class Stats(ctypes.Structure):

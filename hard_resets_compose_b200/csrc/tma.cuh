@@ -21,6 +21,7 @@ constexpr long long kWaitCycles = LIFB_WAIT_CYCLES;
 enum DeviceStatus : int {
     kStatusOk = 0,
     kStatusTmaWaitTimeout = 101,
+    kStatusTokenRange = 102,  // a token id past the embedding table
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }

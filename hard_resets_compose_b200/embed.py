@@ -1,0 +1,73 @@
+"""Embedding with scaling, and its gradient by sorted tokens (csrc/embed.cu).
+
+    y = embedding(tokens, weight, scale)      # y[i] = scale * weight[tokens[i]]
+
+Negative tokens are padding: zeros out, no gradient.  A token past the table
+gives zeros too and is reported as a device error (code 102) by the library's
+next poll or by `_lib.check_device`.  The weight's gradient adds the rows of
+each token in fp32, in an order that the tokens alone fix, and is rounded
+once: the same bits on every call.  The reference has no such operator.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import DTYPES, addr, check, need_cuda, on_device, stream_of
+
+
+def _forward(tokens, weight, scale):
+    n, (V, D) = tokens.numel(), weight.shape
+    y = torch.empty(*tokens.shape, D, dtype=weight.dtype, device=weight.device)
+    with on_device(weight):
+        check(_lib.load().lifb_embed_fwd(addr(tokens), tokens.element_size(), addr(weight), addr(y), n, V, D,
+                                         max(weight.stride(0), D), scale, DTYPES[weight.dtype], stream_of(weight)),
+              "embedding")
+    return y
+
+
+class Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale):
+        ctx.save_for_backward(tokens)
+        ctx.cfg = (weight.shape, weight.dtype, scale)
+        return _forward(tokens, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        tokens, = ctx.saved_tensors
+        (V, D), dtype, scale = ctx.cfg
+        n = tokens.numel()
+        dy = dy.reshape(n, D)
+        if dy.stride(-1) != 1 or dy.stride(0) < D:
+            dy = dy.contiguous()
+        dw = torch.empty(V, D, dtype=dtype, device=dy.device)
+        lib = _lib.load()
+        with on_device(dy):
+            nb = lib.lifb_embed_bwd_workspace_bytes(n, V, D)
+            ws = torch.empty(nb, dtype=torch.uint8, device=dy.device)
+            check(lib.lifb_embed_bwd(addr(tokens), tokens.element_size(), addr(dy), addr(dw), n, V, D,
+                                     max(dy.stride(0), D), scale, DTYPES[dtype], addr(ws), nb, stream_of(dy)),
+                  "embedding")
+            _lib.poll_device("embedding")
+        return None, dw, None
+
+
+def embedding(tokens, weight, scale=1.0):
+    """scale * weight[tokens]: tokens of any shape (int32 or int64, negative:
+    padding), weight [V, D] (fp32, bf16 or fp16); returns [*tokens.shape, D]."""
+    if weight.dim() != 2:
+        raise ValueError(f"embedding: weight must be [V, D], got {tuple(weight.shape)}")
+    if weight.dtype not in DTYPES:
+        raise TypeError(f"embedding: weight must be fp32, bf16 or fp16, got {weight.dtype}")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"embedding: tokens must be int32 or int64, got {tokens.dtype}")
+    need_cuda("embedding", tokens=tokens, weight=weight)
+    tokens = tokens.contiguous()
+    if weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
+        weight = weight.contiguous()
+    if weight.requires_grad and torch.is_grad_enabled():
+        return Embedding.apply(tokens, weight, float(scale))
+    return _forward(tokens, weight, float(scale))

@@ -1,0 +1,174 @@
+"""Leaky attention: linear attention with a decay for each head, the leaky
+integrator with a matrix for a state (csrc/leaky_attn.cu).
+
+    S_t = b S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t,   b = exp(log_decay[h])
+
+    o        = leaky_attention(q, k, v, log_decay)                       # training
+    o, state = leaky_attention(q, k, v, log_decay, state=state, lengths=lengths, return_state=True)   # prompts
+    o        = leaky_attention_step(q, k, v, log_decay, state, slots)    # one token, the state in place
+
+q [B, T, H, Dk], k [B, T, Hk, Dk], v [B, T, Hk, Dv] in fp32 or bf16 (the step
+takes fp16 too), H a multiple of Hk (each key/value head serves H / Hk query
+heads), widths up to 128, log_decay [H] fp32 and at most 0 (-inf: no memory),
+states [B, H, Dk, Dv] fp32.  Any strides with a contiguous last dimension.
+fp16 is refused for sequences: a sum over many tokens leaves its range before
+it leaves bf16's.  The decay is a constant: it gets no gradient.  The reference
+has no such operator.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import DTYPES, addr, check, need_cuda, on_device, stream_of
+
+MAX_WIDTH = 128
+
+
+def _last_dense(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _pack(q, k, v, log_decay, state, lengths, scale):
+    B, T, H, Dk = q.shape
+    Hk, Dv = v.shape[2:]
+    return _lib.LEAKY_ATTN.pack(addr(q), addr(k), addr(v), addr(log_decay), addr(state), addr(lengths), B, T, H, Hk,
+                                Dk, Dv, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], scale, DTYPES[q.dtype])
+
+
+def _forward(q, k, v, log_decay, state, lengths, scale, return_state):
+    B, T, H, Dk = q.shape
+    Dv = v.shape[3]
+    dev = q.device
+    o = torch.empty(B, T, H, Dv, dtype=q.dtype, device=dev)
+    out = torch.empty(B, H, Dk, Dv, device=dev) if return_state else None
+    lib = _lib.load()
+    args = _pack(q, k, v, log_decay, state, lengths, scale)
+    with on_device(q):
+        nb = lib.lifb_leaky_attn_workspace_bytes(args, 0)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        check(lib.lifb_leaky_attn_fwd(args, addr(o), addr(out), addr(ws), nb, stream_of(q)), "leaky_attention")
+    return o, out
+
+
+class LeakyAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, lengths, scale, return_state):
+        o, out = _forward(q, k, v, log_decay, state, lengths, scale, return_state)
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return o, out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, dout):
+        q, k, v, log_decay, state, lengths = ctx.saved_tensors
+        if do is None and dout is None:
+            return (None,) * 8
+        dev = q.device
+        if do is None:
+            do = torch.zeros(*q.shape[:3], v.shape[3], dtype=q.dtype, device=dev)
+        do = _last_dense(do)
+        dout = None if dout is None else dout.contiguous()
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        ds = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
+        lib = _lib.load()
+        args = _pack(q, k, v, log_decay, state, lengths, ctx.scale)
+        with on_device(q):
+            nb = lib.lifb_leaky_attn_workspace_bytes(args, 1)
+            ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+            check(lib.lifb_leaky_attn_bwd(args, addr(do), (_lib.c_i64 * 3)(*do.stride()[:3]), addr(dout), addr(dq),
+                                          addr(dk), addr(dv), addr(ds), addr(ws), nb, stream_of(q)),
+                  "leaky_attention")
+            _lib.poll_device("leaky_attention")
+        return dq, dk, dv, None, ds, None, None, None
+
+
+def _check(what, q, k, v, log_decay, lead, types):
+    if q.dim() != lead + 2 or k.dim() != lead + 2 or v.dim() != lead + 2:
+        raise ValueError(f"{what}: q, k and v must have {lead + 2} dimensions")
+    H, Dk = q.shape[lead:]
+    Hk, Dv = v.shape[lead:]
+    if k.shape[:lead] != q.shape[:lead] or v.shape[:lead] != q.shape[:lead] or k.shape[lead:] != (Hk, Dk):
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
+    if Hk == 0 and H > 0 or Hk > 0 and H % Hk:
+        raise ValueError(f"{what}: {H} heads cannot share {Hk} key/value heads")
+    if Dk > MAX_WIDTH or Dv > MAX_WIDTH:
+        raise ValueError(f"{what}: head widths {Dk} and {Dv}; at most {MAX_WIDTH}")
+    if q.dtype not in types or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"{what}: q, k and v must share one of {', '.join(str(t) for t in types)}, got {q.dtype}, "
+                        f"{k.dtype}, {v.dtype}")
+    if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
+        raise ValueError(f"{what}: log_decay must be [{H}] fp32, got {tuple(log_decay.shape)} {log_decay.dtype}")
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: the decay is a constant and gets no gradient: pass log_decay.detach()")
+    return H, Hk, Dk, Dv
+
+
+def leaky_attention(q, k, v, log_decay, state=None, lengths=None, scale=None, return_state=False):
+    """o [B, T, H, Dv], or (o, final state) with return_state.
+
+    state [B, H, Dk, Dv] fp32: the state before the first token (None: zeros).
+    lengths [B] int32: tokens at and past a sequence's length are not read, give
+    zeros and leave the state alone.  scale: Dk ** -0.5 by default.  Gradients for
+    q, k, v and state."""
+    what = "leaky_attention"
+    H, _, Dk, Dv = _check(what, q, k, v, log_decay, 2, (torch.float32, torch.bfloat16))
+    need_cuda(what, q=q, k=k, v=v, log_decay=log_decay, state=state, lengths=lengths)
+    B = q.shape[0]
+    if state is not None:
+        if state.shape != (B, H, Dk, Dv) or state.dtype != torch.float32:
+            raise ValueError(f"{what}: state must be [{B}, {H}, {Dk}, {Dv}] fp32, got {tuple(state.shape)} "
+                             f"{state.dtype}")
+        state = state.contiguous()
+    if lengths is not None:
+        if lengths.shape != (B,) or lengths.dtype != torch.int32:
+            raise ValueError(f"{what}: lengths must be [{B}] int32, got {tuple(lengths.shape)} {lengths.dtype}")
+        lengths = lengths.contiguous()
+    scale = float(Dk) ** -0.5 if scale is None and Dk > 0 else float(scale or 0.0)
+    args = (_last_dense(q), _last_dense(k), _last_dense(v), log_decay.contiguous(), state, lengths, scale,
+            bool(return_state))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (state is not None and state.requires_grad)):
+        o, out = LeakyAttention.apply(*args)
+    else:
+        o, out = _forward(*args)
+    return (o, out) if return_state else o
+
+
+def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
+    """One token of each sequence: o [B, H, Dv]; `state` is updated in place.
+
+    q [B, H, Dk], k [B, Hk, Dk], v [B, Hk, Dv]; state [n_slots, H, Dk, Dv] fp32, each
+    head's matrix contiguous; slots [B] int32: the place of each sequence's state
+    (None: its own index), at most one sequence to a slot; a place outside the
+    cache (-1, say) is empty: zeros out, nothing changed.  Not differentiable."""
+    what = "leaky_attention_step"
+    H, Hk, Dk, Dv = _check(what, q, k, v, log_decay, 1, tuple(DTYPES))
+    need_cuda(what, q=q, k=k, v=v, log_decay=log_decay, state=state, slots=slots)
+    B = q.shape[0]
+    if state.dim() != 4 or state.shape[1:] != (H, Dk, Dv) or state.dtype != torch.float32:
+        raise ValueError(f"{what}: state must be [slots, {H}, {Dk}, {Dv}] fp32, got {tuple(state.shape)} {state.dtype}")
+    st = state.stride()
+    if Dk * Dv > 1 and ((Dv > 1 and st[3] != 1) or (Dk > 1 and st[2] != Dv)):
+        raise ValueError(f"{what}: each head's state must be contiguous")
+    if slots is None:
+        if state.shape[0] < B:
+            raise ValueError(f"{what}: {B} sequences but {state.shape[0]} states")
+    elif slots.shape != (B,) or slots.dtype != torch.int32:
+        raise ValueError(f"{what}: slots must be [{B}] int32, got {tuple(slots.shape)} {slots.dtype}")
+    else:
+        slots = slots.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        raise RuntimeError(f"{what} is not differentiable: use leaky_attention, or torch.no_grad()")
+    q, k, v, log_decay = _last_dense(q), _last_dense(k), _last_dense(v), log_decay.contiguous()
+    scale = float(Dk) ** -0.5 if scale is None and Dk > 0 else float(scale or 0.0)
+    o = torch.empty(B, H, Dv, dtype=q.dtype, device=q.device)
+    args = _lib.LEAKY_ATTN_STEP.pack(addr(q), addr(k), addr(v), addr(log_decay), addr(slots), B, H, Hk, Dk, Dv,
+                                     state.shape[0], *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *st[:2],
+                                     scale, DTYPES[q.dtype])
+    with on_device(q):
+        check(_lib.load().lifb_leaky_attn_step(args, addr(o), addr(state), stream_of(q)), what)
+    return o

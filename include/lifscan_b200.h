@@ -549,6 +549,95 @@ int lifb_tshard_bwd_fix(const float *I, const float *u_prev, const float *U, con
                         const float *lam_top, float *Lam, int64_t T, int64_t N, float beta,
                         float theta, float alpha, int C, void *ws, size_t bytes, void *stream);
 
+/* ---- Sequence-model operators ----------------------------------------------
+ * What a token model puts around the recurrences above.  The reference has none
+ * of them.  Element types of tensors: */
+#define LIFB_F32 0
+#define LIFB_BF16 1
+#define LIFB_F16 2
+
+/* Embedding: Y[i] = scale * W[tokens[i]] ([n, D], contiguous; W [V, D] with rows
+ * w_stride elements apart).  tokens: n integers of token_bytes (4 or 8).  A
+ * negative token gives a row of zeros; one >= V does too, and reports device
+ * status 102 (lifb_check_device).
+ * Gradient: dW [V, D] (contiguous, written whole) = scale * the sum of dY's rows
+ * of each token, in an order that the tokens alone fix (same bits each call).
+ * Sums in fp32, rounded once.  n < 2^31 - 2^20, V < 2^30. */
+int lifb_embed_fwd(const void *tokens, int token_bytes, const void *W, void *Y, int64_t n, int64_t V,
+                   int64_t D, int64_t w_stride, float scale, int dtype, void *stream);
+size_t lifb_embed_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
+int lifb_embed_bwd(const void *tokens, int token_bytes, const void *dY, void *dW, int64_t n, int64_t V,
+                   int64_t D, int64_t dy_stride, float scale, int dtype, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/* Norms around a block with its gate and scaled residual, over rows of D:
+ *   y = rmsnorm(h) * post;  xo = x + scale * act(gate) * y;  n = rmsnorm(xo) * pre
+ * h NULL: no block (xo is not written, n = rmsnorm(x) * pre); n NULL: no norm
+ * after it.  gate: gate_cols = D (elementwise), 1 (one value a row) or 0 (none).
+ * act 0: g * sigmoid(g), 1: sigmoid(g), 2: g.  x, h, gate, xo, n are of `dtype`,
+ * the weights fp32 or of `dtype`; rows of x, h and gate lie *_stride elements
+ * apart, xo and n are contiguous.  rstd [2][R] fp32: written by the forward
+ * (NULL: not kept), read by the backward.  D <= 8192. */
+typedef struct lifb_norm_gate {
+    const void *x, *h, *gate, *post, *pre;
+    float *rstd;
+    int64_t R, D, x_stride, h_stride, gate_stride, gate_cols;
+    float scale, eps;
+    int act, dtype, weight_dtype;
+} lifb_norm_gate;
+int lifb_norm_gate_fwd(const lifb_norm_gate *args, void *xo, void *n, void *stream);
+/* Gradients from dxo and dn (either may be NULL: zero); dx, dh, dgate, dpost and
+ * dpre (contiguous) are written where not NULL.  The workspace is for dpost and
+ * dpre, whose sums run in a fixed order. */
+size_t lifb_norm_gate_bwd_workspace_bytes(int64_t R, int64_t D, int dtype);
+int lifb_norm_gate_bwd(const lifb_norm_gate *args, const void *dxo, int64_t dxo_stride, const void *dn,
+                       int64_t dn_stride, void *dx, void *dh, void *dgate, void *dpost, void *dpre,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+/* Leaky attention (linear attention with a decay b = exp(log_decay[h]) <= 1 for
+ * each head):  S_t = b S_{t-1} + k_t v_t^T,  o_t = scale * S_t^T q_t.
+ * q [B, T, H, Dk], k [B, T, Hk, Dk], v [B, T, Hk, Dv] (fp32 or bf16; strides in
+ * elements for sequence, token and head; the last dimension contiguous), H a
+ * multiple of Hk, Dk and Dv <= 128, log_decay [H] fp32, state [B, H, Dk, Dv] fp32
+ * (NULL: zeros), lengths [B] (NULL: T each): tokens at and past a sequence's
+ * length are not read, change no state and give zeros. */
+typedef struct lifb_leaky_attn {
+    const void *q, *k, *v;
+    const float *log_decay, *state;
+    const int32_t *lengths;
+    int64_t B, T, H, Hk, Dk, Dv;
+    int64_t q_strides[3], k_strides[3], v_strides[3];
+    float scale;
+    int dtype;
+} lifb_leaky_attn;
+size_t lifb_leaky_attn_workspace_bytes(const lifb_leaky_attn *args, int backward);
+/* o [B, T, H, Dv] contiguous; state_out [B, H, Dk, Dv] (NULL: not wanted). */
+int lifb_leaky_attn_fwd(const lifb_leaky_attn *args, void *o, float *state_out, void *workspace,
+                        size_t workspace_bytes, void *stream);
+/* Gradients from d_o (strides as q's) and the gradient of the final state
+ * (dstate_out; NULL: zeros): dq, dk, dv contiguous, dstate the initial state's
+ * (NULL: not wanted). */
+int lifb_leaky_attn_bwd(const lifb_leaky_attn *args, const void *d_o, const int64_t *d_o_strides,
+                        const float *dstate_out, void *dq, void *dk, void *dv, float *dstate,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
+/* One token of each of B sequences: q [B, H, Dk], k [B, Hk, Dk], v [B, Hk, Dv]
+ * (fp32, bf16 or fp16; strides for sequence and head), o [B, H, Dv] contiguous.
+ * The cache `state` [n_slots, H, Dk, Dv] fp32 (strides for slot and head) is
+ * updated in place; sequence i has slot slots[i] (NULL: i).  A slot outside
+ * [0, n_slots) is an empty place: its output is zero and no state changes.  No
+ * two sequences may share a slot. */
+typedef struct lifb_leaky_attn_step_args {
+    const void *q, *k, *v;
+    const float *log_decay;
+    const int32_t *slots;
+    int64_t B, H, Hk, Dk, Dv, n_slots;
+    int64_t q_strides[2], k_strides[2], v_strides[2], state_strides[2];
+    float scale;
+    int dtype;
+} lifb_leaky_attn_step_args;
+int lifb_leaky_attn_step(const lifb_leaky_attn_step_args *args, void *o, float *state, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
