@@ -455,8 +455,10 @@ Split split_time(int64_t chains, int64_t T, int64_t room)
     return best;
 }
 
+// Blocks that the GPU holds at once, of the kernel that the type and widths point to.
 int64_t attn_room(int64_t dq, int64_t dv, int dtype)
 {
+    if (dtype == LIFB_BF16 && dq % 8 == 0 && dv % 8 == 0) return kAtSms * attn_tc_blocks_per_sm((int)dq, (int)dv);
     return kAtSms * 2 / std::max<int64_t>(1, (dv + kAtTile - 1) / kAtTile);
 }
 
@@ -507,16 +509,20 @@ int at_check(const char *what, const lifb_leaky_attn *p)
     return LIFB_OK;
 }
 
-void run_passes(AttnArgs &a, int passes, int dtype, cudaStream_t s)
+bool run_passes(AttnArgs &a, int passes, int dtype, cudaStream_t s)
 {
+    const bool tc = attn_tc_applies(a, passes, dtype);
+    auto run = [&](bool state_only) {
+        return tc ? attn_tc(a, passes, state_only, s) : attn_simt(a, passes, dtype, state_only, s);
+    };
     if (a.nseg > 1) {
-        attn_simt(a, passes, dtype, true, s);
+        if (!run(true)) return false;
         int64_t mat = 0;
         for (int i = 0; i < passes; i++) mat = std::max<int64_t>(mat, (int64_t)a.p[i].dq * a.p[i].dv);
         count_launches(1);
         k_attn_join<<<dim3((unsigned)((mat + 255) / 256), (unsigned)(a.B * a.H), (unsigned)passes), 256, 0, s>>>(a);
     }
-    attn_simt(a, passes, dtype, false, s);
+    return run(false);
 }
 
 void strides_of(int64_t (&st)[3], const int64_t *from) { st[0] = from[0], st[1] = from[1], st[2] = from[2]; }
@@ -577,8 +583,8 @@ extern "C" int lifb_leaky_attn_fwd(const lifb_leaky_attn *p, void *o, float *sta
     f.s_in = p->state, f.s_out = state_out, f.s_row = p->Dv, f.s_col = 1;
     f.p_scale = f.i_scale = p->scale, f.w_scale = 1.0f;
     f.seg = w.seg[0];
-    run_passes(a, 1, p->dtype, s);
-    if (cudaGetLastError() != cudaSuccess) return at_fail(LIFB_ERR_CUDA, what, "launch failed");
+    if (!run_passes(a, 1, p->dtype, s) || cudaGetLastError() != cudaSuccess)
+        return at_fail(LIFB_ERR_CUDA, what, "launch failed");
     set_last_error("");
     return LIFB_OK;
 }
@@ -660,7 +666,7 @@ extern "C" int lifb_leaky_attn_bwd(const lifb_leaky_attn *p, const void *d_o, co
     z.p_scale = z.w_scale = p->scale, z.i_scale = 1.0f;
     z.shift = 1, z.rev = 1, z.o_f32 = g > 1;
     z.seg = w.seg[2];
-    run_passes(a, 3, p->dtype, s);
+    if (!run_passes(a, 3, p->dtype, s)) return at_fail(LIFB_ERR_CUDA, what, "launch failed");
     if (g > 1) {
         const int64_t rows = p->B * p->T * p->Hk;
         auto blocks = [&](int64_t d) { return (unsigned)std::min<int64_t>((rows * d + 255) / 256, kAtSms * 16); };

@@ -70,6 +70,11 @@ bool make_tmap_2d_typed(CUtensorMap *m, const void *base, bool int32, int64_t N,
 // = 64 or 128 bytes of columns) x box_y rows, in the swizzled shared-memory
 // layout of the tensor cores' K-major operands.
 bool make_tmap_2d_swz(CUtensorMap *m, const float *base, int64_t N, int64_t T, int box_y, int swz_bytes);
+// 4-D bf16 tensor map in the 128-byte swizzled layout: dims (innermost first) with
+// the strides of the other three in elements; box {64, box_y, 1, 1}.  False where
+// an address, a stride (multiples of 16 bytes) or a size does not fit.
+bool make_tmap_4d_bf16(CUtensorMap *m, const void *base, const int64_t (&dims)[4], const int64_t (&strides)[3],
+                       int box_x, int box_y);
 bool make_tmap_3d_u32(CUtensorMap *m, const void *base, int64_t d0, int64_t d1, int64_t d2, int b0, int b1, int b2);
 int *device_status_ptr();                 // status word of the current device
 int read_device_status(bool reset);       // synchronous read (current device)

@@ -101,6 +101,28 @@ bool make_tmap_3d_u32(CUtensorMap *m, const void *base, int64_t d0, int64_t d1, 
     return r == CUDA_SUCCESS;
 }
 
+bool make_tmap_4d_bf16(CUtensorMap *m, const void *base, const int64_t (&dims)[4], const int64_t (&strides)[3],
+                       int box_x, int box_y)
+{
+    bind_primary_context();
+    auto enc = encoder();
+    if (!enc || ((uintptr_t)base & 15) || box_x * 2 != 128 || box_y < 1 || box_y > 256) return false;
+    cuuint64_t d[4], st[3];
+    for (int i = 0; i < 4; i++) {
+        if (dims[i] < 1 || dims[i] >= (int64_t(1) << 31)) return false;
+        d[i] = (cuuint64_t)dims[i];
+    }
+    for (int i = 0; i < 3; i++) {
+        const int64_t bytes = dims[i + 1] == 1 ? 16 : strides[i] * 2;  // one element along it: never used
+        if (bytes <= 0 || bytes % 16 || bytes >= (int64_t(1) << 40)) return false;
+        st[i] = (cuuint64_t)bytes;
+    }
+    cuuint32_t box[4] = {(cuuint32_t)box_x, (cuuint32_t)box_y, 1, 1}, estr[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void *)base, d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int *device_status_ptr()
 {
     int dev = 0;
