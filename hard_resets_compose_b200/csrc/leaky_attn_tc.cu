@@ -23,10 +23,10 @@
 // it, if loads, MMAs and the element-wise work overlap:
 //   warps 0-3   P: tensor memory -> decay, bf16 -> tensor memory (A operand of P V);
 //               O: the epilogue to global memory.  A thread owns a token.
-//   warps 4-7   k's three pieces in shared memory (the first in k's place), then the
+//   4 or 8 more k's three pieces in shared memory (the first in k's place), then the
 //               state: registers += MMA result, its bf16 copy to shared memory.
-//   warp 8      TMA loads: k two chunks deep, q and v reloaded as their MMAs end.
-//   warp 9      issues all MMAs.
+//   one warp    TMA loads: k two chunks deep, q and v reloaded as their MMAs end.
+//   one warp    issues all MMAs.
 // Every wait is bounded (status 101).
 #include <algorithm>
 
@@ -41,7 +41,6 @@ namespace lifb {
 namespace {
 
 constexpr int kTcC = 128;           // tokens of a chunk
-constexpr int kTcThreads = 320;
 constexpr int kTcBlock = kTcC * 128;  // bytes of 128 rows of 64 bf16
 
 struct AttnMaps {
@@ -61,6 +60,11 @@ struct TcLayout {
     static constexpr uint32_t tmem_cols = DV == 64 ? 256 : 512;
     static constexpr uint32_t o1 = 128, o2 = 128 + DV, ds = 128 + 2 * DV;  // ds: dv = 128 only
     static constexpr int blocks_per_sm = DQ == 64 && DV == 64 ? 2 : 1;
+    // warpgroups of the state: where one block has an SM, two, with half of the columns
+    // each, so that the state stays in registers (128 a thread at 14 warps)
+    static constexpr int state_groups = blocks_per_sm == 1 ? 2 : 1;
+    static constexpr int tma_warp = 4 + 4 * state_groups, mma_warp = tma_warp + 1;
+    static constexpr int threads = 32 * (mma_warp + 1);
 };
 
 struct TcBars {
@@ -72,57 +76,90 @@ struct TcBars {
 
 // This thread's row of P: scores from tensor memory, times p_scale * b^distance
 // where the other token is not in the future (and is one of the n), else zero;
-// packed to bf16 into 64 of the same 128 columns.  Powers of b come from the
-// diagonal outwards by one multiplication each.  Forward passes walk the columns
+// packed to bf16 into 64 of the same 128 columns.  Powers of b (pw[i] = b^i) run
+// from the diagonal outwards.  Forward passes walk the columns
 // downwards and pack into the upper half, backward passes the other way round, so
 // that nothing unread is overwritten.
 template <bool REV>
-__device__ __forceinline__ void attn_scores(uint32_t lane_cols, int warp, int lane, int n, float b, float p_scale)
+__device__ __forceinline__ void attn_scores(uint32_t lane_cols, int warp, int lane, int n, float b16,
+                                            const float (&pw)[16], float p_scale)
 {
     float d = 0.0f;
-#pragma unroll 1
-    for (int s = 0; s < 4; s++) {
-        const int kb = REV ? s : 3 - s;  // 32 columns
-        uint32_t w[16];
-        const bool past = REV ? kb < warp : kb > warp;  // wholly on the other side of the diagonal
-        if (past) {
+    auto col = [&](int s) { return (REV ? s : 7 - s) * 16; };
+    uint32_t x[2][16];
+    const int first = 2 * (REV ? warp : 3 - warp);  // before it all columns are on the other side of the diagonal
+    tmem_load16(lane_cols + col(first), x[0]);
+    {
+        const uint32_t zero[8] = {};
+        for (int s = 0; s < first; s++) tmem_store8(lane_cols + (REV ? 0 : 64) + col(s) / 2, zero);
+    }
+    // the pair of column blocks with the diagonal, then the ones past it
 #pragma unroll
-            for (int i = 0; i < 16; i++) w[i] = 0;
-        } else {
-            uint32_t x[32];
-            tmem_load32(lane_cols + kb * 32, x);
-            tmem_wait_ld();
-            float y[32];
-            if (kb == warp) {
+    for (int half = 0; half < 2; half++) {
+        tmem_wait_ld();
+        if (half == 0) tmem_load16(lane_cols + col(first + 1), x[1]);
+        else if (first < 6) tmem_load16(lane_cols + col(first + 2), x[0]);
+        uint32_t w[8];
+        float y[16];
 #pragma unroll
-                for (int t = 0; t < 32; t++) {
-                    const int e = REV ? t : 31 - t;
-                    d = e == lane ? p_scale : d * b;
-                    y[e] = (REV ? e >= lane : e <= lane) ? __uint_as_float(x[e]) * d : 0.0f;
-                }
-            } else {
-#pragma unroll
-                for (int t = 0; t < 32; t++) {
-                    const int e = REV ? t : 31 - t;
-                    d *= b;
-                    y[e] = __uint_as_float(x[e]) * d;
-                }
-            }
-            if (REV && n < kTcC) {
-#pragma unroll
-                for (int e = 0; e < 32; e++)
-                    if (kb * 32 + e >= n) y[e] = 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i++) w[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
+        for (int t = 0; t < 16; t++) {
+            const int e = REV ? t : 15 - t, c = (REV ? half : 1 - half) * 16 + e;  // of the pair's 32 columns
+            d = c == lane ? p_scale : d * pw[1];
+            y[e] = (REV ? c >= lane : c <= lane) ? __uint_as_float(x[half][e]) * d : 0.0f;
+            if (REV && warp * 32 + c >= n) y[e] = 0.0f;
         }
-        tmem_store16(lane_cols + (REV ? 0 : 64) + kb * 16, w);
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
+        tmem_store8(lane_cols + (REV ? 0 : 64) + col(first + half) / 2, w);
+    }
+    d *= pw[1];  // of the next block's nearest column
+#pragma unroll 1
+    for (int s = first + 2; s < 8; s += 2) {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            tmem_wait_ld();
+            if (half == 0) tmem_load16(lane_cols + col(s + 1), x[1]);
+            else if (s < 6) tmem_load16(lane_cols + col(s + 2), x[0]);
+            uint32_t w[8];
+            float y[16];
+#pragma unroll
+            for (int t = 0; t < 16; t++) {
+                const int e = REV ? t : 15 - t;
+                y[e] = __uint_as_float(x[half][e]) * (d * pw[t]);
+                if (REV && n < kTcC && col(s + half) + e >= n) y[e] = 0.0f;
+            }
+            d *= b16;
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
+            tmem_store8(lane_cols + (REV ? 0 : 64) + col(s + half) / 2, w);
+        }
     }
     tmem_wait_st();
 }
 
+// A 4 x 4 transposition of 16-byte elements among the four lanes of a quad:
+// m[i] of lane j becomes m[j] of lane i.
+__device__ __forceinline__ void quad_transpose(uint32_t (&m)[4][4], int lane)
+{
+#pragma unroll
+    for (int step = 1; step <= 2; step *= 2) {
+        const bool up = lane & step;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (i & step) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t send = up ? m[i][e] : m[i + step][e];
+                const uint32_t got = __shfl_xor_sync(~0u, send, step);
+                if (up) m[i][e] = got;
+                else m[i + step][e] = got;
+            }
+        }
+    }
+}
+
 template <int DQ, int DV, bool STATE_ONLY>
-__global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
+__global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>::blocks_per_sm))
     k_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps maps, int *status)
 {
     using L = TcLayout<DQ, DV>;
@@ -145,7 +182,7 @@ __global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
     auto first_token = [&](int c) { return s0 + (int64_t)(p.rev ? chunks - 1 - c : c) * kTcC; };
     auto tokens = [&](int64_t t0) { return (int)min((int64_t)kTcC, min(s1, len) - t0); };
 
-    if (warp == 9) tmem_alloc(&tmem_slot, L::tmem_cols);
+    if (warp == L::mma_warp) tmem_alloc(&tmem_slot, L::tmem_cols);
     if (tid == 0) {
         mbar_init(&bars.q_full, 1);
         mbar_init(&bars.q_free, 1);
@@ -157,13 +194,13 @@ __global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
         mbar_init(&bars.v_free, 1);
         mbar_init(&bars.p_full, 1);
         mbar_init(&bars.p_ready, 128);
-        mbar_init(&bars.kw_ready, 128);
-        mbar_init(&bars.s_ready, 128);
+        mbar_init(&bars.kw_ready, 128 * L::state_groups);
+        mbar_init(&bars.s_ready, 128 * L::state_groups);
         mbar_init(&bars.s_free, 1);
         mbar_init(&bars.o_full, 1);
         mbar_init(&bars.o_free, 128);
         mbar_init(&bars.ds_full, 1);
-        mbar_init(&bars.ds_free, 128);
+        mbar_init(&bars.ds_free, 128 * L::state_groups);
         mbar_init(&bars.done, 1);
         fence_barrier_init();
     }
@@ -184,7 +221,7 @@ __global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
         return false;
     };
 
-    if (warp == 8) {
+    if (warp == L::tma_warp) {
         // ---- loads
         if (lane == 0) {
             prefetch_tmap(&maps.k[pi]);
@@ -220,7 +257,7 @@ __global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
             if (nv > 0) mbar_wait(&bars.v_full, (nv - 1) & 1);
             for (int i = std::max(0, nk - 2); i < nk; i++) mbar_wait(&bars.k_full[i & 1], (i >> 1) & 1);
         }
-    } else if (warp == 9) {
+    } else if (warp == L::mma_warp) {
         // ---- MMAs
         if (lane == 0) {
             const uint32_t sb = smem_u32(base);
@@ -290,15 +327,20 @@ __global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
         if (!STATE_ONLY) {
             const uint32_t lanes = (uint32_t)(warp * 32) << 16;
             const int row = warp * 32 + lane;
-            const float beta = decay_pow(ld, 1.0f);
+            float pw[16];
+            pw[0] = 1.0f;
+            pw[1] = decay_pow(ld, 1.0f);
+#pragma unroll
+            for (int i = 2; i < 16; i++) pw[i] = pw[i / 2] * pw[i - i / 2];
+            const float b16 = pw[8] * pw[8];
             const int64_t o_at = b * p.os[0] + h * p.os[2];
             for (int c = 0; c < chunks; c++) {
                 const int64_t t0 = first_token(c);
                 const int n = tokens(t0);
                 if (!wait_warp(&bars.p_full, c)) break;
                 tcgen05_after();
-                if (p.rev) attn_scores<true>(tmem + lanes, warp, lane, n, beta, p.p_scale);
-                else attn_scores<false>(tmem + lanes, warp, lane, n, beta, p.p_scale);
+                if (p.rev) attn_scores<true>(tmem + lanes, warp, lane, n, b16, pw, p.p_scale);
+                else attn_scores<false>(tmem + lanes, warp, lane, n, b16, pw, p.p_scale);
                 tcgen05_before();
                 mbar_arrive(&bars.p_ready);
 
@@ -310,9 +352,10 @@ __global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
                 const int64_t at = o_at + (t0 + row) * p.os[1];
 #pragma unroll 1
                 for (int g = 0; g < DV / 32; g++) {
-                    uint32_t x[32], y[32];
+                    uint32_t x[32], y[2][16];
                     tmem_load32(tmem + lanes + L::o1 + g * 32, x);
-                    tmem_load32(tmem + lanes + L::o2 + g * 32, y);
+                    tmem_load16(tmem + lanes + L::o2 + g * 32, y[0]);
+                    tmem_load16(tmem + lanes + L::o2 + g * 32 + 16, y[1]);
                     tmem_wait_ld();
                     if (g == DV / 32 - 1) {
                         tcgen05_before();
@@ -321,21 +364,27 @@ __global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
                     float o[32];
 #pragma unroll
                     for (int e = 0; e < 32; e++)
-                        o[e] = row < n ? fmaf(w, __uint_as_float(y[e]), __uint_as_float(x[e])) : 0.0f;
+                        o[e] = row < n ? fmaf(w, __uint_as_float(y[e / 16][e % 16]), __uint_as_float(x[e])) : 0.0f;
                     if (in && p.o_f32) {
                         float *dst = (float *)p.o + at + g * 32;
 #pragma unroll
                         for (int e = 0; e < 32; e += 4)
                             if (g * 32 + e < p.dv)
                                 *reinterpret_cast<float4 *>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                    } else if (in) {
-                        __nv_bfloat16 *dst = (__nv_bfloat16 *)p.o + at + g * 32;
+                    } else if (!p.o_f32) {
+                        // four lanes hold four rows of 64 bytes: transposed among them, so that they
+                        // write 64 consecutive bytes of one row at a time
+                        uint32_t m[4][4];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8)
-                            if (g * 32 + e < p.dv)
-                                *reinterpret_cast<uint4 *>(dst + e) =
-                                    make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]),
-                                               pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
+                        for (int e = 0; e < 16; e++) m[e / 4][e % 4] = pack_bf16(o[2 * e], o[2 * e + 1]);
+                        quad_transpose(m, lane);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int r4 = (row & ~3) + i, col = g * 32 + (lane & 3) * 8;
+                            if (t0 + r4 < s1 && col < p.dv)
+                                *reinterpret_cast<uint4 *>((__nv_bfloat16 *)p.o + o_at + (t0 + r4) * p.os[1] + col) =
+                                    make_uint4(m[i][0], m[i][1], m[i][2], m[i][3]);
+                        }
                     }
                     __syncwarp();
                 }
@@ -353,11 +402,12 @@ __global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
             }
         }
     } else {
-        // ---- k's pieces and the state: one row of the state a thread
-        const int st = tid - 128, sw = warp - 4;
-        const uint32_t lanes = (uint32_t)(sw * 32) << 16;
+        // ---- k's pieces and the state: one row of the state a thread, SC of its columns
+        constexpr int NB = L::state_groups, SC = DV / NB;
+        const int at = tid - 128, st = at & 127, c0 = (at >> 7) * SC;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const bool has_row = st < DQ;  // uniform over a warp
-        float S[DV];
+        float S[SC];
         const int64_t mat = (int64_t)p.dq * p.dv;
         {
             const float *s_in = nullptr;
@@ -372,82 +422,102 @@ __global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
                 }
             }
 #pragma unroll
-            for (int j = 0; j < DV; j++) S[j] = s_in && st < p.dq && j < p.dv ? s_in[st * row + j * col] : 0.0f;
+            for (int j = 0; j < SC; j++)
+                S[j] = s_in && st < p.dq && c0 + j < p.dv ? s_in[st * row + (c0 + j) * col] : 0.0f;
         }
         auto put_state = [&] {  // its bf16 copy, the B operand of Q S
             if (has_row) {
 #pragma unroll
-                for (int j = 0; j < DV; j += 8)
-                    *reinterpret_cast<uint4 *>(base + L::s + (j / 64) * (DQ * 128) + st * 128 +
-                                               (((j % 64) / 8) ^ (st & 7)) * 16) =
+                for (int j = 0; j < SC; j += 8) {
+                    const int col = c0 + j;
+                    *reinterpret_cast<uint4 *>(base + L::s + (col / 64) * (DQ * 128) + st * 128 +
+                                               (((col % 64) / 8) ^ (st & 7)) * 16) =
                         make_uint4(pack_bf16(S[j], S[j + 1]), pack_bf16(S[j + 2], S[j + 3]),
                                    pack_bf16(S[j + 4], S[j + 5]), pack_bf16(S[j + 6], S[j + 7]));
+                }
             }
             fence_proxy_async_shared();
             mbar_arrive(&bars.s_ready);
         };
         if (!STATE_ONLY && chunks > 0) put_state();
         const DecayFactor full(ld, kTcC);
-        // the weights of the eight tokens whose columns this thread scales
-        float wk[8];
+        // the weights of the tokens whose columns this thread scales
+        constexpr int NW = 8 / NB;
+        float wk[NW];
         int wn = -1;  // the chunk size that they are for
         for (int c = 0; c < chunks; c++) {
             const int64_t t0 = first_token(c);
             const int n = tokens(t0);
             if (n != wn) {  // the first chunk, the one with the sequence's end, and the one after it
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int row = st / 8 + 16 * i, r = p.rev ? n - 1 - row : row;
+                for (int i = 0; i < NW; i++) {
+                    const int row = at / 8 + 16 * NB * i, r = p.rev ? n - 1 - row : row;
                     wk[i] = row < n ? p.w_scale * decay_pow(ld, (float)(n - 1 - r + p.shift)) : 0.0f;
                 }
                 wn = n;
             }
             if (!wait_warp(&bars.k_full[c & 1], c >> 1)) break;
             if (!STATE_ONLY && !wait_warp(&bars.p_full, c)) break;  // Q K^T has read k
-            if (t0 + kTcC > len && t0 + n < min(t0 + kTcC, a.T)) {
+            if (t0 + n < min(t0 + kTcC, a.T)) {
                 // what lies past the end may be anything: a zero weight does not remove it from v
                 if (!wait_warp(&bars.v_full, c)) break;
                 uint4 *v4 = reinterpret_cast<uint4 *>(base + L::v);
-                for (int i = st; i < (int)L::kV / 16; i += 128)
+                for (int i = at; i < (int)L::kV / 16; i += 128 * NB)
                     if (i / 8 % kTcC >= n) v4[i] = make_uint4(0, 0, 0, 0);
             }
             uint4 *k4 = reinterpret_cast<uint4 *>(base + L::k + (c & 1) * L::kQ);
             uint4 *mid4 = reinterpret_cast<uint4 *>(base + L::mid), *lo4 = reinterpret_cast<uint4 *>(base + L::lo);
 #pragma unroll 1
-            for (int blk = 0; blk < DQ / 64; blk++)
+            for (int blk = 0; blk < DQ / 64; blk++) {
+                // four loads first: a thread's vectors do not depend on one another
+                const int i0 = blk * (kTcBlock / 16) + at;  // rows at / 8 + 16 NB it
 #pragma unroll
-            for (int it = 0; it < 8; it++) {
-                const int i = blk * (kTcBlock / 16) + it * 128 + st;  // row st / 8 + 16 it of the block
-                const uint4 x = k4[i];
-                const float w = wk[it];
-                const bool zero = st / 8 + 16 * it >= n;
-                uint32_t in[4] = {x.x, x.y, x.z, x.w}, hi[4], mid[4], lo[4];
+                for (int j = 0; j < NW; j += 4) {
+                uint4 x[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float f0 = zero ? 0.0f : bf16_lo(in[e]) * w, f1 = zero ? 0.0f : bf16_hi(in[e]) * w;
-                    hi[e] = pack_bf16(f0, f1);
-                    const float g0 = f0 - bf16_lo(hi[e]), g1 = f1 - bf16_hi(hi[e]);
-                    mid[e] = pack_bf16(g0, g1);
-                    lo[e] = pack_bf16(g0 - bf16_lo(mid[e]), g1 - bf16_hi(mid[e]));
+                for (int it = 0; it < 4; it++) x[it] = k4[i0 + (j + it) * 128 * NB];
+#pragma unroll
+                for (int it = 0; it < 4; it++) {
+                    const int i = i0 + (j + it) * 128 * NB;
+                    const float w = wk[j + it];
+                    const bool zero = at / 8 + 16 * NB * (j + it) >= n;
+                    uint32_t in[4] = {x[it].x, x[it].y, x[it].z, x[it].w}, hi[4], mid[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float f0 = zero ? 0.0f : bf16_lo(in[e]) * w, f1 = zero ? 0.0f : bf16_hi(in[e]) * w;
+                        hi[e] = pack_bf16(f0, f1);
+                        const float g0 = f0 - bf16_lo(hi[e]), g1 = f1 - bf16_hi(hi[e]);
+                        mid[e] = pack_bf16(g0, g1);
+                        lo[e] = pack_bf16(g0 - bf16_lo(mid[e]), g1 - bf16_hi(mid[e]));
+                    }
+                    k4[i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    mid4[i] = make_uint4(mid[0], mid[1], mid[2], mid[3]);
+                    lo4[i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
-                k4[i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                mid4[i] = make_uint4(mid[0], mid[1], mid[2], mid[3]);
-                lo4[i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
             }
             fence_proxy_async_shared();
             mbar_arrive(&bars.kw_ready);
 
-            const DecayFactor bn = n == kTcC ? full : DecayFactor(ld, n);
+            float bn_hi = full.hi, bn_lo = full.lo;
+            if (n != kTcC) {
+                const DecayFactor f(ld, n);
+                bn_hi = f.hi;
+                bn_lo = f.lo;
+            }
             if (!wait_warp(&bars.ds_full, c)) break;
             tcgen05_after();
             if (has_row) {
 #pragma unroll
-                for (int g = 0; g < DV / 32; g++) {
+                for (int g = 0; g < SC / 32; g++) {
                     uint32_t x[32];
-                    tmem_load32(ds_cols + lanes + g * 32, x);
+                    tmem_load32(ds_cols + lanes + c0 + g * 32, x);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; e++) S[g * 32 + e] = bn.times(S[g * 32 + e]) + __uint_as_float(x[e]);
+                    for (int e = 0; e < 32; e++) {
+                        float &z = S[g * 32 + e];
+                        z = fmaf(z, bn_hi, fmaf(z, bn_lo, __uint_as_float(x[e])));
+                    }
                 }
             }
             tcgen05_before();
@@ -468,13 +538,13 @@ __global__ void __launch_bounds__(kTcThreads, (TcLayout<DQ, DV>::blocks_per_sm))
         }
         if (s_out && st < p.dq) {
 #pragma unroll
-            for (int j = 0; j < DV; j++)
-                if (j < p.dv) s_out[st * row + j * col] = S[j];
+            for (int j = 0; j < SC; j++)
+                if (c0 + j < p.dv) s_out[st * row + (c0 + j) * col] = S[j];
         }
     }
     tcgen05_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == L::mma_warp) {
         tcgen05_after();
         tmem_free(tmem, L::tmem_cols);
     }
@@ -497,7 +567,7 @@ bool launch_tc(const AttnArgs &a, const AttnMaps &m, int passes, bool state_only
     auto kern = state_only ? k_attn_tc<DQ, DV, true> : k_attn_tc<DQ, DV, false>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
     count_launches(1);
-    kern<<<dim3((unsigned)(a.B * a.H * a.nseg), (unsigned)passes), kTcThreads, smem, s>>>(a, m, device_status_ptr());
+    kern<<<dim3((unsigned)(a.B * a.H * a.nseg), (unsigned)passes), TcLayout<DQ, DV>::threads, smem, s>>>(a, m, device_status_ptr());
     return true;
 }
 
