@@ -458,7 +458,7 @@ Split split_time(int64_t chains, int64_t T, int64_t room)
 // Blocks that the GPU holds at once, of the kernel that the type and widths point to.
 int64_t attn_room(int64_t dq, int64_t dv, int dtype)
 {
-    if (dtype == LIFB_BF16 && dq % 8 == 0 && dv % 8 == 0) return kAtSms * attn_tc_blocks_per_sm((int)dq, (int)dv);
+    if (dtype == LIFB_BF16 && dq % 8 == 0 && dv % 8 == 0) return kAtSms;
     return kAtSms * 2 / std::max<int64_t>(1, (dv + kAtTile - 1) / kAtTile);
 }
 

@@ -88,7 +88,6 @@ bool attn_simt(const AttnArgs &a, int passes, int dtype, bool state_only, cudaSt
 // leaky_attn_tc.cu: chunks of 128 tokens on the tensor cores, bf16 operands that TMA
 // can load (16-byte aligned strides, widths multiples of 8).
 bool attn_tc_applies(const AttnArgs &a, int passes, int dtype);
-int attn_tc_blocks_per_sm(int dq, int dv);
 bool attn_tc(const AttnArgs &a, int passes, bool state_only, cudaStream_t s);
 
 }  // namespace lifb

@@ -15,20 +15,30 @@
 // Precision: P and S enter their MMAs rounded to bf16, like the inputs are; S
 // itself stays in fp32 registers of its warps, one row of the state a thread.  A
 // rounded weighted k would put 2^-9 into the fp32 state, so b^(C-1-r) k is split
-// into three bf16 pieces (24 bits) that three MMAs add up.
+// into bf16 pieces that as many MMAs add up: two (2^-18) where the state only feeds
+// further bf16 products, three (24 bits) where it is returned.
 //
-// Per chunk and head at dq = dv = 128: 6 x 128^3 multiply-adds (3 of them the
-// state's pieces), 3072 cycles of the tensor cores at 4096 a cycle and SM, against
-// 128 KB of q, k, v, o: 5500 cycles at 1/148 of 6.46 TB/s.  So memory should bound
-// it, if loads, MMAs and the element-wise work overlap:
-//   warps 0-3   P: tensor memory -> decay, bf16 -> tensor memory (A operand of P V);
-//               O: the epilogue to global memory.  A thread owns a token.
-//   4 or 8 more k's three pieces in shared memory (the first in k's place), then the
-//               state: registers += MMA result, its bf16 copy to shared memory.
-//   one warp    TMA loads: k two chunks deep, q and v reloaded as their MMAs end.
-//   one warp    issues all MMAs.
+// Per chunk and head at dq = dv = 128: q, k, v, o are 128 KB, 4800 cycles of the
+// memory that 128 busy SMs share; the MMAs are 5 x 128^3 multiply-adds, 2560 cycles
+// at 4096 a cycle and SM, but an MMA with both operands in shared memory reads 8 KB
+// in 64 cycles, all that shared memory can give (128 bytes a cycle): with the loads
+// and the element-wise writes 512 KB pass through it, 4000 cycles.  So no stage may wait
+// for another (measured: with P, k's pieces, O and S done by 12 warps one after
+// another 7400 cycles a chunk):
+//   scores      P: tensor memory -> decay, bf16 -> tensor memory (A operand of P V).
+//               A thread owns a token.  Two warpgroups where dv = 64 leaves tensor
+//               memory for two P's, in turn.
+//   output      the epilogue to global memory.  A thread owns a token.
+//   state       k's pieces in shared memory (the first in k's place), then the state:
+//               registers += MMA result, its bf16 copy to shared memory.  One warpgroup
+//               for each 64 columns.
+//   one warp    TMA loads, as far ahead as there are tiles.
+//   one warp    issues all MMAs: Q S of a chunk first (the last state is there),
+//               then the state's while the scores are worked on, P V, the next Q K^T.
+// Registers are moved from the other warpgroups to the state's (setmaxnreg).
 // Every wait is bounded (status 101).
 #include <algorithm>
+#include <type_traits>
 
 #include "leaky_attn.h"
 #include "lifb_common.cuh"
@@ -43,6 +53,7 @@ namespace {
 constexpr int kTcC = 128;           // tokens of a chunk
 constexpr int kTcBlock = kTcC * 128;  // bytes of 128 rows of 64 bf16
 
+// Tensor maps of the passes of one launch.
 struct AttnMaps {
     CUtensorMap q[kAttnMaxPasses], k[kAttnMaxPasses], v[kAttnMaxPasses];
 };
@@ -50,27 +61,44 @@ struct AttnMaps {
 // Shared memory of a block: tiles of 64-column blocks.  What an MMA with fewer
 // than 128 rows of A reads past its 64 columns (dq = 64) must lie inside: a piece is
 // never the last tile.
-template <int DQ, int DV>
+template <int DQ, int DV, int NP>
 struct TcLayout {
     static constexpr uint32_t kQ = DQ / 64 * kTcBlock, kV = DV / 64 * kTcBlock, kS = DV / 64 * DQ * 128;
-    static constexpr uint32_t mid = 0, lo = kQ, k = 2 * kQ, q = 4 * kQ, v = 5 * kQ, s = 5 * kQ + kV;
-    static constexpr uint32_t bytes = 5 * kQ + kV + kS;
-    // columns of tensor memory.  dv = 64: the state's MMA result lies over the half
-    // of P's scores that its bf16 form leaves free, so that two blocks share an SM.
-    static constexpr uint32_t tmem_cols = DV == 64 ? 256 : 512;
-    static constexpr uint32_t o1 = 128, o2 = 128 + DV, ds = 128 + 2 * DV;  // ds: dv = 128 only
-    static constexpr int blocks_per_sm = DQ == 64 && DV == 64 ? 2 : 1;
-    // warpgroups of the state: where one block has an SM, two, with half of the columns
-    // each, so that the state stays in registers (128 a thread at 14 warps)
-    static constexpr int state_groups = blocks_per_sm == 1 ? 2 : 1;
-    static constexpr int tma_warp = 4 + 4 * state_groups, mma_warp = tma_warp + 1;
-    static constexpr int threads = 32 * (mma_warp + 1);
+    static constexpr int nq = DQ == 64 || DV == 64 ? 2 : 1, nv = DQ == 128 && NP == 3 ? 1 : 2, nk = 2;
+    static constexpr uint32_t mid = 0, lo = kQ, k = (NP - 1) * kQ, q = k + nk * kQ, v = q + nq * kQ, s = v + nv * kV,
+                              bytes = s + kS;
+    static_assert(bytes + 1024 + 512 <= 227 * 1024, "tiles fit an SM");
+    // columns of tensor memory
+    static constexpr int np = DV == 64 ? 2 : 1;  // P's in flight
+    static_assert(np <= nq && np <= nk, "Q K^T of the next chunk does not wait for this one's other MMAs");
+    static constexpr uint32_t tmem_cols = 512, o1 = np * 128, o2 = o1 + DV, ds = o2 + DV;
+    static_assert(ds + DV <= tmem_cols, "accumulators fit");
+    // warpgroups: scores, output, state, and one with the loading and the issuing warp
+    static constexpr int score_groups = np, state_groups = DV / 64;
+    static constexpr int output_group = score_groups, first_state = score_groups + 1,
+                         last_group = first_state + state_groups;
+    static constexpr int threads = 128 * (last_group + 1);
+    // registers a thread: 640 threads are launched with 96 each, 480 for the five groups
+    static constexpr int score_regs = 80, output_regs = 80, state_regs = DV == 64 ? 152 : 128, last_regs = 64;
+    static_assert(threads == 640 && score_groups * score_regs + output_regs + state_groups * state_regs + last_regs <= 480,
+                  "no more registers than the block was launched with");
 };
 
 struct TcBars {
-    uint64_t q_full, q_free, k_full[2], k_free[2], v_full, v_free;
-    uint64_t p_full, p_ready, kw_ready, s_ready, s_free, o_full, o_free, ds_full, ds_free, done;
+    uint64_t q_full[2], q_free[2], k_full[2], k_free[2], v_full[2], v_free[2];
+    uint64_t p_full[2], p_ready[2], kw_ready, s_ready, s_free, o_full, o_free, ds_full, ds_free, done;
 };
+
+template <int N>
+__device__ __forceinline__ void regs_inc()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 }  // namespace
 
@@ -158,16 +186,48 @@ __device__ __forceinline__ void quad_transpose(uint32_t (&m)[4][4], int lane)
     }
 }
 
-template <int DQ, int DV, bool STATE_ONLY>
-__global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>::blocks_per_sm))
+// w * x for eight bf16 elements x (four words) as NP bf16 pieces; `zero`: x is not a
+// token of the sequence and may be anything.
+// Two pieces: with w = wh + wm in bf16, hi = x wh rounded, and what that rounding
+// dropped is exact in bf16 (the product has 16 bits), so mid = x wm + it.
+template <int NP>
+__device__ __forceinline__ void split_weighted(const uint32_t (&in)[4], bool zero, float w, uint32_t (&hi)[4],
+                                               uint32_t (&mid)[4], uint32_t (&lo)[4])
+{
+    if constexpr (NP == 2) {
+        const __nv_bfloat16 w1 = __float2bfloat16_rn(w), w2 = __float2bfloat16_rn(w - __bfloat162float(w1));
+        const __nv_bfloat162 wh = __halves2bfloat162(w1, w1), wm = __halves2bfloat162(w2, w2);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t xe = zero ? 0u : in[e];
+            const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&xe);
+            const __nv_bfloat162 h = __hmul2_rn(x, wh);
+            const __nv_bfloat162 m = __hfma2(x, wm, __hfma2(x, wh, __hneg2(h)));
+            hi[e] = *reinterpret_cast<const uint32_t *>(&h);
+            mid[e] = *reinterpret_cast<const uint32_t *>(&m);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float f0 = zero ? 0.0f : bf16_lo(in[e]) * w, f1 = zero ? 0.0f : bf16_hi(in[e]) * w;
+            hi[e] = pack_bf16(f0, f1);
+            const float g0 = f0 - bf16_lo(hi[e]), g1 = f1 - bf16_hi(hi[e]);
+            mid[e] = pack_bf16(g0, g1);
+            lo[e] = pack_bf16(g0 - bf16_lo(mid[e]), g1 - bf16_hi(mid[e]));
+        }
+    }
+}
+
+template <int DQ, int DV, int NP, bool STATE_ONLY>
+__global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     k_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps maps, int *status)
 {
-    using L = TcLayout<DQ, DV>;
+    using L = TcLayout<DQ, DV, NP>;
     extern __shared__ unsigned char tc_raw[];
     unsigned char *base = (unsigned char *)(((uintptr_t)tc_raw + 1023) & ~(uintptr_t)1023);
     __shared__ TcBars bars;
     __shared__ uint32_t tmem_slot;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = warp >> 2;
     const int pi = blockIdx.y;
     const AttnPass &p = a.p[pi];
     const int64_t bh = blockIdx.x / a.nseg;
@@ -182,18 +242,18 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>
     auto first_token = [&](int c) { return s0 + (int64_t)(p.rev ? chunks - 1 - c : c) * kTcC; };
     auto tokens = [&](int64_t t0) { return (int)min((int64_t)kTcC, min(s1, len) - t0); };
 
-    if (warp == L::mma_warp) tmem_alloc(&tmem_slot, L::tmem_cols);
-    if (tid == 0) {
-        mbar_init(&bars.q_full, 1);
-        mbar_init(&bars.q_free, 1);
+    if (warp == 0) tmem_alloc(&tmem_slot, L::tmem_cols);
+    if (tid == 32) {
         for (int i = 0; i < 2; i++) {
+            mbar_init(&bars.q_full[i], 1);
+            mbar_init(&bars.q_free[i], 1);
             mbar_init(&bars.k_full[i], 1);
             mbar_init(&bars.k_free[i], 1);
+            mbar_init(&bars.v_full[i], 1);
+            mbar_init(&bars.v_free[i], 1);
+            mbar_init(&bars.p_full[i], 1);
+            mbar_init(&bars.p_ready[i], 128);
         }
-        mbar_init(&bars.v_full, 1);
-        mbar_init(&bars.v_free, 1);
-        mbar_init(&bars.p_full, 1);
-        mbar_init(&bars.p_ready, 128);
         mbar_init(&bars.kw_ready, 128 * L::state_groups);
         mbar_init(&bars.s_ready, 128 * L::state_groups);
         mbar_init(&bars.s_free, 1);
@@ -208,7 +268,6 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>
     __syncthreads();
     tcgen05_after();
     const uint32_t tmem = tmem_slot;
-    const uint32_t ds_cols = tmem + (DV == 64 ? (p.rev ? 64u : 0u) : L::ds);
     // bounded waits; a role that gives up ends, and the others then run out of theirs
     auto wait = [&](uint64_t *bar, uint32_t phase) {  // one thread's
         if (mbar_wait(bar, phase & 1)) return true;
@@ -221,129 +280,139 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>
         return false;
     };
 
-    if (warp == L::tma_warp) {
-        // ---- loads
-        if (lane == 0) {
+    if (group == L::last_group) {
+        regs_dec<L::last_regs>();
+        if ((warp & 3) == 0 && lane == 0) {
+            // ---- loads
             prefetch_tmap(&maps.k[pi]);
             prefetch_tmap(&maps.v[pi]);
             if (!STATE_ONLY) prefetch_tmap(&maps.q[pi]);
             const int hq = (int)(h / p.qg), hk = (int)(h / p.kg), hv = (int)(h / p.vg), ib = (int)b;
-            auto load = [&](const CUtensorMap *m, uint32_t at, int blocks, int64_t t0, int head, uint64_t *bar) {
-                mbar_arrive_expect_tx(bar, blocks * kTcBlock);
-                for (int i = 0; i < blocks; i++)
-                    tma_load_4d(base + at + i * kTcBlock, m, i * 64, (int)t0, head, ib, bar);
-            };
-            auto load_k = [&](int c) {
-                load(&maps.k[pi], L::k + (c & 1) * L::kQ, DQ / 64, first_token(c), hk, &bars.k_full[c & 1]);
+            // tile c of an operand with N buffers of `bytes` from `at`; false: gave up
+            auto load = [&](const CUtensorMap *m, uint32_t at, uint32_t bytes, int N, int c, int head, uint64_t *full,
+                            uint64_t *free) {
+                const int i = c % N, use = c / N;
+                if (use > 0 && !wait(&free[i], use - 1)) return false;
+                mbar_arrive_expect_tx(&full[i], bytes);
+                for (uint32_t j = 0; j < bytes / kTcBlock; j++)
+                    tma_load_4d(base + at + i * bytes + j * kTcBlock, m, j * 64, (int)first_token(c), head, ib, &full[i]);
+                return true;
             };
             int nk = 0, nq = 0, nv = 0;  // loads issued
-            if (chunks > 0) load_k(nk++);
             for (int c = 0; c < chunks; c++) {
+                if (!load(&maps.k[pi], L::k, L::kQ, L::nk, c, hk, bars.k_full, bars.k_free)) break;
+                nk++;
                 if (!STATE_ONLY) {
-                    if (c > 0 && !wait(&bars.q_free, c - 1)) break;
-                    load(&maps.q[pi], L::q, DQ / 64, first_token(c), hq, &bars.q_full);
+                    if (!load(&maps.q[pi], L::q, L::kQ, L::nq, c, hq, bars.q_full, bars.q_free)) break;
                     nq++;
                 }
-                if (c > 0 && !wait(&bars.v_free, c - 1)) break;
-                load(&maps.v[pi], L::v, DV / 64, first_token(c), hv, &bars.v_full);
+                if (!load(&maps.v[pi], L::v, L::kV, L::nv, c, hv, bars.v_full, bars.v_free)) break;
                 nv++;
-                if (c + 1 < chunks) {
-                    if (c > 0 && !wait(&bars.k_free[(c + 1) & 1], (c - 1) >> 1)) break;
-                    load_k(nk++);
-                }
             }
             // no copy is left in flight, whatever happened
-            if (nq > 0) mbar_wait(&bars.q_full, (nq - 1) & 1);
-            if (nv > 0) mbar_wait(&bars.v_full, (nv - 1) & 1);
-            for (int i = std::max(0, nk - 2); i < nk; i++) mbar_wait(&bars.k_full[i & 1], (i >> 1) & 1);
-        }
-    } else if (warp == L::mma_warp) {
-        // ---- MMAs
-        if (lane == 0) {
+            for (int c = max(0, nk - L::nk); c < nk; c++) mbar_wait(&bars.k_full[c % L::nk], (c / L::nk) & 1);
+            for (int c = max(0, nq - L::nq); c < nq; c++) mbar_wait(&bars.q_full[c % L::nq], (c / L::nq) & 1);
+            for (int c = max(0, nv - L::nv); c < nv; c++) mbar_wait(&bars.v_full[c % L::nv], (c / L::nv) & 1);
+        } else if ((warp & 3) == 1 && lane == 0) {
+            // ---- MMAs
             const uint32_t sb = smem_u32(base);
             constexpr uint32_t kIdP = umma_idesc_bf16(kTcC, kTcC, false, false);
             constexpr uint32_t kIdO = umma_idesc_bf16(kTcC, DV, false, true);
             constexpr uint32_t kIdS = umma_idesc_bf16(kTcC, DV, true, true);
-            const uint32_t pb_cols = tmem + (p.rev ? 0u : 64u);  // P in bf16
-            int c = 0;
-            for (; c < chunks; c++) {
-                const uint32_t k_at = sb + L::k + (c & 1) * L::kQ;
-                const bool tail = tokens(first_token(c)) < kTcC;
-                if (!STATE_ONLY) {
-                    if (!wait(&bars.q_full, c) || !wait(&bars.k_full[c & 1], c >> 1)) break;
-                    // P's columns: the last chunk's P V has read them, and (dv = 64) its state's result is out
-                    if (c > 0 && !wait(&bars.o_full, c - 1)) break;
-                    if (DV == 64 && c > 0 && !wait(&bars.ds_free, c - 1)) break;
-                    tcgen05_after();
+            auto p_cols = [&](int c) { return tmem + (c % L::np) * 128; };
+            auto scores = [&](int c) {  // Q K^T of chunk c
+                if (!wait(&bars.q_full[c % L::nq], c / L::nq) || !wait(&bars.k_full[c % L::nk], c / L::nk)) return false;
+                // P V of the chunk that had these columns is done
+                if (c >= L::np && !wait(&bars.o_full, c - L::np)) return false;
+                tcgen05_after();
+                const uint32_t q_at = sb + L::q + (c % L::nq) * L::kQ, k_at = sb + L::k + (c % L::nk) * L::kQ;
 #pragma unroll
-                    for (int k = 0; k < DQ / 16; k++) {
-                        const uint32_t off = (k / 4) * kTcBlock + (k % 4) * 32;
-                        umma_bf16_ss(tmem, umma_desc_sw128(sb + L::q + off, 16), umma_desc_sw128(k_at + off, 16), kIdP,
-                                     k > 0);
-                    }
-                    umma_arrive(&bars.p_full);
-                    if (!wait(&bars.s_ready, c)) break;
-                    if (c > 0 && !wait(&bars.o_free, c - 1)) break;
+                for (int k = 0; k < DQ / 16; k++) {
+                    const uint32_t off = (k / 4) * kTcBlock + (k % 4) * 32;
+                    umma_bf16_ss(p_cols(c), umma_desc_sw128(q_at + off, 16), umma_desc_sw128(k_at + off, 16), kIdP, k > 0);
+                }
+                umma_arrive(&bars.p_full[c % L::np]);
+                return true;
+            };
+            auto body = [&](int c) {
+                const uint32_t q_at = sb + L::q + (c % L::nq) * L::kQ, k_at = sb + L::k + (c % L::nk) * L::kQ,
+                               v_at = sb + L::v + (c % L::nv) * L::kV;
+                if (!STATE_ONLY) {
+                    if (L::np > 1 && c + 1 < chunks && !scores(c + 1)) return false;
+                    if (!wait(&bars.s_ready, c)) return false;
+                    if (c > 0 && !wait(&bars.o_free, c - 1)) return false;
                     tcgen05_after();
 #pragma unroll
                     for (int k = 0; k < DQ / 16; k++)
-                        umma_bf16_ss(tmem + L::o2, umma_desc_sw128(sb + L::q + (k / 4) * kTcBlock + (k % 4) * 32, 16),
+                        umma_bf16_ss(tmem + L::o2, umma_desc_sw128(q_at + (k / 4) * kTcBlock + (k % 4) * 32, 16),
                                      umma_desc_sw128(sb + L::s + k * 2048, DQ * 128), kIdO, k > 0);
-                    umma_arrive(&bars.q_free);
+                    umma_arrive(&bars.q_free[c % L::nq]);
                     umma_arrive(&bars.s_free);
-                    if (!wait(&bars.v_full, c) || !wait(&bars.p_ready, c)) break;
-                    if (tail && !wait(&bars.kw_ready, c)) break;  // v's rows past the end are cleared there
-                    tcgen05_after();
-#pragma unroll
-                    for (int k = 0; k < kTcC / 16; k++)
-                        umma_bf16_ts(tmem + L::o1, pb_cols + k * 8, umma_desc_sw128(sb + L::v + k * 2048, kTcBlock),
-                                     kIdO, k > 0);
-                    umma_arrive(&bars.o_full);
-                } else {
-                    if (!wait(&bars.v_full, c)) break;
                 }
-                if (!wait(&bars.kw_ready, c)) break;
-                if ((STATE_ONLY || DV != 64) && c > 0 && !wait(&bars.ds_free, c - 1)) break;
+                if (!wait(&bars.v_full[c % L::nv], c / L::nv) || !wait(&bars.kw_ready, c)) return false;
+                if (c > 0 && !wait(&bars.ds_free, c - 1)) return false;
                 tcgen05_after();
 #pragma unroll
-                for (int piece = 0; piece < 3; piece++) {
+                for (int piece = 0; piece < NP; piece++) {
                     const uint32_t at = piece == 0 ? k_at : sb + (piece == 1 ? L::mid : L::lo);
 #pragma unroll
                     for (int k = 0; k < kTcC / 16; k++)
-                        umma_bf16_ss(ds_cols, umma_desc_sw128(at + k * 2048, kTcBlock),
-                                     umma_desc_sw128(sb + L::v + k * 2048, kTcBlock), kIdS, piece > 0 || k > 0);
+                        umma_bf16_ss(tmem + L::ds, umma_desc_sw128(at + k * 2048, kTcBlock),
+                                     umma_desc_sw128(v_at + k * 2048, kTcBlock), kIdS, piece > 0 || k > 0);
                 }
                 umma_arrive(&bars.ds_full);
-                umma_arrive(&bars.v_free);
-                umma_arrive(&bars.k_free[c & 1]);
-            }
-            if (c > 0 || chunks > 0) {  // nothing of the tensor cores is left running
-                umma_arrive(&bars.done);
-                mbar_wait(&bars.done, 0);
-            }
+                umma_arrive(&bars.k_free[c % L::nk]);
+                if (!STATE_ONLY) {
+                    if (!wait(&bars.p_ready[c % L::np], c / L::np)) return false;
+                    tcgen05_after();
+                    const uint32_t pb = p_cols(c) + (p.rev ? 0u : 64u);  // P in bf16
+#pragma unroll
+                    for (int k = 0; k < kTcC / 16; k++)
+                        umma_bf16_ts(tmem + L::o1, pb + k * 8, umma_desc_sw128(v_at + k * 2048, kTcBlock), kIdO, k > 0);
+                    umma_arrive(&bars.o_full);
+                }
+                umma_arrive(&bars.v_free[c % L::nv]);
+                if (!STATE_ONLY && L::np == 1 && c + 1 < chunks) return scores(c + 1);
+                return true;
+            };
+            if (chunks > 0 && (STATE_ONLY || scores(0)))
+                for (int c = 0; c < chunks; c++)
+                    if (!body(c)) break;
+            umma_arrive(&bars.done);  // nothing of the tensor cores is left running
+            mbar_wait(&bars.done, 0);
         }
-    } else if (warp < 4) {
-        // ---- P and O: one token a thread
+    } else if (group < L::score_groups) {
+        // ---- P: one token a thread
+        regs_dec<L::score_regs>();
         if (!STATE_ONLY) {
-            const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-            const int row = warp * 32 + lane;
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             float pw[16];
             pw[0] = 1.0f;
             pw[1] = decay_pow(ld, 1.0f);
 #pragma unroll
             for (int i = 2; i < 16; i++) pw[i] = pw[i / 2] * pw[i - i / 2];
             const float b16 = pw[8] * pw[8];
+            for (int c = group; c < chunks; c += L::np) {
+                const int n = tokens(first_token(c));
+                if (!wait_warp(&bars.p_full[group], c / L::np)) break;
+                tcgen05_after();
+                const uint32_t cols = tmem + lanes + group * 128;
+                if (p.rev) attn_scores<true>(cols, warp & 3, lane, n, b16, pw, p.p_scale);
+                else attn_scores<false>(cols, warp & 3, lane, n, b16, pw, p.p_scale);
+                tcgen05_before();
+                mbar_arrive(&bars.p_ready[group]);
+            }
+        }
+    } else if (group == L::output_group) {
+        // ---- O: one token a thread
+        regs_dec<L::output_regs>();
+        if (!STATE_ONLY) {
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const int row = tid & 127;
             const int64_t o_at = b * p.os[0] + h * p.os[2];
             for (int c = 0; c < chunks; c++) {
                 const int64_t t0 = first_token(c);
                 const int n = tokens(t0);
-                if (!wait_warp(&bars.p_full, c)) break;
-                tcgen05_after();
-                if (p.rev) attn_scores<true>(tmem + lanes, warp, lane, n, b16, pw, p.p_scale);
-                else attn_scores<false>(tmem + lanes, warp, lane, n, b16, pw, p.p_scale);
-                tcgen05_before();
-                mbar_arrive(&bars.p_ready);
-
                 const int r = p.rev ? n - 1 - row : row;
                 const float w = row < n ? p.i_scale * decay_pow(ld, (float)(r + 1 - p.shift)) : 0.0f;
                 if (!wait_warp(&bars.o_full, c)) break;
@@ -391,7 +460,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>
             }
             // tokens past the sequence's end in chunks that have none of it
             const int64_t z0 = s0 + (int64_t)chunks * kTcC, nz = max((int64_t)0, s1 - z0) * (p.dv / 8);
-            for (int64_t i = tid; i < nz; i += 128) {
+            for (int64_t i = row; i < nz; i += 128) {
                 const int64_t r = i / (p.dv / 8), at = o_at + (z0 + r) * p.os[1] + (i - r * (p.dv / 8)) * 8;
                 if (p.o_f32) {
                     *reinterpret_cast<float4 *>((float *)p.o + at) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -402,9 +471,10 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>
             }
         }
     } else {
-        // ---- k's pieces and the state: one row of the state a thread, SC of its columns
-        constexpr int NB = L::state_groups, SC = DV / NB;
-        const int at = tid - 128, st = at & 127, c0 = (at >> 7) * SC;
+        // ---- k's pieces and the state: one row of the state a thread, 64 of its columns
+        regs_inc<L::state_regs>();
+        constexpr int NB = L::state_groups, SC = 64;
+        const int at = tid - L::first_state * 128, st = at & 127, c0 = (at >> 7) * SC;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const bool has_row = st < DQ;  // uniform over a warp
         float S[SC];
@@ -428,13 +498,11 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>
         auto put_state = [&] {  // its bf16 copy, the B operand of Q S
             if (has_row) {
 #pragma unroll
-                for (int j = 0; j < SC; j += 8) {
-                    const int col = c0 + j;
-                    *reinterpret_cast<uint4 *>(base + L::s + (col / 64) * (DQ * 128) + st * 128 +
-                                               (((col % 64) / 8) ^ (st & 7)) * 16) =
+                for (int j = 0; j < SC; j += 8)
+                    *reinterpret_cast<uint4 *>(base + L::s + (at >> 7) * (DQ * 128) + st * 128 +
+                                               ((j / 8) ^ (st & 7)) * 16) =
                         make_uint4(pack_bf16(S[j], S[j + 1]), pack_bf16(S[j + 2], S[j + 3]),
                                    pack_bf16(S[j + 4], S[j + 5]), pack_bf16(S[j + 6], S[j + 7]));
-                }
             }
             fence_proxy_async_shared();
             mbar_arrive(&bars.s_ready);
@@ -456,44 +524,39 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>
                 }
                 wn = n;
             }
-            if (!wait_warp(&bars.k_full[c & 1], c >> 1)) break;
-            if (!STATE_ONLY && !wait_warp(&bars.p_full, c)) break;  // Q K^T has read k
+            if (!wait_warp(&bars.k_full[c % L::nk], c / L::nk)) break;
+            if (!STATE_ONLY && !wait_warp(&bars.p_full[c % L::np], c / L::np)) break;  // Q K^T has read k
             if (t0 + n < min(t0 + kTcC, a.T)) {
                 // what lies past the end may be anything: a zero weight does not remove it from v
-                if (!wait_warp(&bars.v_full, c)) break;
-                uint4 *v4 = reinterpret_cast<uint4 *>(base + L::v);
+                if (!wait_warp(&bars.v_full[c % L::nv], c / L::nv)) break;
+                uint4 *v4 = reinterpret_cast<uint4 *>(base + L::v + (c % L::nv) * L::kV);
                 for (int i = at; i < (int)L::kV / 16; i += 128 * NB)
                     if (i / 8 % kTcC >= n) v4[i] = make_uint4(0, 0, 0, 0);
             }
-            uint4 *k4 = reinterpret_cast<uint4 *>(base + L::k + (c & 1) * L::kQ);
-            uint4 *mid4 = reinterpret_cast<uint4 *>(base + L::mid), *lo4 = reinterpret_cast<uint4 *>(base + L::lo);
+            // the last chunk's MMAs (ds_full, below) have read the other pieces
+            uint4 *k4 = reinterpret_cast<uint4 *>(base + L::k + (c % L::nk) * L::kQ);
+            uint4 *mid4 = reinterpret_cast<uint4 *>(base + L::mid);
+            uint4 *lo4 = reinterpret_cast<uint4 *>(base + L::lo);
 #pragma unroll 1
             for (int blk = 0; blk < DQ / 64; blk++) {
                 // four loads first: a thread's vectors do not depend on one another
                 const int i0 = blk * (kTcBlock / 16) + at;  // rows at / 8 + 16 NB it
 #pragma unroll
                 for (int j = 0; j < NW; j += 4) {
-                uint4 x[4];
+                    uint4 x[4];
 #pragma unroll
-                for (int it = 0; it < 4; it++) x[it] = k4[i0 + (j + it) * 128 * NB];
+                    for (int it = 0; it < 4; it++) x[it] = k4[i0 + (j + it) * 128 * NB];
 #pragma unroll
-                for (int it = 0; it < 4; it++) {
-                    const int i = i0 + (j + it) * 128 * NB;
-                    const float w = wk[j + it];
-                    const bool zero = at / 8 + 16 * NB * (j + it) >= n;
-                    uint32_t in[4] = {x[it].x, x[it].y, x[it].z, x[it].w}, hi[4], mid[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float f0 = zero ? 0.0f : bf16_lo(in[e]) * w, f1 = zero ? 0.0f : bf16_hi(in[e]) * w;
-                        hi[e] = pack_bf16(f0, f1);
-                        const float g0 = f0 - bf16_lo(hi[e]), g1 = f1 - bf16_hi(hi[e]);
-                        mid[e] = pack_bf16(g0, g1);
-                        lo[e] = pack_bf16(g0 - bf16_lo(mid[e]), g1 - bf16_hi(mid[e]));
+                    for (int it = 0; it < 4; it++) {
+                        const int i = i0 + (j + it) * 128 * NB;
+                        const bool zero = at / 8 + 16 * NB * (j + it) >= n;
+                        const uint32_t in[4] = {x[it].x, x[it].y, x[it].z, x[it].w};
+                        uint32_t hi[4], mid[4], lo[4];
+                        split_weighted<NP>(in, zero, wk[j + it], hi, mid, lo);
+                        k4[i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        mid4[i] = make_uint4(mid[0], mid[1], mid[2], mid[3]);
+                        if (NP == 3) lo4[i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
-                    k4[i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    mid4[i] = make_uint4(mid[0], mid[1], mid[2], mid[3]);
-                    lo4[i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
                 }
             }
             fence_proxy_async_shared();
@@ -511,7 +574,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>
 #pragma unroll
                 for (int g = 0; g < SC / 32; g++) {
                     uint32_t x[32];
-                    tmem_load32(ds_cols + lanes + c0 + g * 32, x);
+                    tmem_load32(tmem + L::ds + lanes + c0 + g * 32, x);
                     tmem_wait_ld();
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
@@ -544,7 +607,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV>::threads), (TcLayout<DQ, DV>
     }
     tcgen05_before();
     __syncthreads();
-    if (warp == L::mma_warp) {
+    if (warp == 0) {
         tcgen05_after();
         tmem_free(tmem, L::tmem_cols);
     }
@@ -560,14 +623,15 @@ bool operand_map(CUtensorMap *m, const void *base, const int64_t (&st)[3], int d
     return make_tmap_4d_bf16(m, base, dims, strides, 64, kTcC);
 }
 
-template <int DQ, int DV>
+template <int DQ, int DV, int NP>
 bool launch_tc(const AttnArgs &a, const AttnMaps &m, int passes, bool state_only, cudaStream_t s)
 {
-    const size_t smem = TcLayout<DQ, DV>::bytes + 1024;
-    auto kern = state_only ? k_attn_tc<DQ, DV, true> : k_attn_tc<DQ, DV, false>;
+    using L = TcLayout<DQ, DV, NP>;
+    const size_t smem = L::bytes + 1024;
+    auto kern = state_only ? k_attn_tc<DQ, DV, NP, true> : k_attn_tc<DQ, DV, NP, false>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
     count_launches(1);
-    kern<<<dim3((unsigned)(a.B * a.H * a.nseg), (unsigned)passes), TcLayout<DQ, DV>::threads, smem, s>>>(a, m, device_status_ptr());
+    kern<<<dim3((unsigned)(a.B * a.H * a.nseg), (unsigned)passes), L::threads, smem, s>>>(a, m, device_status_ptr());
     return true;
 }
 
@@ -588,21 +652,22 @@ bool attn_tc_applies(const AttnArgs &a, int passes, int dtype)
     return true;
 }
 
-int attn_tc_blocks_per_sm(int dq, int dv) { return width_class(dq) == 64 && width_class(dv) == 64 ? 2 : 1; }
-
 bool attn_tc(const AttnArgs &a, int passes, bool state_only, cudaStream_t s)
 {
-    // passes of one pair of width classes share a launch
+    // passes of one pair of width classes, and with a returned state or without, share a launch
     bool launched[kAttnMaxPasses] = {};
     for (int i = 0; i < passes; i++) {
         if (launched[i]) continue;
         const int dq = width_class(a.p[i].dq), dv = width_class(a.p[i].dv);
+        const bool exact_state = a.p[i].s_out != nullptr;
         AttnArgs b = a;
         AttnMaps m = {};
         int n = 0;
         for (int j = i; j < passes; j++) {
             const AttnPass &p = a.p[j];
-            if (launched[j] || width_class(p.dq) != dq || width_class(p.dv) != dv) continue;
+            if (launched[j] || width_class(p.dq) != dq || width_class(p.dv) != dv ||
+                (p.s_out != nullptr) != exact_state)
+                continue;
             if (!operand_map(&m.q[n], p.q, p.qs, p.dq, a.T, a.H / p.qg, a.B) ||
                 !operand_map(&m.k[n], p.k, p.ks, p.dq, a.T, a.H / p.kg, a.B) ||
                 !operand_map(&m.v[n], p.v, p.vs, p.dv, a.T, a.H / p.vg, a.B))
@@ -610,10 +675,14 @@ bool attn_tc(const AttnArgs &a, int passes, bool state_only, cudaStream_t s)
             launched[j] = true;
             b.p[n++] = p;
         }
-        const bool ok = dq == 64 ? (dv == 64 ? launch_tc<64, 64>(b, m, n, state_only, s)
-                                             : launch_tc<64, 128>(b, m, n, state_only, s))
-                                 : (dv == 64 ? launch_tc<128, 64>(b, m, n, state_only, s)
-                                             : launch_tc<128, 128>(b, m, n, state_only, s));
+        auto run = [&](auto np) {
+            constexpr int NP = decltype(np)::value;
+            return dq == 64 ? (dv == 64 ? launch_tc<64, 64, NP>(b, m, n, state_only, s)
+                                        : launch_tc<64, 128, NP>(b, m, n, state_only, s))
+                            : (dv == 64 ? launch_tc<128, 64, NP>(b, m, n, state_only, s)
+                                        : launch_tc<128, 128, NP>(b, m, n, state_only, s));
+        };
+        const bool ok = exact_state ? run(std::integral_constant<int, 3>()) : run(std::integral_constant<int, 2>());
         if (!ok) return false;
     }
     return true;
