@@ -504,8 +504,8 @@ int at_check(const char *what, const lifb_leaky_attn *p)
         return at_fail(LIFB_ERR_INVALID_ARGUMENT, what, "H must be a multiple of Hk");
     if (p->Dk > kAttnMaxDim || p->Dv > kAttnMaxDim)
         return at_fail(LIFB_ERR_UNSUPPORTED, what, "head widths up to 128");
-    if (p->T >= (int64_t(1) << 31) || p->B * p->H >= (int64_t(1) << 16))
-        return at_fail(LIFB_ERR_UNSUPPORTED, what, "needs T < 2^31 and B * H < 2^16");
+    if (p->T >= (int64_t(1) << 31) - 256 || p->B * p->H >= (int64_t(1) << 16))
+        return at_fail(LIFB_ERR_UNSUPPORTED, what, "needs T < 2^31 - 256 and B * H < 2^16");
     return LIFB_OK;
 }
 

@@ -104,62 +104,59 @@ __device__ __forceinline__ void regs_dec()
 
 // This thread's row of P: scores from tensor memory, times p_scale * b^distance
 // where the other token is not in the future (and is one of the n), else zero;
-// packed to bf16 into 64 of the same 128 columns.  Powers of b (pw[i] = b^i) run
-// from the diagonal outwards.  Forward passes walk the columns
+// packed to bf16 into 64 of the same 128 columns.  Powers of b run from the
+// diagonal outwards (pw: of 16 columns, in their order).  Forward passes walk the columns
 // downwards and pack into the upper half, backward passes the other way round, so
 // that nothing unread is overwritten.
 template <bool REV>
-__device__ __forceinline__ void attn_scores(uint32_t lane_cols, int warp, int lane, int n, float b16,
-                                            const float (&pw)[16], float p_scale)
+__device__ __forceinline__ void attn_scores(uint32_t lane_cols, int warp, int lane, int n, float b, float b16,
+                                            const uint64_t (&pw)[8], float p_scale)
 {
     float d = 0.0f;
     auto col = [&](int s) { return (REV ? s : 7 - s) * 16; };
+    auto out = [&](int s) { return lane_cols + (REV ? 0 : 64) + col(s) / 2; };
     uint32_t x[2][16];
     const int first = 2 * (REV ? warp : 3 - warp);  // before it all columns are on the other side of the diagonal
     tmem_load16(lane_cols + col(first), x[0]);
     {
         const uint32_t zero[8] = {};
-        for (int s = 0; s < first; s++) tmem_store8(lane_cols + (REV ? 0 : 64) + col(s) / 2, zero);
+        for (int s = 0; s < first; s++) tmem_store8(out(s), zero);
     }
-    // the pair of column blocks with the diagonal, then the ones past it
-#pragma unroll
-    for (int half = 0; half < 2; half++) {
-        tmem_wait_ld();
-        if (half == 0) tmem_load16(lane_cols + col(first + 1), x[1]);
-        else if (first < 6) tmem_load16(lane_cols + col(first + 2), x[0]);
-        uint32_t w[8];
-        float y[16];
-#pragma unroll
-        for (int t = 0; t < 16; t++) {
-            const int e = REV ? t : 15 - t, c = (REV ? half : 1 - half) * 16 + e;  // of the pair's 32 columns
-            d = c == lane ? p_scale : d * pw[1];
-            y[e] = (REV ? c >= lane : c <= lane) ? __uint_as_float(x[half][e]) * d : 0.0f;
-            if (REV && warp * 32 + c >= n) y[e] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
-        tmem_store8(lane_cols + (REV ? 0 : 64) + col(first + half) / 2, w);
-    }
-    d *= pw[1];  // of the next block's nearest column
+    // the two column blocks with the diagonal, then the ones past it, two at a time
 #pragma unroll 1
-    for (int s = first + 2; s < 8; s += 2) {
+    for (int s = first; s < 8; s += 2) {
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             tmem_wait_ld();
             if (half == 0) tmem_load16(lane_cols + col(s + 1), x[1]);
             else if (s < 6) tmem_load16(lane_cols + col(s + 2), x[0]);
             uint32_t w[8];
-            float y[16];
+            if (s == first) {
 #pragma unroll
-            for (int t = 0; t < 16; t++) {
-                const int e = REV ? t : 15 - t;
-                y[e] = __uint_as_float(x[half][e]) * (d * pw[t]);
-                if (REV && n < kTcC && col(s + half) + e >= n) y[e] = 0.0f;
+                for (int t = 0; t < 16; t++) {
+                    const int e = REV ? t : 15 - t, c = (REV ? half : 1 - half) * 16 + e;  // of the pair's 32
+                    d = c == lane ? p_scale : d * b;
+                    const bool on = (REV ? c >= lane : c <= lane) && !(REV && warp * 32 + c >= n);
+                    x[half][e] = on ? __float_as_uint(__uint_as_float(x[half][e]) * d) : 0u;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[i] = pack2_bf16(two(x[half][2 * i], x[half][2 * i + 1]));
+                if (half == 1) d *= b;  // of the next block's nearest column
+            } else {
+                const uint64_t dd = two(d, d);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    w[i] = pack2_bf16(mul2(two(x[half][2 * i], x[half][2 * i + 1]), mul2(pw[i], dd)));
+                if (REV && n < kTcC) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if (col(s + half) + 2 * i >= n) w[i] = 0;
+                        else if (col(s + half) + 2 * i + 1 >= n) w[i] &= 0xFFFFu;
+                    }
+                }
+                d *= b16;
             }
-            d *= b16;
-#pragma unroll
-            for (int i = 0; i < 8; i++) w[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
-            tmem_store8(lane_cols + (REV ? 0 : 64) + col(s + half) / 2, w);
+            tmem_store8(out(s + half), w);
         }
     }
     tmem_wait_st();
@@ -186,37 +183,47 @@ __device__ __forceinline__ void quad_transpose(uint32_t (&m)[4][4], int lane)
     }
 }
 
-// w * x for eight bf16 elements x (four words) as NP bf16 pieces; `zero`: x is not a
-// token of the sequence and may be anything.
-// Two pieces: with w = wh + wm in bf16, hi = x wh rounded, and what that rounding
-// dropped is exact in bf16 (the product has 16 bits), so mid = x wm + it.
+// A token's weight, as the pieces of its weighted key need it: two bf16 values
+// (each twice in a word) whose sum is w to 2^-18, or w itself.
 template <int NP>
-__device__ __forceinline__ void split_weighted(const uint32_t (&in)[4], bool zero, float w, uint32_t (&hi)[4],
-                                               uint32_t (&mid)[4], uint32_t (&lo)[4])
-{
-    if constexpr (NP == 2) {
-        const __nv_bfloat16 w1 = __float2bfloat16_rn(w), w2 = __float2bfloat16_rn(w - __bfloat162float(w1));
-        const __nv_bfloat162 wh = __halves2bfloat162(w1, w1), wm = __halves2bfloat162(w2, w2);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint32_t xe = zero ? 0u : in[e];
-            const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&xe);
-            const __nv_bfloat162 h = __hmul2_rn(x, wh);
-            const __nv_bfloat162 m = __hfma2(x, wm, __hfma2(x, wh, __hneg2(h)));
-            hi[e] = *reinterpret_cast<const uint32_t *>(&h);
-            mid[e] = *reinterpret_cast<const uint32_t *>(&m);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float f0 = zero ? 0.0f : bf16_lo(in[e]) * w, f1 = zero ? 0.0f : bf16_hi(in[e]) * w;
-            hi[e] = pack_bf16(f0, f1);
-            const float g0 = f0 - bf16_lo(hi[e]), g1 = f1 - bf16_hi(hi[e]);
-            mid[e] = pack_bf16(g0, g1);
-            lo[e] = pack_bf16(g0 - bf16_lo(mid[e]), g1 - bf16_hi(mid[e]));
-        }
+struct TokenWeight {
+    uint32_t wh, wm;
+    __device__ __forceinline__ void set(float w)
+    {
+        wh = NP == 2 ? pack_bf16(w, w) : __float_as_uint(w);
+        wm = NP == 2 ? pack_bf16(w - bf16_lo(wh), w - bf16_lo(wh)) : 0;
     }
-}
+    // w * x for eight bf16 elements x (four words) as NP bf16 pieces.  Two pieces: hi =
+    // x wh rounded; what that dropped is exact in bf16 (the product has 16 bits), so
+    // mid = x wm + it.
+    __device__ __forceinline__ void split(const uint4 &x4, uint4 &hi4, uint4 &mid4, uint4 &lo4) const
+    {
+        const uint32_t in[4] = {x4.x, x4.y, x4.z, x4.w};
+        uint32_t hi[4], mid[4], lo[4] = {};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if constexpr (NP == 2) {
+                const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&in[e]);
+                const __nv_bfloat162 h2 = *reinterpret_cast<const __nv_bfloat162 *>(&wh);
+                const __nv_bfloat162 m2 = *reinterpret_cast<const __nv_bfloat162 *>(&wm);
+                const __nv_bfloat162 h = __hmul2_rn(x, h2);
+                const __nv_bfloat162 m = __hfma2(x, m2, __hfma2(x, h2, __hneg2(h)));
+                hi[e] = *reinterpret_cast<const uint32_t *>(&h);
+                mid[e] = *reinterpret_cast<const uint32_t *>(&m);
+            } else {
+                const float w = __uint_as_float(wh);
+                const float f0 = bf16_lo(in[e]) * w, f1 = bf16_hi(in[e]) * w;
+                hi[e] = pack_bf16(f0, f1);
+                const float g0 = f0 - bf16_lo(hi[e]), g1 = f1 - bf16_hi(hi[e]);
+                mid[e] = pack_bf16(g0, g1);
+                lo[e] = pack_bf16(g0 - bf16_lo(mid[e]), g1 - bf16_hi(mid[e]));
+            }
+        }
+        hi4 = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        mid4 = make_uint4(mid[0], mid[1], mid[2], mid[3]);
+        lo4 = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+};
 
 template <int DQ, int DV, int NP, bool STATE_ONLY>
 __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
@@ -237,10 +244,11 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     const int64_t len = attn_length(a.lengths, b, a.T);
     const float ld = a.log_decay[h];
     const int64_t seg = p.rev ? a.nseg - 1 - u : u;  // in time
-    const int64_t s0 = seg * a.seg_tokens, s1 = min(a.T, s0 + a.seg_tokens);
-    const int chunks = (int)(max((int64_t)0, min(s1, len) - s0 + kTcC - 1) / kTcC);  // with tokens in them
-    auto first_token = [&](int c) { return s0 + (int64_t)(p.rev ? chunks - 1 - c : c) * kTcC; };
-    auto tokens = [&](int64_t t0) { return (int)min((int64_t)kTcC, min(s1, len) - t0); };
+    // T < 2^31 - 2^7: a token's number, and one chunk past the last, fit an int
+    const int s0 = (int)(seg * a.seg_tokens), s1 = (int)min(a.T, seg * a.seg_tokens + a.seg_tokens);
+    const int end = min(s1, (int)len);                         // of the tokens that count
+    const int chunks = max(0, end - s0 + kTcC - 1) / kTcC;     // with tokens in them
+    const int t_first = p.rev ? s0 + (chunks - 1) * kTcC : s0, t_step = p.rev ? -kTcC : kTcC;
 
     if (warp == 0) tmem_alloc(&tmem_slot, L::tmem_cols);
     if (tid == 32) {
@@ -295,7 +303,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 if (use > 0 && !wait(&free[i], use - 1)) return false;
                 mbar_arrive_expect_tx(&full[i], bytes);
                 for (uint32_t j = 0; j < bytes / kTcBlock; j++)
-                    tma_load_4d(base + at + i * bytes + j * kTcBlock, m, j * 64, (int)first_token(c), head, ib, &full[i]);
+                    tma_load_4d(base + at + i * bytes + j * kTcBlock, m, j * 64, t_first + c * t_step, head, ib, &full[i]);
                 return true;
             };
             int nk = 0, nq = 0, nv = 0;  // loads issued
@@ -326,10 +334,11 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 if (c >= L::np && !wait(&bars.o_full, c - L::np)) return false;
                 tcgen05_after();
                 const uint32_t q_at = sb + L::q + (c % L::nq) * L::kQ, k_at = sb + L::k + (c % L::nk) * L::kQ;
+                const uint64_t dq = umma_desc_sw128(q_at, 16), dk = umma_desc_sw128(k_at, 16);
 #pragma unroll
                 for (int k = 0; k < DQ / 16; k++) {
-                    const uint32_t off = (k / 4) * kTcBlock + (k % 4) * 32;
-                    umma_bf16_ss(p_cols(c), umma_desc_sw128(q_at + off, 16), umma_desc_sw128(k_at + off, 16), kIdP, k > 0);
+                    const uint32_t off = ((k / 4) * kTcBlock + (k % 4) * 32) >> 4;
+                    umma_bf16_ss(p_cols(c), dq + off, dk + off, kIdP, k > 0);
                 }
                 umma_arrive(&bars.p_full[c % L::np]);
                 return true;
@@ -342,23 +351,23 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                     if (!wait(&bars.s_ready, c)) return false;
                     if (c > 0 && !wait(&bars.o_free, c - 1)) return false;
                     tcgen05_after();
+                    const uint64_t dq = umma_desc_sw128(q_at, 16), ds = umma_desc_sw128(sb + L::s, DQ * 128);
 #pragma unroll
                     for (int k = 0; k < DQ / 16; k++)
-                        umma_bf16_ss(tmem + L::o2, umma_desc_sw128(q_at + (k / 4) * kTcBlock + (k % 4) * 32, 16),
-                                     umma_desc_sw128(sb + L::s + k * 2048, DQ * 128), kIdO, k > 0);
+                        umma_bf16_ss(tmem + L::o2, dq + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4), ds + k * 128, kIdO, k > 0);
                     umma_arrive(&bars.q_free[c % L::nq]);
                     umma_arrive(&bars.s_free);
                 }
                 if (!wait(&bars.v_full[c % L::nv], c / L::nv) || !wait(&bars.kw_ready, c)) return false;
                 if (c > 0 && !wait(&bars.ds_free, c - 1)) return false;
                 tcgen05_after();
-#pragma unroll
+                const uint64_t dv = umma_desc_sw128(v_at, kTcBlock);
+#pragma unroll 1
                 for (int piece = 0; piece < NP; piece++) {
-                    const uint32_t at = piece == 0 ? k_at : sb + (piece == 1 ? L::mid : L::lo);
+                    const uint64_t dk = umma_desc_sw128(piece == 0 ? k_at : sb + (piece == 1 ? L::mid : L::lo), kTcBlock);
 #pragma unroll
                     for (int k = 0; k < kTcC / 16; k++)
-                        umma_bf16_ss(tmem + L::ds, umma_desc_sw128(at + k * 2048, kTcBlock),
-                                     umma_desc_sw128(v_at + k * 2048, kTcBlock), kIdS, piece > 0 || k > 0);
+                        umma_bf16_ss(tmem + L::ds, dk + k * 128, dv + k * 128, kIdS, piece > 0 || k > 0);
                 }
                 umma_arrive(&bars.ds_full);
                 umma_arrive(&bars.k_free[c % L::nk]);
@@ -368,7 +377,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                     const uint32_t pb = p_cols(c) + (p.rev ? 0u : 64u);  // P in bf16
 #pragma unroll
                     for (int k = 0; k < kTcC / 16; k++)
-                        umma_bf16_ts(tmem + L::o1, pb + k * 8, umma_desc_sw128(v_at + k * 2048, kTcBlock), kIdO, k > 0);
+                        umma_bf16_ts(tmem + L::o1, pb + k * 8, dv + k * 128, kIdO, k > 0);
                     umma_arrive(&bars.o_full);
                 }
                 umma_arrive(&bars.v_free[c % L::nv]);
@@ -386,19 +395,27 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
         regs_dec<L::score_regs>();
         if (!STATE_ONLY) {
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            float pw[16];
-            pw[0] = 1.0f;
-            pw[1] = decay_pow(ld, 1.0f);
+            const float b1 = decay_pow(ld, 1.0f);
+            uint64_t pw[8];
+            float b16 = 1.0f;
+            {
+                float f[16];
 #pragma unroll
-            for (int i = 2; i < 16; i++) pw[i] = pw[i / 2] * pw[i - i / 2];
-            const float b16 = pw[8] * pw[8];
+                for (int i = 0; i < 16; i++) {
+                    f[i] = b16;
+                    b16 *= b1;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    pw[i] = p.rev ? two(f[2 * i], f[2 * i + 1]) : two(f[15 - 2 * i], f[14 - 2 * i]);
+            }
             for (int c = group; c < chunks; c += L::np) {
-                const int n = tokens(first_token(c));
+                const int n = min(kTcC, end - (t_first + c * t_step));
                 if (!wait_warp(&bars.p_full[group], c / L::np)) break;
                 tcgen05_after();
                 const uint32_t cols = tmem + lanes + group * 128;
-                if (p.rev) attn_scores<true>(cols, warp & 3, lane, n, b16, pw, p.p_scale);
-                else attn_scores<false>(cols, warp & 3, lane, n, b16, pw, p.p_scale);
+                if (p.rev) attn_scores<true>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
+                else attn_scores<false>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
                 tcgen05_before();
                 mbar_arrive(&bars.p_ready[group]);
             }
@@ -411,55 +428,56 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             const int row = tid & 127;
             const int64_t o_at = b * p.os[0] + h * p.os[2];
             for (int c = 0; c < chunks; c++) {
-                const int64_t t0 = first_token(c);
-                const int n = tokens(t0);
+                const int t0 = t_first + c * t_step, n = min(kTcC, end - t0);
                 const int r = p.rev ? n - 1 - row : row;
                 const float w = row < n ? p.i_scale * decay_pow(ld, (float)(r + 1 - p.shift)) : 0.0f;
                 if (!wait_warp(&bars.o_full, c)) break;
                 tcgen05_after();
-                const bool in = t0 + row < s1;
-                const int64_t at = o_at + (t0 + row) * p.os[1];
+                const uint64_t ww = two(w, w);
+                const bool full = s1 - t0 >= kTcC && p.dv == DV;
 #pragma unroll 1
-                for (int g = 0; g < DV / 32; g++) {
-                    uint32_t x[32], y[2][16];
-                    tmem_load32(tmem + lanes + L::o1 + g * 32, x);
-                    tmem_load16(tmem + lanes + L::o2 + g * 32, y[0]);
-                    tmem_load16(tmem + lanes + L::o2 + g * 32 + 16, y[1]);
+                for (int g = 0; g < DV; g += 32) {
+                    uint32_t x[32], y[32];
+                    tmem_load32(tmem + lanes + L::o1 + g, x);
+                    tmem_load32(tmem + lanes + L::o2 + g, y);
                     tmem_wait_ld();
-                    if (g == DV / 32 - 1) {
+                    if (g == DV - 32) {
                         tcgen05_before();
                         mbar_arrive(&bars.o_free);
                     }
-                    float o[32];
+                    uint64_t o[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e++)
-                        o[e] = row < n ? fmaf(w, __uint_as_float(y[e / 16][e % 16]), __uint_as_float(x[e])) : 0.0f;
-                    if (in && p.o_f32) {
-                        float *dst = (float *)p.o + at + g * 32;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            if (g * 32 + e < p.dv)
-                                *reinterpret_cast<float4 *>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                    } else if (!p.o_f32) {
+                    for (int e = 0; e < 16; e++) {
+                        o[e] = fma2(ww, two(y[2 * e], y[2 * e + 1]), two(x[2 * e], x[2 * e + 1]));
+                        if (row >= n) o[e] = 0;
+                    }
+                    if (!p.o_f32) {
                         // four lanes hold four rows of 64 bytes: transposed among them, so that they
                         // write 64 consecutive bytes of one row at a time
                         uint32_t m[4][4];
 #pragma unroll
-                        for (int e = 0; e < 16; e++) m[e / 4][e % 4] = pack_bf16(o[2 * e], o[2 * e + 1]);
+                        for (int e = 0; e < 16; e++) m[e / 4][e % 4] = pack2_bf16(o[e]);
                         quad_transpose(m, lane);
+                        const int col = g + (lane & 3) * 8;
+                        __nv_bfloat16 *dst = (__nv_bfloat16 *)p.o + o_at + (int64_t)(t0 + (row & ~3)) * p.os[1] + col;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int r4 = (row & ~3) + i, col = g * 32 + (lane & 3) * 8;
-                            if (t0 + r4 < s1 && col < p.dv)
-                                *reinterpret_cast<uint4 *>((__nv_bfloat16 *)p.o + o_at + (t0 + r4) * p.os[1] + col) =
+                        for (int i = 0; i < 4; i++)
+                            if (full || (t0 + (row & ~3) + i < s1 && col < p.dv))
+                                *reinterpret_cast<uint4 *>(dst + i * p.os[1]) =
                                     make_uint4(m[i][0], m[i][1], m[i][2], m[i][3]);
-                        }
+                    } else if (t0 + row < s1) {
+                        float *dst = (float *)p.o + o_at + (int64_t)(t0 + row) * p.os[1] + g;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2)
+                            if (g + 2 * e < p.dv)
+                                *reinterpret_cast<ulonglong2 *>(dst + 2 * e) = make_ulonglong2(o[e], o[e + 1]);
                     }
                     __syncwarp();
                 }
             }
             // tokens past the sequence's end in chunks that have none of it
-            const int64_t z0 = s0 + (int64_t)chunks * kTcC, nz = max((int64_t)0, s1 - z0) * (p.dv / 8);
+            const int z0 = s0 + chunks * kTcC;
+            const int64_t nz = (int64_t)max(0, s1 - z0) * (p.dv / 8);
             for (int64_t i = row; i < nz; i += 128) {
                 const int64_t r = i / (p.dv / 8), at = o_at + (z0 + r) * p.os[1] + (i - r * (p.dv / 8)) * 8;
                 if (p.o_f32) {
@@ -477,7 +495,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
         const int at = tid - L::first_state * 128, st = at & 127, c0 = (at >> 7) * SC;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const bool has_row = st < DQ;  // uniform over a warp
-        float S[SC];
+        uint64_t S[SC / 2];  // pairs of columns
         const int64_t mat = (int64_t)p.dq * p.dv;
         {
             const float *s_in = nullptr;
@@ -492,8 +510,13 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 }
             }
 #pragma unroll
-            for (int j = 0; j < SC; j++)
-                S[j] = s_in && st < p.dq && c0 + j < p.dv ? s_in[st * row + (c0 + j) * col] : 0.0f;
+            for (int j = 0; j < SC; j += 2) {
+                float f[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (s_in && st < p.dq && c0 + j + e < p.dv) f[e] = s_in[st * row + (c0 + j + e) * col];
+                S[j / 2] = two(f[0], f[1]);
+            }
         }
         auto put_state = [&] {  // its bf16 copy, the B operand of Q S
             if (has_row) {
@@ -501,8 +524,8 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 for (int j = 0; j < SC; j += 8)
                     *reinterpret_cast<uint4 *>(base + L::s + (at >> 7) * (DQ * 128) + st * 128 +
                                                ((j / 8) ^ (st & 7)) * 16) =
-                        make_uint4(pack_bf16(S[j], S[j + 1]), pack_bf16(S[j + 2], S[j + 3]),
-                                   pack_bf16(S[j + 4], S[j + 5]), pack_bf16(S[j + 6], S[j + 7]));
+                        make_uint4(pack2_bf16(S[j / 2]), pack2_bf16(S[j / 2 + 1]), pack2_bf16(S[j / 2 + 2]),
+                                   pack2_bf16(S[j / 2 + 3]));
             }
             fence_proxy_async_shared();
             mbar_arrive(&bars.s_ready);
@@ -511,22 +534,21 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
         const DecayFactor full(ld, kTcC);
         // the weights of the tokens whose columns this thread scales
         constexpr int NW = 8 / NB;
-        float wk[NW];
+        TokenWeight<NP> wk[NW];
         int wn = -1;  // the chunk size that they are for
         for (int c = 0; c < chunks; c++) {
-            const int64_t t0 = first_token(c);
-            const int n = tokens(t0);
+            const int t0 = t_first + c * t_step, n = min(kTcC, end - t0);
             if (n != wn) {  // the first chunk, the one with the sequence's end, and the one after it
 #pragma unroll
                 for (int i = 0; i < NW; i++) {
                     const int row = at / 8 + 16 * NB * i, r = p.rev ? n - 1 - row : row;
-                    wk[i] = row < n ? p.w_scale * decay_pow(ld, (float)(n - 1 - r + p.shift)) : 0.0f;
+                    wk[i].set(row < n ? p.w_scale * decay_pow(ld, (float)(n - 1 - r + p.shift)) : 0.0f);
                 }
                 wn = n;
             }
             if (!wait_warp(&bars.k_full[c % L::nk], c / L::nk)) break;
             if (!STATE_ONLY && !wait_warp(&bars.p_full[c % L::np], c / L::np)) break;  // Q K^T has read k
-            if (t0 + n < min(t0 + kTcC, a.T)) {
+            if (t0 + n < min(t0 + kTcC, (int)a.T)) {
                 // what lies past the end may be anything: a zero weight does not remove it from v
                 if (!wait_warp(&bars.v_full[c % L::nv], c / L::nv)) break;
                 uint4 *v4 = reinterpret_cast<uint4 *>(base + L::v + (c % L::nv) * L::kV);
@@ -545,29 +567,27 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 for (int j = 0; j < NW; j += 4) {
                     uint4 x[4];
 #pragma unroll
-                    for (int it = 0; it < 4; it++) x[it] = k4[i0 + (j + it) * 128 * NB];
+                    for (int it = 0; it < 4; it++) {
+                        x[it] = k4[i0 + (j + it) * 128 * NB];
+                        // not a token: anything may be there
+                        if (n < kTcC && at / 8 + 16 * NB * (j + it) >= n) x[it] = make_uint4(0, 0, 0, 0);
+                    }
 #pragma unroll
                     for (int it = 0; it < 4; it++) {
                         const int i = i0 + (j + it) * 128 * NB;
-                        const bool zero = at / 8 + 16 * NB * (j + it) >= n;
-                        const uint32_t in[4] = {x[it].x, x[it].y, x[it].z, x[it].w};
-                        uint32_t hi[4], mid[4], lo[4];
-                        split_weighted<NP>(in, zero, wk[j + it], hi, mid, lo);
-                        k4[i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        mid4[i] = make_uint4(mid[0], mid[1], mid[2], mid[3]);
-                        if (NP == 3) lo4[i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        uint4 hi, mid, lo;
+                        wk[j + it].split(x[it], hi, mid, lo);
+                        k4[i] = hi;
+                        mid4[i] = mid;
+                        if (NP == 3) lo4[i] = lo;
                     }
                 }
             }
             fence_proxy_async_shared();
             mbar_arrive(&bars.kw_ready);
 
-            float bn_hi = full.hi, bn_lo = full.lo;
-            if (n != kTcC) {
-                const DecayFactor f(ld, n);
-                bn_hi = f.hi;
-                bn_lo = f.lo;
-            }
+            const DecayFactor bn = n == kTcC ? full : DecayFactor(ld, n);
+            const uint64_t bn_hi = two(bn.hi, bn.hi), bn_lo = two(bn.lo, bn.lo);
             if (!wait_warp(&bars.ds_full, c)) break;
             tcgen05_after();
             if (has_row) {
@@ -577,9 +597,9 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                     tmem_load32(tmem + L::ds + lanes + c0 + g * 32, x);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        float &z = S[g * 32 + e];
-                        z = fmaf(z, bn_hi, fmaf(z, bn_lo, __uint_as_float(x[e])));
+                    for (int e = 0; e < 16; e++) {
+                        uint64_t &z = S[g * 16 + e];
+                        z = fma2(z, bn_hi, fma2(z, bn_lo, two(x[2 * e], x[2 * e + 1])));
                     }
                 }
             }
@@ -601,8 +621,13 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
         }
         if (s_out && st < p.dq) {
 #pragma unroll
-            for (int j = 0; j < SC; j++)
-                if (c0 + j < p.dv) s_out[st * row + (c0 + j) * col] = S[j];
+            for (int j = 0; j < SC; j += 2) {
+                float f[2];
+                both(S[j / 2], f[0], f[1]);
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (c0 + j + e < p.dv) s_out[st * row + (c0 + j + e) * col] = f[e];
+            }
         }
     }
     tcgen05_before();
