@@ -64,29 +64,34 @@ struct AttnMaps {
 template <int DQ, int DV, int NP>
 struct TcLayout {
     static constexpr uint32_t kQ = DQ / 64 * kTcBlock, kV = DV / 64 * kTcBlock, kS = DV / 64 * DQ * 128;
-    static constexpr int nq = DQ == 64 || DV == 64 ? 2 : 1, nv = DQ == 128 && NP == 3 ? 1 : 2, nk = 2;
-    static constexpr uint32_t mid = 0, lo = kQ, k = (NP - 1) * kQ, q = k + nk * kQ, v = q + nq * kQ, s = v + nv * kV,
+    static constexpr bool small = DQ == 64 && DV == 64;
+    static constexpr int np = small ? 2 : 1;  // P's in flight, in tensor memory
+    // tiles in flight: of q one more than P's, so that the next Q K^T need not wait for
+    // Q S (where three pieces of 128 columns leave no room for it, it does)
+    static constexpr int nq = DQ == 128 && DV == 128 && NP == 3 ? 1 : np + 1, nk = np;
+    static constexpr int nv = DQ == 128 && (DV == 128 || NP == 3) ? 1 : 2, nm = small ? 2 : 1;  // nm: sets of pieces
+    static constexpr bool early = nq > np;
+    static constexpr uint32_t pieces = 0, k = nm * NP * kQ, q = k + nk * kQ, v = q + nq * kQ, s = v + nv * kV,
                               bytes = s + kS;
     static_assert(bytes + 1024 + 512 <= 227 * 1024, "tiles fit an SM");
     // columns of tensor memory
-    static constexpr int np = DV == 64 ? 2 : 1;  // P's in flight
-    static_assert(np <= nq && np <= nk, "Q K^T of the next chunk does not wait for this one's other MMAs");
     static constexpr uint32_t tmem_cols = 512, o1 = np * 128, o2 = o1 + DV, ds = o2 + DV;
     static_assert(ds + DV <= tmem_cols, "accumulators fit");
     // warpgroups: scores, output, state, and one with the loading and the issuing warp
     static constexpr int score_groups = np, state_groups = DV / 64;
     static constexpr int output_group = score_groups, first_state = score_groups + 1,
                          last_group = first_state + state_groups;
-    static constexpr int threads = 128 * (last_group + 1);
+    static constexpr int threads = 640;  // five groups; one of them idles at dq = 128, dv = 64
     // registers a thread: 640 threads are launched with 96 each, 480 for the five groups
     static constexpr int score_regs = 80, output_regs = 80, state_regs = DV == 64 ? 152 : 128, last_regs = 64;
-    static_assert(threads == 640 && score_groups * score_regs + output_regs + state_groups * state_regs + last_regs <= 480,
+    static constexpr int idle_groups = 5 - (score_groups + 1 + state_groups + 1);
+    static_assert(score_groups * score_regs + output_regs + state_groups * state_regs + last_regs + idle_groups * 24 <= 480,
                   "no more registers than the block was launched with");
 };
 
 struct TcBars {
-    uint64_t q_full[2], q_free[2], k_full[2], k_free[2], v_full[2], v_free[2];
-    uint64_t p_full[2], p_ready[2], kw_ready, s_ready, s_free, o_full, o_free, ds_full, ds_free, done;
+    uint64_t q_full[3], q_free[3], k_full[2], k_free[2], v_full[2], v_free[2];
+    uint64_t p_full[2], p_ready[2], kw_ready[2], s_ready, s_free, o_full, o_free, ds_full, ds_free, done;
 };
 
 template <int N>
@@ -162,25 +167,12 @@ __device__ __forceinline__ void attn_scores(uint32_t lane_cols, int warp, int la
     tmem_wait_st();
 }
 
-// A 4 x 4 transposition of 16-byte elements among the four lanes of a quad:
-// m[i] of lane j becomes m[j] of lane i.
-__device__ __forceinline__ void quad_transpose(uint32_t (&m)[4][4], int lane)
+// 32 bytes, a whole sector, in one store.
+__device__ __forceinline__ void store_32_bytes(void *p, const uint32_t (&m)[8])
 {
-#pragma unroll
-    for (int step = 1; step <= 2; step *= 2) {
-        const bool up = lane & step;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (i & step) continue;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t send = up ? m[i][e] : m[i + step][e];
-                const uint32_t got = __shfl_xor_sync(~0u, send, step);
-                if (up) m[i][e] = got;
-                else m[i + step][e] = got;
-            }
-        }
-    }
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(m[0]), "r"(m[1]), "r"(m[2]),
+                 "r"(m[3]), "r"(m[4]), "r"(m[5]), "r"(m[6]), "r"(m[7])
+                 : "memory");
 }
 
 // A token's weight, as the pieces of its weighted key need it: two bf16 values
@@ -252,17 +244,19 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
 
     if (warp == 0) tmem_alloc(&tmem_slot, L::tmem_cols);
     if (tid == 32) {
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 3; i++) {
             mbar_init(&bars.q_full[i], 1);
             mbar_init(&bars.q_free[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
             mbar_init(&bars.k_full[i], 1);
-            mbar_init(&bars.k_free[i], 1);
+            mbar_init(&bars.k_free[i], (STATE_ONLY ? 0 : 1) + 128 * L::state_groups);
             mbar_init(&bars.v_full[i], 1);
             mbar_init(&bars.v_free[i], 1);
             mbar_init(&bars.p_full[i], 1);
             mbar_init(&bars.p_ready[i], 128);
+            mbar_init(&bars.kw_ready[i], 128 * L::state_groups);
         }
-        mbar_init(&bars.kw_ready, 128 * L::state_groups);
         mbar_init(&bars.s_ready, 128 * L::state_groups);
         mbar_init(&bars.s_free, 1);
         mbar_init(&bars.o_full, 1);
@@ -328,65 +322,74 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             constexpr uint32_t kIdO = umma_idesc_bf16(kTcC, DV, false, true);
             constexpr uint32_t kIdS = umma_idesc_bf16(kTcC, DV, true, true);
             auto p_cols = [&](int c) { return tmem + (c % L::np) * 128; };
-            auto scores = [&](int c) {  // Q K^T of chunk c
+            auto scores = [&](int c) {  // Q K^T; its columns are free
                 if (!wait(&bars.q_full[c % L::nq], c / L::nq) || !wait(&bars.k_full[c % L::nk], c / L::nk)) return false;
-                // P V of the chunk that had these columns is done
-                if (c >= L::np && !wait(&bars.o_full, c - L::np)) return false;
                 tcgen05_after();
-                const uint32_t q_at = sb + L::q + (c % L::nq) * L::kQ, k_at = sb + L::k + (c % L::nk) * L::kQ;
-                const uint64_t dq = umma_desc_sw128(q_at, 16), dk = umma_desc_sw128(k_at, 16);
+                const uint64_t dq = umma_desc_sw128(sb + L::q + (c % L::nq) * L::kQ, 16);
+                const uint64_t dk = umma_desc_sw128(sb + L::k + (c % L::nk) * L::kQ, 16);
 #pragma unroll
                 for (int k = 0; k < DQ / 16; k++) {
                     const uint32_t off = ((k / 4) * kTcBlock + (k % 4) * 32) >> 4;
                     umma_bf16_ss(p_cols(c), dq + off, dk + off, kIdP, k > 0);
                 }
                 umma_arrive(&bars.p_full[c % L::np]);
+                umma_arrive(&bars.k_free[c % L::nk]);
+                return true;
+            };
+            auto carried = [&](int c) {  // Q S
+                if (!wait(&bars.s_ready, c)) return false;
+                tcgen05_after();
+                const uint64_t dq = umma_desc_sw128(sb + L::q + (c % L::nq) * L::kQ, 16);
+                const uint64_t ds = umma_desc_sw128(sb + L::s, DQ * 128);
+#pragma unroll
+                for (int k = 0; k < DQ / 16; k++)
+                    umma_bf16_ss(tmem + L::o2, dq + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4), ds + k * 128, kIdO,
+                                 k > 0);
+                umma_arrive(&bars.q_free[c % L::nq]);
+                umma_arrive(&bars.s_free);
                 return true;
             };
             auto body = [&](int c) {
-                const uint32_t q_at = sb + L::q + (c % L::nq) * L::kQ, k_at = sb + L::k + (c % L::nk) * L::kQ,
-                               v_at = sb + L::v + (c % L::nv) * L::kV;
-                if (!STATE_ONLY) {
-                    if (L::np > 1 && c + 1 < chunks && !scores(c + 1)) return false;
-                    if (!wait(&bars.s_ready, c)) return false;
-                    if (c > 0 && !wait(&bars.o_free, c - 1)) return false;
-                    tcgen05_after();
-                    const uint64_t dq = umma_desc_sw128(q_at, 16), ds = umma_desc_sw128(sb + L::s, DQ * 128);
-#pragma unroll
-                    for (int k = 0; k < DQ / 16; k++)
-                        umma_bf16_ss(tmem + L::o2, dq + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4), ds + k * 128, kIdO, k > 0);
-                    umma_arrive(&bars.q_free[c % L::nq]);
-                    umma_arrive(&bars.s_free);
-                }
-                if (!wait(&bars.v_full[c % L::nv], c / L::nv) || !wait(&bars.kw_ready, c)) return false;
+                const uint64_t dv = umma_desc_sw128(sb + L::v + (c % L::nv) * L::kV, kTcBlock);
+                if (!wait(&bars.v_full[c % L::nv], c / L::nv) || !wait(&bars.kw_ready[c % L::nm], c / L::nm)) return false;
                 if (c > 0 && !wait(&bars.ds_free, c - 1)) return false;
                 tcgen05_after();
-                const uint64_t dv = umma_desc_sw128(v_at, kTcBlock);
 #pragma unroll 1
                 for (int piece = 0; piece < NP; piece++) {
-                    const uint64_t dk = umma_desc_sw128(piece == 0 ? k_at : sb + (piece == 1 ? L::mid : L::lo), kTcBlock);
+                    const uint64_t dk = umma_desc_sw128(sb + L::pieces + ((c % L::nm) * NP + piece) * L::kQ, kTcBlock);
 #pragma unroll
                     for (int k = 0; k < kTcC / 16; k++)
                         umma_bf16_ss(tmem + L::ds, dk + k * 128, dv + k * 128, kIdS, piece > 0 || k > 0);
                 }
                 umma_arrive(&bars.ds_full);
-                umma_arrive(&bars.k_free[c % L::nk]);
-                if (!STATE_ONLY) {
-                    if (!wait(&bars.p_ready[c % L::np], c / L::np)) return false;
-                    tcgen05_after();
-                    const uint32_t pb = p_cols(c) + (p.rev ? 0u : 64u);  // P in bf16
+                if (STATE_ONLY) {
+                    umma_arrive(&bars.v_free[c % L::nv]);
+                    return true;
+                }
+                if (!wait(&bars.p_ready[c % L::np], c / L::np)) return false;
+                if (c > 0 && !wait(&bars.o_free, c - 1)) return false;
+                if (!L::early && !carried(c)) return false;
+                tcgen05_after();
+                const uint32_t pb = p_cols(c) + (p.rev ? 0u : 64u);  // P in bf16
 #pragma unroll
-                    for (int k = 0; k < kTcC / 16; k++)
-                        umma_bf16_ts(tmem + L::o1, pb + k * 8, dv + k * 128, kIdO, k > 0);
+                for (int k = 0; k < kTcC / 16; k++)
+                    umma_bf16_ts(tmem + L::o1, pb + k * 8, dv + k * 128, kIdO, k > 0);
+                umma_arrive(&bars.v_free[c % L::nv]);
+                if (!L::early) umma_arrive(&bars.o_full);
+                if (c + L::np < chunks) {
+                    if (!wait(&bars.v_free[c % L::nv], c / L::nv)) return false;  // P V is done: P's columns are free
+                    if (!scores(c + L::np)) return false;
+                }
+                if (L::early) {
+                    if (!carried(c)) return false;
                     umma_arrive(&bars.o_full);
                 }
-                umma_arrive(&bars.v_free[c % L::nv]);
-                if (!STATE_ONLY && L::np == 1 && c + 1 < chunks) return scores(c + 1);
                 return true;
             };
-            if (chunks > 0 && (STATE_ONLY || scores(0)))
-                for (int c = 0; c < chunks; c++)
-                    if (!body(c)) break;
+            bool ok = true;
+            if (!STATE_ONLY)
+                for (int c = 0; ok && c < L::np && c < chunks; c++) ok = scores(c);
+            for (int c = 0; ok && c < chunks; c++) ok = body(c);
             umma_arrive(&bars.done);  // nothing of the tensor cores is left running
             mbar_wait(&bars.done, 0);
         }
@@ -427,6 +430,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const int row = tid & 127;
             const int64_t o_at = b * p.os[0] + h * p.os[2];
+            const bool sectors = p.dv % 16 == 0 && (uintptr_t)p.o % 32 == 0;  // rows of whole 32-byte sectors
             for (int c = 0; c < chunks; c++) {
                 const int t0 = t_first + c * t_step, n = min(kTcC, end - t0);
                 const int r = p.rev ? n - 1 - row : row;
@@ -434,7 +438,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 if (!wait_warp(&bars.o_full, c)) break;
                 tcgen05_after();
                 const uint64_t ww = two(w, w);
-                const bool full = s1 - t0 >= kTcC && p.dv == DV;
+                char *o_row = (char *)p.o + (o_at + (int64_t)(t0 + row) * p.os[1]) * (p.o_f32 ? 4 : 2);
 #pragma unroll 1
                 for (int g = 0; g < DV; g += 32) {
                     uint32_t x[32], y[32];
@@ -447,30 +451,36 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                     }
                     uint64_t o[16];
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
+                    for (int e = 0; e < 16; e++)
                         o[e] = fma2(ww, two(y[2 * e], y[2 * e + 1]), two(x[2 * e], x[2 * e + 1]));
-                        if (row >= n) o[e] = 0;
+                    if (row >= n) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[e] = 0;
                     }
-                    if (!p.o_f32) {
-                        // four lanes hold four rows of 64 bytes: transposed among them, so that they
-                        // write 64 consecutive bytes of one row at a time
-                        uint32_t m[4][4];
+                    if (t0 + row < s1) {
+                        if (!p.o_f32) {
+                            __nv_bfloat16 *dst = (__nv_bfloat16 *)o_row + g;
 #pragma unroll
-                        for (int e = 0; e < 16; e++) m[e / 4][e % 4] = pack2_bf16(o[e]);
-                        quad_transpose(m, lane);
-                        const int col = g + (lane & 3) * 8;
-                        __nv_bfloat16 *dst = (__nv_bfloat16 *)p.o + o_at + (int64_t)(t0 + (row & ~3)) * p.os[1] + col;
+                            for (int e = 0; e < 16; e += 8) {
+                                const uint32_t m[8] = {pack2_bf16(o[e]),     pack2_bf16(o[e + 1]), pack2_bf16(o[e + 2]),
+                                                       pack2_bf16(o[e + 3]), pack2_bf16(o[e + 4]), pack2_bf16(o[e + 5]),
+                                                       pack2_bf16(o[e + 6]), pack2_bf16(o[e + 7])};
+                                if (sectors && g + 2 * e < p.dv) {
+                                    store_32_bytes(dst + 2 * e, m);
+                                } else {
+                                    if (g + 2 * e < p.dv)
+                                        *reinterpret_cast<uint4 *>(dst + 2 * e) = make_uint4(m[0], m[1], m[2], m[3]);
+                                    if (g + 2 * e + 8 < p.dv)
+                                        *reinterpret_cast<uint4 *>(dst + 2 * e + 8) = make_uint4(m[4], m[5], m[6], m[7]);
+                                }
+                            }
+                        } else {
+                            float *dst = (float *)o_row + g;
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (full || (t0 + (row & ~3) + i < s1 && col < p.dv))
-                                *reinterpret_cast<uint4 *>(dst + i * p.os[1]) =
-                                    make_uint4(m[i][0], m[i][1], m[i][2], m[i][3]);
-                    } else if (t0 + row < s1) {
-                        float *dst = (float *)p.o + o_at + (int64_t)(t0 + row) * p.os[1] + g;
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2)
-                            if (g + 2 * e < p.dv)
-                                *reinterpret_cast<ulonglong2 *>(dst + 2 * e) = make_ulonglong2(o[e], o[e + 1]);
+                            for (int e = 0; e < 16; e += 2)
+                                if (g + 2 * e < p.dv)
+                                    *reinterpret_cast<ulonglong2 *>(dst + 2 * e) = make_ulonglong2(o[e], o[e + 1]);
+                        }
                     }
                     __syncwarp();
                 }
@@ -488,7 +498,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 }
             }
         }
-    } else {
+    } else if (group < L::last_group) {
         // ---- k's pieces and the state: one row of the state a thread, 64 of its columns
         regs_inc<L::state_regs>();
         constexpr int NB = L::state_groups, SC = 64;
@@ -536,7 +546,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
         constexpr int NW = 8 / NB;
         TokenWeight<NP> wk[NW];
         int wn = -1;  // the chunk size that they are for
-        for (int c = 0; c < chunks; c++) {
+        auto weigh = [&](int c) {  // k's pieces of chunk c; the MMAs that read this set of them are done
             const int t0 = t_first + c * t_step, n = min(kTcC, end - t0);
             if (n != wn) {  // the first chunk, the one with the sequence's end, and the one after it
 #pragma unroll
@@ -546,46 +556,50 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 }
                 wn = n;
             }
-            if (!wait_warp(&bars.k_full[c % L::nk], c / L::nk)) break;
-            if (!STATE_ONLY && !wait_warp(&bars.p_full[c % L::np], c / L::np)) break;  // Q K^T has read k
-            if (t0 + n < min(t0 + kTcC, (int)a.T)) {
-                // what lies past the end may be anything: a zero weight does not remove it from v
-                if (!wait_warp(&bars.v_full[c % L::nv], c / L::nv)) break;
-                uint4 *v4 = reinterpret_cast<uint4 *>(base + L::v + (c % L::nv) * L::kV);
-                for (int i = at; i < (int)L::kV / 16; i += 128 * NB)
-                    if (i / 8 % kTcC >= n) v4[i] = make_uint4(0, 0, 0, 0);
-            }
-            // the last chunk's MMAs (ds_full, below) have read the other pieces
-            uint4 *k4 = reinterpret_cast<uint4 *>(base + L::k + (c % L::nk) * L::kQ);
-            uint4 *mid4 = reinterpret_cast<uint4 *>(base + L::mid);
-            uint4 *lo4 = reinterpret_cast<uint4 *>(base + L::lo);
+            if (!wait_warp(&bars.k_full[c % L::nk], c / L::nk)) return false;
+            const uint4 *k4 = reinterpret_cast<const uint4 *>(base + L::k + (c % L::nk) * L::kQ) + at;
+            uint4 *to = reinterpret_cast<uint4 *>(base + L::pieces + (c % L::nm) * NP * L::kQ) + at;
 #pragma unroll 1
             for (int blk = 0; blk < DQ / 64; blk++) {
-                // four loads first: a thread's vectors do not depend on one another
-                const int i0 = blk * (kTcBlock / 16) + at;  // rows at / 8 + 16 NB it
 #pragma unroll
                 for (int j = 0; j < NW; j += 4) {
+                    // four loads first: a thread's vectors (rows at / 8 + 16 NB i) do not depend on one another
                     uint4 x[4];
 #pragma unroll
                     for (int it = 0; it < 4; it++) {
-                        x[it] = k4[i0 + (j + it) * 128 * NB];
+                        x[it] = k4[(j + it) * 128 * NB];
                         // not a token: anything may be there
                         if (n < kTcC && at / 8 + 16 * NB * (j + it) >= n) x[it] = make_uint4(0, 0, 0, 0);
                     }
 #pragma unroll
                     for (int it = 0; it < 4; it++) {
-                        const int i = i0 + (j + it) * 128 * NB;
                         uint4 hi, mid, lo;
                         wk[j + it].split(x[it], hi, mid, lo);
-                        k4[i] = hi;
-                        mid4[i] = mid;
-                        if (NP == 3) lo4[i] = lo;
+                        uint4 *dst = to + (j + it) * 128 * NB;
+                        dst[0] = hi;
+                        dst[L::kQ / 16] = mid;
+                        if (NP == 3) dst[2 * (L::kQ / 16)] = lo;
                     }
                 }
+                k4 += kTcBlock / 16;
+                to += kTcBlock / 16;
+            }
+            mbar_arrive(&bars.k_free[c % L::nk]);
+            if (t0 + n < min(t0 + kTcC, (int)a.T)) {
+                // what lies past the end may be anything: a zero weight does not remove it from v
+                if (!wait_warp(&bars.v_full[c % L::nv], c / L::nv)) return false;
+                uint4 *v4 = reinterpret_cast<uint4 *>(base + L::v + (c % L::nv) * L::kV);
+                for (int i = at; i < (int)L::kV / 16; i += 128 * NB)
+                    if (i / 8 % kTcC >= n) v4[i] = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_shared();
-            mbar_arrive(&bars.kw_ready);
-
+            mbar_arrive(&bars.kw_ready[c % L::nm]);
+            return true;
+        };
+        bool ok = chunks > 0 && weigh(0);
+        for (int c = 0; ok && c < chunks; c++) {
+            const int n = min(kTcC, end - (t_first + c * t_step));
+            if (L::nm == 2 && c + 1 < chunks && !weigh(c + 1)) break;
             const DecayFactor bn = n == kTcC ? full : DecayFactor(ld, n);
             const uint64_t bn_hi = two(bn.hi, bn.hi), bn_lo = two(bn.lo, bn.lo);
             if (!wait_warp(&bars.ds_full, c)) break;
@@ -605,7 +619,9 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             }
             tcgen05_before();
             mbar_arrive(&bars.ds_free);
-            if (!STATE_ONLY && c + 1 < chunks) {
+            if (c + 1 == chunks) break;
+            if (L::nm == 1 && !weigh(c + 1)) break;
+            if (!STATE_ONLY) {
                 if (!wait_warp(&bars.s_free, c)) break;
                 put_state();
             }
@@ -629,6 +645,8 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                     if (c0 + j + e < p.dv) s_out[st * row + (c0 + j + e) * col] = f[e];
             }
         }
+    } else {
+        regs_dec<24>();  // a group without a role
     }
     tcgen05_before();
     __syncthreads();
