@@ -226,7 +226,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     unsigned char *base = (unsigned char *)(((uintptr_t)tc_raw + 1023) & ~(uintptr_t)1023);
     __shared__ TcBars bars;
     __shared__ uint32_t tmem_slot;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = warp >> 2;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0), group = warp >> 2;
     const int pi = blockIdx.y;
     const AttnPass &p = a.p[pi];
     const int64_t bh = blockIdx.x / a.nseg;
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     tcgen05_before();
     __syncthreads();
     tcgen05_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = __shfl_sync(~0u, tmem_slot, 0);
     // bounded waits; a role that gives up ends, and the others then run out of theirs
     auto wait = [&](uint64_t *bar, uint32_t phase) {  // one thread's
         if (mbar_wait(bar, phase & 1)) return true;
@@ -315,83 +315,91 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             for (int c = max(0, nk - L::nk); c < nk; c++) mbar_wait(&bars.k_full[c % L::nk], (c / L::nk) & 1);
             for (int c = max(0, nq - L::nq); c < nq; c++) mbar_wait(&bars.q_full[c % L::nq], (c / L::nq) & 1);
             for (int c = max(0, nv - L::nv); c < nv; c++) mbar_wait(&bars.v_full[c % L::nv], (c / L::nv) & 1);
-        } else if ((warp & 3) == 1 && lane == 0) {
-            // ---- MMAs
+        } else if ((warp & 3) == 1) {
+            // ---- MMAs: the warp together, one lane issues
             const uint32_t sb = smem_u32(base);
             constexpr uint32_t kIdP = umma_idesc_bf16(kTcC, kTcC, false, false);
             constexpr uint32_t kIdO = umma_idesc_bf16(kTcC, DV, false, true);
             constexpr uint32_t kIdS = umma_idesc_bf16(kTcC, DV, true, true);
             auto p_cols = [&](int c) { return tmem + (c % L::np) * 128; };
             auto scores = [&](int c) {  // Q K^T; its columns are free
-                if (!wait(&bars.q_full[c % L::nq], c / L::nq) || !wait(&bars.k_full[c % L::nk], c / L::nk)) return false;
+                if (!wait_warp(&bars.q_full[c % L::nq], c / L::nq)) return false;
+                if (!wait_warp(&bars.k_full[c % L::nk], c / L::nk)) return false;
                 tcgen05_after();
                 const uint64_t dq = umma_desc_sw128(sb + L::q + (c % L::nq) * L::kQ, 16);
                 const uint64_t dk = umma_desc_sw128(sb + L::k + (c % L::nk) * L::kQ, 16);
+                if (elect_lane()) {
 #pragma unroll
-                for (int k = 0; k < DQ / 16; k++) {
-                    const uint32_t off = ((k / 4) * kTcBlock + (k % 4) * 32) >> 4;
-                    umma_bf16_ss(p_cols(c), dq + off, dk + off, kIdP, k > 0);
+                    for (int k = 0; k < DQ / 16; k++) {
+                        const uint32_t off = ((k / 4) * kTcBlock + (k % 4) * 32) >> 4;
+                        umma_bf16_ss(p_cols(c), dq + off, dk + off, kIdP, k > 0);
+                    }
+                    umma_arrive(&bars.p_full[c % L::np]);
+                    umma_arrive(&bars.k_free[c % L::nk]);
                 }
-                umma_arrive(&bars.p_full[c % L::np]);
-                umma_arrive(&bars.k_free[c % L::nk]);
                 return true;
             };
             auto carried = [&](int c) {  // Q S
-                if (!wait(&bars.s_ready, c)) return false;
+                if (!wait_warp(&bars.s_ready, c)) return false;
                 tcgen05_after();
                 const uint64_t dq = umma_desc_sw128(sb + L::q + (c % L::nq) * L::kQ, 16);
                 const uint64_t ds = umma_desc_sw128(sb + L::s, DQ * 128);
+                if (elect_lane()) {
 #pragma unroll
-                for (int k = 0; k < DQ / 16; k++)
-                    umma_bf16_ss(tmem + L::o2, dq + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4), ds + k * 128, kIdO,
-                                 k > 0);
-                umma_arrive(&bars.q_free[c % L::nq]);
-                umma_arrive(&bars.s_free);
+                    for (int k = 0; k < DQ / 16; k++)
+                        umma_bf16_ss(tmem + L::o2, dq + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4), ds + k * 128, kIdO,
+                                     k > 0);
+                    umma_arrive(&bars.q_free[c % L::nq]);
+                    umma_arrive(&bars.s_free);
+                    if (L::early) umma_arrive(&bars.o_full);
+                }
                 return true;
             };
             auto body = [&](int c) {
                 const uint64_t dv = umma_desc_sw128(sb + L::v + (c % L::nv) * L::kV, kTcBlock);
-                if (!wait(&bars.v_full[c % L::nv], c / L::nv) || !wait(&bars.kw_ready[c % L::nm], c / L::nm)) return false;
-                if (c > 0 && !wait(&bars.ds_free, c - 1)) return false;
+                if (!wait_warp(&bars.v_full[c % L::nv], c / L::nv)) return false;
+                if (!wait_warp(&bars.kw_ready[c % L::nm], c / L::nm)) return false;
+                if (c > 0 && !wait_warp(&bars.ds_free, c - 1)) return false;
                 tcgen05_after();
+                if (elect_lane()) {
 #pragma unroll 1
-                for (int piece = 0; piece < NP; piece++) {
-                    const uint64_t dk = umma_desc_sw128(sb + L::pieces + ((c % L::nm) * NP + piece) * L::kQ, kTcBlock);
+                    for (int piece = 0; piece < NP; piece++) {
+                        const uint64_t dk = umma_desc_sw128(sb + L::pieces + ((c % L::nm) * NP + piece) * L::kQ, kTcBlock);
 #pragma unroll
-                    for (int k = 0; k < kTcC / 16; k++)
-                        umma_bf16_ss(tmem + L::ds, dk + k * 128, dv + k * 128, kIdS, piece > 0 || k > 0);
+                        for (int k = 0; k < kTcC / 16; k++)
+                            umma_bf16_ss(tmem + L::ds, dk + k * 128, dv + k * 128, kIdS, piece > 0 || k > 0);
+                    }
+                    umma_arrive(&bars.ds_full);
+                    if (STATE_ONLY) umma_arrive(&bars.v_free[c % L::nv]);
                 }
-                umma_arrive(&bars.ds_full);
-                if (STATE_ONLY) {
-                    umma_arrive(&bars.v_free[c % L::nv]);
-                    return true;
-                }
-                if (!wait(&bars.p_ready[c % L::np], c / L::np)) return false;
-                if (c > 0 && !wait(&bars.o_free, c - 1)) return false;
+                if (STATE_ONLY) return true;
+                if (!wait_warp(&bars.p_ready[c % L::np], c / L::np)) return false;
+                if (c > 0 && !wait_warp(&bars.o_free, c - 1)) return false;
                 if (!L::early && !carried(c)) return false;
                 tcgen05_after();
                 const uint32_t pb = p_cols(c) + (p.rev ? 0u : 64u);  // P in bf16
+                if (elect_lane()) {
 #pragma unroll
-                for (int k = 0; k < kTcC / 16; k++)
-                    umma_bf16_ts(tmem + L::o1, pb + k * 8, dv + k * 128, kIdO, k > 0);
-                umma_arrive(&bars.v_free[c % L::nv]);
-                if (!L::early) umma_arrive(&bars.o_full);
+                    for (int k = 0; k < kTcC / 16; k++)
+                        umma_bf16_ts(tmem + L::o1, pb + k * 8, dv + k * 128, kIdO, k > 0);
+                    umma_arrive(&bars.v_free[c % L::nv]);
+                    if (!L::early) umma_arrive(&bars.o_full);
+                }
                 if (c + L::np < chunks) {
-                    if (!wait(&bars.v_free[c % L::nv], c / L::nv)) return false;  // P V is done: P's columns are free
+                    // P V is done: P's columns are free
+                    if (!wait_warp(&bars.v_free[c % L::nv], c / L::nv)) return false;
                     if (!scores(c + L::np)) return false;
                 }
-                if (L::early) {
-                    if (!carried(c)) return false;
-                    umma_arrive(&bars.o_full);
-                }
-                return true;
+                return !L::early || carried(c);
             };
             bool ok = true;
             if (!STATE_ONLY)
                 for (int c = 0; ok && c < L::np && c < chunks; c++) ok = scores(c);
             for (int c = 0; ok && c < chunks; c++) ok = body(c);
-            umma_arrive(&bars.done);  // nothing of the tensor cores is left running
-            mbar_wait(&bars.done, 0);
+            if (elect_lane()) {  // nothing of the tensor cores is left running
+                umma_arrive(&bars.done);
+                mbar_wait(&bars.done, 0);
+            }
         }
     } else if (group < L::score_groups) {
         // ---- P: one token a thread

@@ -58,6 +58,20 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u
         : "memory");
 }
 
+// True in one lane of a converged warp (always the same one).  Warp-uniform code around
+// the MMAs keeps their descriptors in uniform registers; from a branch on the lane
+// number each MMA first has to move them there.
+__device__ __forceinline__ bool elect_lane()
+{
+    uint32_t on;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(on));
+    return on != 0;
+}
+
 // An arrival on `bar` once all MMAs that this thread has issued are done.
 __device__ __forceinline__ void umma_arrive(uint64_t *bar)
 {
