@@ -19,13 +19,14 @@
 // r(h) and r(x') of each row, 8 bytes.  A group of TPR threads (a power of two)
 // owns a row, NIT vectors of VEC elements a thread; groups walk the rows with
 // a grid stride, so that the weights stay in registers and the backward adds
-// its rows' parts of dpre and dpost there, in row order; the groups' sums (fp32)
-// are added by a second launch in a fixed order.
+// its rows' parts of dpre and dpost there, in row order; the groups' and then the
+// blocks' sums (fp32; a second launch) are added in a fixed order.
 #include <algorithm>
 
 #include "lifb_common.cuh"
 #include "lifb_internal.h"
 #include "seq_types.cuh"
+#include "tma.cuh"
 
 namespace lifb {
 
@@ -47,7 +48,7 @@ struct NormArgs {
     float *rstd;                   // [2][R]: r(h), r(x')
     const void *dxo, *dn;
     void *dx, *dh, *dgate;
-    float *part;  // [blocks * groups][2][D]
+    float *part;  // [blocks][2][D]
     int64_t R, D;
     float scale, eps;
     int act, gate_row, w_f32;
@@ -84,28 +85,22 @@ __device__ __forceinline__ void row_sum(float (&v)[NV], int tpr, float *sh, int 
     }
 }
 
-__device__ __forceinline__ float act_value(int act, float g)
-{
-    if (act == kActLinear) return g;
-    const float sg = 1.0f / (1.0f + expf(-g));
-    return act == kActSilu ? g * sg : sg;
-}
+// sigmoid(g) by the 2-ulp power and the 1-ulp reciprocal: the norms would wait for
+// expf and the division (measured: 60 of the backward's 130 instructions an element).
+__device__ __forceinline__ float sigmoid(float g) { return rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * g)); }
 
-// act(g) and act'(g)
-__device__ __forceinline__ void act_grad(int act, float g, float &a, float &da)
+// act(g) and act'(g) of g and its sigmoid
+__device__ __forceinline__ float act_value(int act, float g, float sg)
 {
-    if (act == kActLinear) {
-        a = g;
-        da = 1.0f;
-        return;
-    }
-    const float sg = 1.0f / (1.0f + expf(-g));
-    a = act == kActSilu ? g * sg : sg;
-    da = act == kActSilu ? sg * (1.0f + g * (1.0f - sg)) : sg * (1.0f - sg);
+    return act == kActSilu ? g * sg : act == kActSigmoid ? sg : g;
+}
+__device__ __forceinline__ float act_grad(int act, float g, float sg)
+{
+    return act == kActSilu ? sg + g * (sg - sg * sg) : act == kActSigmoid ? sg - sg * sg : 1.0f;
 }
 
 template <typename T, int VEC>
-__device__ __forceinline__ void load_weight(const void *w, int f32, int64_t c, float (&x)[VEC])
+__device__ __forceinline__ void load_weight(const void *w, int f32, int c, float (&x)[VEC])
 {
     if (f32) {
 #pragma unroll
@@ -115,47 +110,71 @@ __device__ __forceinline__ void load_weight(const void *w, int f32, int64_t c, f
     }
 }
 
-template <typename T, int VEC, int NIT, int MAXT>
-__global__ void __launch_bounds__(MAXT)
+// A row's vectors of one tensor, as they are in memory: loaded for the next row
+// while the present one waits for its sums.  Absent tensors and columns are zero.
+template <typename T, int VEC, int NIT>
+struct RowPart {
+    Pack<T, VEC> p[NIT];
+    __device__ __forceinline__ void load(const void *base, int64_t at, int c0, int step, int D, bool on)
+    {
+#pragma unroll
+        for (int i = 0; i < NIT; i++) {
+            const int c = c0 + i * step;
+            p[i].zero();
+            if (on && c < D) p[i].load((const T *)base + at + c);
+        }
+    }
+};
+
+// GATE: the gate's form at compile time (0 none, 1 elementwise, 2 one value a row), or -1
+// (as the arguments say).
+template <typename T, int VEC, int NIT, int MAXT, int GATE>
+__global__ void __launch_bounds__(MAXT, MAXT == kNgThreads && VEC * NIT <= 8 ? 3 : 1)
     k_norm_fwd(const __grid_constant__ NormArgs a, int tpr)
 {
     __shared__ float sh[2 * 32];
     int flip = 0;
-    const int lane = threadIdx.x & (tpr - 1);
-    const int64_t groups = blockDim.x / tpr, g = threadIdx.x / tpr;
+    const int lane = threadIdx.x & (tpr - 1), c0 = lane * VEC, step = tpr * VEC, D = (int)a.D;
+    const int64_t groups = blockDim.x / tpr, g = threadIdx.x / tpr, stride = gridDim.x * groups;
+    const bool full_gate = GATE == 1 || (GATE < 0 && a.gate && !a.gate_row);
+    const bool row_gate = GATE == 2 || (GATE < 0 && a.gate && a.gate_row);
     const float inv_d = 1.0f / (float)a.D;
     float post[NIT][VEC], pre[NIT][VEC];
 #pragma unroll
     for (int i = 0; i < NIT; i++) {
-        const int64_t c = ((int64_t)i * tpr + lane) * VEC;
-        if (c < a.D) {
+        const int c = c0 + i * step;
+        if (c < D) {
             if (a.h) load_weight<T, VEC>(a.post, a.w_f32, c, post[i]);
             if (a.n) load_weight<T, VEC>(a.pre, a.w_f32, c, pre[i]);
         }
     }
+    RowPart<T, VEC, NIT> nx, nh, ng;
+    float grow = 0.0f;
+    auto fetch = [&](int64_t r) {
+        const bool on = r < a.R;
+        nx.load(a.x, r * a.sx, c0, step, D, on);
+        if (a.h) nh.load(a.h, r * a.sh, c0, step, D, on);
+        if (full_gate) ng.load(a.gate, r * a.sg, c0, step, D, on);
+        if (row_gate) grow = on ? to_f32(((const T *)a.gate)[r * a.sg]) : 0.0f;
+    };
+    fetch(blockIdx.x * groups + g);
     // every group of a block makes the same number of rounds
-    for (int64_t r0 = blockIdx.x * groups; r0 < a.R; r0 += gridDim.x * groups) {
+    for (int64_t r0 = blockIdx.x * groups; r0 < a.R; r0 += stride) {
         const int64_t r = r0 + g;
         const bool on = r < a.R;
-        float x[NIT][VEC], h[NIT][VEC], gt[NIT][VEC];
+        float x[NIT][VEC];
         float ss[1] = {0.0f};
-        float grow = 0.0f;
-        if (on && a.h && a.gate && a.gate_row) grow = to_f32(((const T *)a.gate)[r * a.sg]);
 #pragma unroll
-        for (int i = 0; i < NIT; i++) {
-            const int64_t c = ((int64_t)i * tpr + lane) * VEC;
-            const bool in = on && c < a.D;
-#pragma unroll
-            for (int e = 0; e < VEC; e++) x[i][e] = h[i][e] = gt[i][e] = 0.0f;
-            if (in) {
-                load_f32((const T *)a.x + r * a.sx + c, x[i]);
-                if (a.h) {
-                    load_f32((const T *)a.h + r * a.sh + c, h[i]);
-                    if (a.gate && !a.gate_row) load_f32((const T *)a.gate + r * a.sg + c, gt[i]);
-                }
-            }
-        }
+        for (int i = 0; i < NIT; i++) nx.p[i].get(x[i]);
         if (a.h) {
+            float h[NIT][VEC], av[NIT][VEC];
+            const float arow = row_gate ? act_value(a.act, grow, sigmoid(grow)) : 1.0f;
+#pragma unroll
+            for (int i = 0; i < NIT; i++) {
+                nh.p[i].get(h[i]);
+                if (full_gate) ng.p[i].get(av[i]);
+            }
+            fetch(r + stride);
 #pragma unroll
             for (int i = 0; i < NIT; i++)
 #pragma unroll
@@ -163,22 +182,25 @@ __global__ void __launch_bounds__(MAXT)
             row_sum(ss, tpr, sh, flip);
             const float rh = rsqrtf(ss[0] * inv_d + a.eps);
             if (on && lane == 0 && a.rstd) a.rstd[r] = rh;
-            const float arow = a.gate && a.gate_row ? act_value(a.act, grow) : 1.0f;
+            const float k = a.scale * rh * arow;
+            ss[0] = 0.0f;
 #pragma unroll
             for (int i = 0; i < NIT; i++) {
-                const int64_t c = ((int64_t)i * tpr + lane) * VEC;
-                if (on && c < a.D) {
+                const int c = c0 + i * step;
+                if (c < D) {
 #pragma unroll
                     for (int e = 0; e < VEC; e++) {
-                        const float av = a.gate && !a.gate_row ? act_value(a.act, gt[i][e]) : arow;
-                        x[i][e] += a.scale * (av * (h[i][e] * rh * post[i][e]));
+                        float y = h[i][e] * post[i][e];
+                        if (full_gate) y *= act_value(a.act, av[i][e], sigmoid(av[i][e]));
+                        x[i][e] += k * y;
                     }
-                    store_f32((T *)a.xo + r * a.D + c, x[i]);
+                    if (on) store_f32((T *)a.xo + r * a.D + c, x[i]);
                 }
             }
+        } else {
+            fetch(r + stride);
         }
         if (a.n) {
-            ss[0] = 0.0f;
 #pragma unroll
             for (int i = 0; i < NIT; i++)
 #pragma unroll
@@ -188,8 +210,8 @@ __global__ void __launch_bounds__(MAXT)
             if (on && lane == 0 && a.rstd) a.rstd[a.R + r] = rx;
 #pragma unroll
             for (int i = 0; i < NIT; i++) {
-                const int64_t c = ((int64_t)i * tpr + lane) * VEC;
-                if (on && c < a.D) {
+                const int c = c0 + i * step;
+                if (on && c < D) {
                     float y[VEC];
 #pragma unroll
                     for (int e = 0; e < VEC; e++) y[e] = x[i][e] * rx * pre[i][e];
@@ -200,73 +222,85 @@ __global__ void __launch_bounds__(MAXT)
     }
 }
 
-template <typename T, int VEC, int NIT, int MAXT>
-__global__ void __launch_bounds__(MAXT)
+template <typename T, int VEC, int NIT, int MAXT, int GATE>
+__global__ void __launch_bounds__(MAXT, MAXT == kNgThreads && VEC * NIT <= 8 ? 2 : 1)
     k_norm_bwd(const __grid_constant__ NormArgs a, int tpr)
 {
     __shared__ float sh[2 * 2 * 32];
+    extern __shared__ float ng_part[];  // [groups][2][D], more than one group a block
     int flip = 0;
-    const int lane = threadIdx.x & (tpr - 1);
-    const int64_t groups = blockDim.x / tpr, g = threadIdx.x / tpr;
+    const int lane = threadIdx.x & (tpr - 1), c0 = lane * VEC, step = tpr * VEC, D = (int)a.D;
+    const int64_t groups = blockDim.x / tpr, g = threadIdx.x / tpr, stride = gridDim.x * groups;
+    const bool full_gate = GATE == 1 || (GATE < 0 && a.gate && !a.gate_row);
+    const bool row_gate = GATE == 2 || (GATE < 0 && a.gate && a.gate_row);
     const float inv_d = 1.0f / (float)a.D;
     float post[NIT][VEC], pre[NIT][VEC], dpost[NIT][VEC], dpre[NIT][VEC];
 #pragma unroll
     for (int i = 0; i < NIT; i++) {
-        const int64_t c = ((int64_t)i * tpr + lane) * VEC;
+        const int c = c0 + i * step;
 #pragma unroll
         for (int e = 0; e < VEC; e++) dpost[i][e] = dpre[i][e] = post[i][e] = pre[i][e] = 0.0f;
-        if (c < a.D) {
+        if (c < D) {
             if (a.h) load_weight<T, VEC>(a.post, a.w_f32, c, post[i]);
             if (a.dn) load_weight<T, VEC>(a.pre, a.w_f32, c, pre[i]);
         }
     }
-    for (int64_t r0 = blockIdx.x * groups; r0 < a.R; r0 += gridDim.x * groups) {
+    RowPart<T, VEC, NIT> nt, nu, nx, nh, ng;
+    float nrh = 0.0f, nrx = 0.0f, ngr = 0.0f;
+    auto fetch = [&](int64_t r) {
+        const bool on = r < a.R;
+        if (a.dn) nu.load(a.dn, r * a.sdn, c0, step, D, on);
+        if (a.dn) nx.load(a.x, r * a.sx, c0, step, D, on);
+        if (a.h) nh.load(a.h, r * a.sh, c0, step, D, on);
+        if (full_gate) ng.load(a.gate, r * a.sg, c0, step, D, on);
+        nt.load(a.dxo, r * a.sdx, c0, step, D, on && a.dxo);
+        if (a.h) nrh = on ? a.rstd[r] : 0.0f;
+        if (a.dn) nrx = on ? a.rstd[a.R + r] : 0.0f;
+        if (row_gate) ngr = on ? to_f32(((const T *)a.gate)[r * a.sg]) : 0.0f;
+    };
+    fetch(blockIdx.x * groups + g);
+    for (int64_t r0 = blockIdx.x * groups; r0 < a.R; r0 += stride) {
         const int64_t r = r0 + g;
         const bool on = r < a.R;
-        // t: dx', then the gradient of x'; x: x, then x'; hh: h, then h r(h)
-        float t[NIT][VEC], x[NIT][VEC], hh[NIT][VEC], gt[NIT][VEC], u[NIT][VEC];
-        float rh = 0.0f, rx = 0.0f, grow = 0.0f;
-        if (on) {
-            if (a.h) rh = a.rstd[r];
-            if (a.dn) rx = a.rstd[a.R + r];
-            if (a.h && a.gate && a.gate_row) grow = to_f32(((const T *)a.gate)[r * a.sg]);
-        }
+        // t: dx', then the gradient of x'; hh: h r(h); gt: the gate; sg: its sigmoid
+        float t[NIT][VEC], hh[NIT][VEC], gt[NIT][VEC], sg[NIT][VEC], x[NIT][VEC], u[NIT][VEC];
+        const float rh = nrh, rx = nrx, grow = ngr;
 #pragma unroll
         for (int i = 0; i < NIT; i++) {
-            const int64_t c = ((int64_t)i * tpr + lane) * VEC;
-            const bool in = on && c < a.D;
-#pragma unroll
-            for (int e = 0; e < VEC; e++) t[i][e] = x[i][e] = hh[i][e] = gt[i][e] = u[i][e] = 0.0f;
-            if (in) {
-                if (a.dxo) load_f32((const T *)a.dxo + r * a.sdx + c, t[i]);
-                if (a.dn) {
-                    load_f32((const T *)a.dn + r * a.sdn + c, u[i]);
-                    load_f32((const T *)a.x + r * a.sx + c, x[i]);
-                }
-                if (a.h) {
-                    load_f32((const T *)a.h + r * a.sh + c, hh[i]);
-                    if (a.gate && !a.gate_row) load_f32((const T *)a.gate + r * a.sg + c, gt[i]);
-                }
-            }
+            nt.p[i].get(t[i]);
+            if (a.dn) nu.p[i].get(u[i]);
+            if (a.dn) nx.p[i].get(x[i]);
+            if (a.h) nh.p[i].get(hh[i]);
+            if (full_gate) ng.p[i].get(gt[i]);
         }
+        fetch(r + stride);
         float arow = 1.0f, darow = 0.0f;
-        if (a.h && a.gate && a.gate_row) act_grad(a.act, grow, arow, darow);
+        if (row_gate) {
+            const float s = sigmoid(grow);
+            arow = act_value(a.act, grow, s);
+            darow = act_grad(a.act, grow, s);
+        }
         if (a.h) {
 #pragma unroll
             for (int i = 0; i < NIT; i++)
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
-                    const float av = a.gate && !a.gate_row ? act_value(a.act, gt[i][e]) : arow;
                     hh[i][e] *= rh;
-                    x[i][e] += a.scale * (av * (hh[i][e] * post[i][e]));
+                    if (full_gate) sg[i][e] = sigmoid(gt[i][e]);
                 }
         }
         if (a.dn) {
             float m[1] = {0.0f};
+            const float k = a.scale * arow;
 #pragma unroll
             for (int i = 0; i < NIT; i++)
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
+                    if (a.h) {
+                        float y = hh[i][e] * post[i][e];
+                        if (full_gate) y *= act_value(a.act, gt[i][e], sg[i][e]);
+                        x[i][e] += k * y;
+                    }
                     x[i][e] *= rx;
                     dpre[i][e] += u[i][e] * x[i][e];
                     u[i][e] *= pre[i][e];
@@ -281,8 +315,8 @@ __global__ void __launch_bounds__(MAXT)
         }
 #pragma unroll
         for (int i = 0; i < NIT; i++) {
-            const int64_t c = ((int64_t)i * tpr + lane) * VEC;
-            if (on && c < a.D && a.dx) store_f32((T *)a.dx + r * a.D + c, t[i]);
+            const int c = c0 + i * step;
+            if (on && c < D && a.dx) store_f32((T *)a.dx + r * a.D + c, t[i]);
         }
         if (a.h) {
             float m[2] = {0.0f, 0.0f};  // mean of w * hh; the row gate's sum of t * y
@@ -290,46 +324,57 @@ __global__ void __launch_bounds__(MAXT)
             for (int i = 0; i < NIT; i++)
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
-                    float av = arow, da = 0.0f;
-                    if (a.gate && !a.gate_row) act_grad(a.act, gt[i][e], av, da);
-                    const float st = a.scale * t[i][e], ty = st * (hh[i][e] * post[i][e]);
-                    gt[i][e] = ty * da;
-                    m[1] += ty;
-                    dpost[i][e] += st * av * hh[i][e];
+                    const float st = a.scale * t[i][e], sh_ = st * hh[i][e];
+                    float av = arow;
+                    if (full_gate) {
+                        av = act_value(a.act, gt[i][e], sg[i][e]);
+                        gt[i][e] = sh_ * post[i][e] * act_grad(a.act, gt[i][e], sg[i][e]);
+                    }
+                    if (row_gate) m[1] += sh_ * post[i][e];
+                    dpost[i][e] += av * sh_;
                     t[i][e] = st * av * post[i][e];
                     m[0] += t[i][e] * hh[i][e];
                 }
-            row_sum(m, tpr, sh + 0, flip);
+            row_sum(m, tpr, sh, flip);
             const float mw = m[0] * inv_d;
 #pragma unroll
             for (int i = 0; i < NIT; i++) {
-                const int64_t c = ((int64_t)i * tpr + lane) * VEC;
-                if (!(on && c < a.D)) continue;
+                const int c = c0 + i * step;
+                if (!(on && c < D)) continue;
                 float d[VEC];
 #pragma unroll
                 for (int e = 0; e < VEC; e++) d[e] = rh * (t[i][e] - hh[i][e] * mw);
                 if (a.dh) store_f32((T *)a.dh + r * a.D + c, d);
-                if (a.dgate && !a.gate_row) store_f32((T *)a.dgate + r * a.D + c, gt[i]);
+                if (full_gate && a.dgate) store_f32((T *)a.dgate + r * a.D + c, gt[i]);
             }
-            if (a.dgate && a.gate_row && on && lane == 0) ((T *)a.dgate)[r] = from_f32<T>(m[1] * darow);
+            if (row_gate && a.dgate && on && lane == 0) ((T *)a.dgate)[r] = from_f32<T>(m[1] * darow);
         }
     }
     if (!a.part) return;
-    float *part = a.part + (blockIdx.x * groups + g) * 2 * a.D;
+    // the block's sums: its groups' parts added in order
+    float *part = a.part + (int64_t)blockIdx.x * 2 * D, *mine = groups > 1 ? ng_part + g * 2 * D : part;
 #pragma unroll
     for (int i = 0; i < NIT; i++) {
-        const int64_t c = ((int64_t)i * tpr + lane) * VEC;
-        if (c < a.D) {
+        const int c = c0 + i * step;
+        if (c < D) {
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                part[c + e] = dpost[i][e];
-                part[a.D + c + e] = dpre[i][e];
+                mine[c + e] = dpost[i][e];
+                mine[D + c + e] = dpre[i][e];
             }
+        }
+    }
+    if (groups > 1) {
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) {
+            float v = 0.0f;
+            for (int j = 0; j < (int)groups; j++) v += ng_part[j * 2 * D + c];
+            part[c] = v;
         }
     }
 }
 
-// Adds the groups' parts column by column, in order: 32 columns a block, one
+// Adds the blocks' parts column by column, in order: 32 columns a block, one
 // warp for every kNgReduceRows-th part, then the warps' sums.
 template <typename T>
 __global__ void __launch_bounds__(32 * kNgReduceRows)
@@ -375,7 +420,8 @@ bool norm_shape(int64_t D, bool wide, int elem, NormShape &s)
     auto spread = [&](int tpr) {
         s.tpr = tpr;
         s.nit = 1;
-        while (s.nit < most && (int64_t)s.tpr * s.nit < vecs) s.nit *= 2;
+        // one element a vector: 4 or 16 of them, whichever is enough
+        while (s.nit < most && ((int64_t)s.tpr * s.nit < vecs || (!wide && s.nit < 4) || (!wide && s.nit == 8))) s.nit *= 2;
         return (int64_t)s.tpr * s.nit >= vecs;
     };
     s.threads = kNgThreads;
@@ -389,41 +435,36 @@ bool norm_shape(int64_t D, bool wide, int elem, NormShape &s)
     return spread(kNgMaxThreads);
 }
 
-int64_t norm_blocks(const NormShape &s, int64_t R)
+int64_t norm_blocks(const NormShape &s, int64_t R, bool bwd)
 {
     const int64_t groups = s.threads / s.tpr;
-    const int64_t per_sm = 1024 / s.threads;
+    const int64_t per_sm = s.threads == kNgMaxThreads || s.vec * s.nit > 8 ? 1 : bwd ? 2 : 3;
     return std::max<int64_t>(1, std::min<int64_t>((R + groups - 1) / groups, kNgSms * per_sm));
 }
 
-template <typename T, int VEC, int NIT>
+template <typename T, int VEC, int NIT, int MAXT, int GATE>
 void norm_launch(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
 {
-    const unsigned blocks = (unsigned)norm_blocks(sh, a.R);
+    const unsigned blocks = (unsigned)norm_blocks(sh, a.R, bwd);
+    const size_t groups = sh.threads / sh.tpr, smem = groups > 1 && a.part ? groups * 2 * a.D * 4 : 0;  // 32 KB at most
     count_launches(1);
-    if (sh.threads == kNgThreads) {
-        if (bwd) k_norm_bwd<T, VEC, NIT, kNgThreads><<<blocks, kNgThreads, 0, s>>>(a, sh.tpr);
-        else k_norm_fwd<T, VEC, NIT, kNgThreads><<<blocks, kNgThreads, 0, s>>>(a, sh.tpr);
-    } else if constexpr (VEC * NIT == kNgMaxElems) {  // a block of a long row is full
-        if (bwd) k_norm_bwd<T, VEC, NIT, kNgMaxThreads><<<blocks, kNgMaxThreads, 0, s>>>(a, sh.tpr);
-        else k_norm_fwd<T, VEC, NIT, kNgMaxThreads><<<blocks, kNgMaxThreads, 0, s>>>(a, sh.tpr);
-    }
+    if (bwd) k_norm_bwd<T, VEC, NIT, MAXT, GATE><<<blocks, MAXT, smem, s>>>(a, sh.tpr);
+    else k_norm_fwd<T, VEC, NIT, MAXT, GATE><<<blocks, MAXT, 0, s>>>(a, sh.tpr);
 }
 
-template <typename T, int VEC>
-void norm_pick(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
+template <typename T, int VEC, int NIT>
+void norm_gate(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
 {
-    switch (sh.nit) {
-        case 1: norm_launch<T, VEC, 1>(bwd, a, sh, s); break;
-        case 2: norm_launch<T, VEC, 2>(bwd, a, sh, s); break;
-        case 4:
-            if constexpr (VEC <= 4) norm_launch<T, VEC, 4>(bwd, a, sh, s);
-            break;
-        case 8:
-            if constexpr (VEC == 1) norm_launch<T, VEC, 8>(bwd, a, sh, s);
-            break;
-        default:
-            if constexpr (VEC == 1) norm_launch<T, VEC, 16>(bwd, a, sh, s);
+    if (sh.threads == kNgMaxThreads) {
+        if constexpr (VEC * NIT == kNgMaxElems) norm_launch<T, VEC, NIT, kNgMaxThreads, -1>(bwd, a, sh, s);
+    } else if constexpr (VEC == 1) {
+        norm_launch<T, VEC, NIT, kNgThreads, -1>(bwd, a, sh, s);
+    } else if (!a.gate) {
+        norm_launch<T, VEC, NIT, kNgThreads, 0>(bwd, a, sh, s);
+    } else if (a.gate_row) {
+        norm_launch<T, VEC, NIT, kNgThreads, 2>(bwd, a, sh, s);
+    } else {
+        norm_launch<T, VEC, NIT, kNgThreads, 1>(bwd, a, sh, s);
     }
 }
 
@@ -431,8 +472,16 @@ template <typename T>
 void norm_run(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
 {
     constexpr int VEC = 16 / sizeof(T);
-    if (sh.vec == VEC) norm_pick<T, VEC>(bwd, a, sh, s);
-    else norm_pick<T, 1>(bwd, a, sh, s);
+    if (sh.vec == 1) {
+        if (sh.nit == 4) norm_gate<T, 1, 4>(bwd, a, sh, s);
+        else norm_gate<T, 1, 16>(bwd, a, sh, s);
+    } else if (sh.nit == 1) {
+        norm_gate<T, VEC, 1>(bwd, a, sh, s);
+    } else if (sh.nit == 2) {
+        norm_gate<T, VEC, 2>(bwd, a, sh, s);
+    } else if constexpr (VEC == 4) {
+        norm_gate<T, VEC, 4>(bwd, a, sh, s);
+    }
 }
 
 int norm_fail(int status, const char *what, const char *why)
@@ -510,7 +559,7 @@ extern "C" size_t lifb_norm_gate_bwd_workspace_bytes(int64_t R, int64_t D, int d
     for (int wide = 0; wide < 2; wide++) {
         NormShape sh;
         if (norm_shape(D, wide != 0, (int)dtype_bytes(dtype), sh))
-            most = std::max(most, (size_t)norm_blocks(sh, R) * (sh.threads / sh.tpr) * 2 * D * 4);
+            most = std::max(most, (size_t)norm_blocks(sh, R, true) * 2 * D * 4);
     }
     return most;
 }
@@ -526,7 +575,8 @@ extern "C" int lifb_norm_gate_bwd(const lifb_norm_gate *p, const void *dxo, int6
     if (int st = norm_check(what, p, a)) return st;
     cudaStream_t s = (cudaStream_t)stream;
     const bool weights = dpost || dpre;
-    if (a.R == 0 || a.D == 0) {
+    if (a.D == 0) return LIFB_OK;
+    if (a.R == 0) {
         const size_t nb = (size_t)a.D * (a.w_f32 ? 4 : dtype_bytes(p->dtype));
         if ((dpost && cudaMemsetAsync(dpost, 0, nb, s) != cudaSuccess) ||
             (dpre && cudaMemsetAsync(dpre, 0, nb, s) != cudaSuccess))
@@ -556,7 +606,7 @@ extern "C" int lifb_norm_gate_bwd(const lifb_norm_gate *p, const void *dxo, int6
         return norm_fail(LIFB_ERR_UNSUPPORTED, what, "rows longer than 8192 elements");
     LIFB_BY_DTYPE(p->dtype, T, norm_run<T>(true, a, sh, s));
     if (weights) {
-        const int64_t parts = norm_blocks(sh, a.R) * (sh.threads / sh.tpr);
+        const int64_t parts = norm_blocks(sh, a.R, true);
         const unsigned blocks = (unsigned)((2 * a.D + 31) / 32);
         count_launches(1);
         LIFB_BY_DTYPE(p->dtype, T,
