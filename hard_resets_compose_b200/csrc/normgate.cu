@@ -25,6 +25,7 @@
 
 #include "lifb_common.cuh"
 #include "lifb_internal.h"
+#include "f32x2.cuh"
 #include "seq_types.cuh"
 #include "tma.cuh"
 
@@ -53,6 +54,14 @@ struct NormArgs {
     float scale, eps;
     int act, gate_row, w_f32;
 };
+
+// Blocks of a kernel that an SM holds; registers are spread accordingly.
+// (Single elements take twice the registers of packed ones.)
+__host__ __device__ constexpr int norm_blocks_per_sm(bool bwd, int threads, int vec, int nit)
+{
+    const int elems = vec == 1 ? 2 * nit : vec * nit;
+    return threads > kNgThreads || elems > 16 ? 1 : elems > 8 ? (bwd ? 1 : 2) : elems > 4 ? (bwd ? 2 : 4) : (bwd ? 4 : 5);
+}
 
 }  // namespace
 
@@ -85,30 +94,45 @@ __device__ __forceinline__ void row_sum(float (&v)[NV], int tpr, float *sh, int 
     }
 }
 
-// sigmoid(g) by the 2-ulp power and the 1-ulp reciprocal: the norms would wait for
-// expf and the division (measured: 60 of the backward's 130 instructions an element).
+// sigmoid(g) by the 2-ulp power and the 1-ulp reciprocal: with expf and the division
+// the norms waited for them instead of memory.
 __device__ __forceinline__ float sigmoid(float g) { return rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * g)); }
 
-// act(g) and act'(g) of g and its sigmoid
-__device__ __forceinline__ float act_value(int act, float g, float sg)
+// act(g) and act'(g) of one value, a row's gate
+__device__ __forceinline__ float act_value(int act, float g)
 {
-    return act == kActSilu ? g * sg : act == kActSigmoid ? sg : g;
+    return act == kActLinear ? g : act == kActSilu ? g * sigmoid(g) : sigmoid(g);
 }
-__device__ __forceinline__ float act_grad(int act, float g, float sg)
+__device__ __forceinline__ float act_grad(int act, float g)
 {
-    return act == kActSilu ? sg + g * (sg - sg * sg) : act == kActSigmoid ? sg - sg * sg : 1.0f;
+    const float sg = sigmoid(g);
+    return act == kActLinear ? 1.0f : act == kActSilu ? sg + g * (sg - sg * sg) : sg - sg * sg;
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_weight(const void *w, int f32, int c, float (&x)[VEC])
+// The same of a pair: act(g), and with `da` act'(g).
+__device__ __forceinline__ uint64_t act_pair(int act, uint64_t g, uint64_t *da)
 {
-    if (f32) {
-#pragma unroll
-        for (int e = 0; e < VEC; e++) x[e] = ((const float *)w)[c + e];
-    } else {
-        load_f32((const T *)w + c, x);
+    if (act == kActLinear) {
+        if (da) *da = two(1.0f, 1.0f);
+        return g;
     }
+    float z0, z1;
+    both(mul2(g, two(-1.4426950408889634f, -1.4426950408889634f)), z0, z1);
+    both(add2(two(ex2_approx(z0), ex2_approx(z1)), two(1.0f, 1.0f)), z0, z1);
+    const uint64_t sg = two(rcp_approx(z0), rcp_approx(z1));
+    if (da) {
+        const uint64_t d = fma2(mul2(sg, two(-1.0f, -1.0f)), sg, sg);  // sg - sg^2
+        *da = act == kActSilu ? fma2(g, d, sg) : d;
+    }
+    return act == kActSilu ? mul2(g, sg) : sg;
 }
+
+// A row's elements of one thread, NIT vectors of VEC, as pairs in that order.
+template <typename T, int VEC, int NIT>
+struct Row {
+    static constexpr int kPairs = VEC * NIT / 2;
+    uint64_t v[kPairs];
+};
 
 // A row's vectors of one tensor, as they are in memory: loaded for the next row
 // while the present one waits for its sums.  Absent tensors and columns are zero.
@@ -124,36 +148,68 @@ struct RowPart {
             if (on && c < D) p[i].load((const T *)base + at + c);
         }
     }
+    __device__ __forceinline__ void get(Row<T, VEC, NIT> &x) const
+    {
+        float f[NIT][VEC];
+#pragma unroll
+        for (int i = 0; i < NIT; i++) p[i].get(f[i]);
+#pragma unroll
+        for (int i = 0; i < VEC * NIT; i += 2) x.v[i / 2] = two(f[i / VEC][i % VEC], f[(i + 1) / VEC][(i + 1) % VEC]);
+    }
 };
 
-// GATE: the gate's form at compile time (0 none, 1 elementwise, 2 one value a row), or -1
-// (as the arguments say).
-template <typename T, int VEC, int NIT, int MAXT, int GATE>
-__global__ void __launch_bounds__(MAXT, MAXT == kNgThreads && VEC * NIT <= 8 ? 3 : 1)
+template <typename T, int VEC, int NIT>
+__device__ __forceinline__ void store_row(const Row<T, VEC, NIT> &x, void *base, int64_t at, int c0, int step, int D)
+{
+    float f[NIT][VEC];
+#pragma unroll
+    for (int i = 0; i < VEC * NIT; i += 2) both(x.v[i / 2], f[i / VEC][i % VEC], f[(i + 1) / VEC][(i + 1) % VEC]);
+#pragma unroll
+    for (int i = 0; i < NIT; i++)
+        if (c0 + i * step < D) store_f32((T *)base + at + c0 + i * step, f[i]);
+}
+
+// A weight's elements of this thread, zero past the row's end.
+template <typename T, int VEC, int NIT>
+__device__ __forceinline__ void load_weight(Row<T, VEC, NIT> &x, const void *w, int f32, int c0, int step, int D)
+{
+    float f[NIT][VEC];
+#pragma unroll
+    for (int i = 0; i < NIT; i++)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const int c = c0 + i * step;
+            f[i][e] = c >= D || !w ? 0.0f : f32 ? ((const float *)w)[c + e] : to_f32(((const T *)w)[c + e]);
+        }
+#pragma unroll
+    for (int i = 0; i < VEC * NIT; i += 2) x.v[i / 2] = two(f[i / VEC][i % VEC], f[(i + 1) / VEC][(i + 1) % VEC]);
+}
+
+// GATE: the gate's form at compile time (0 none, 1 elementwise, 2 one value a row) or -1
+// (as the arguments say); ACT: its activation, or -1.
+template <typename T, int VEC, int NIT, int MAXT, int GATE, int ACT>
+__global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(false, MAXT, VEC, NIT))
     k_norm_fwd(const __grid_constant__ NormArgs a, int tpr)
 {
+    using R = Row<T, VEC, NIT>;
+    constexpr int P = R::kPairs;
     __shared__ float sh[2 * 32];
     int flip = 0;
     const int lane = threadIdx.x & (tpr - 1), c0 = lane * VEC, step = tpr * VEC, D = (int)a.D;
     const int64_t groups = blockDim.x / tpr, g = threadIdx.x / tpr, stride = gridDim.x * groups;
     const bool full_gate = GATE == 1 || (GATE < 0 && a.gate && !a.gate_row);
     const bool row_gate = GATE == 2 || (GATE < 0 && a.gate && a.gate_row);
+    const int act = ACT >= 0 ? ACT : a.act;
     const float inv_d = 1.0f / (float)a.D;
-    float post[NIT][VEC], pre[NIT][VEC];
-#pragma unroll
-    for (int i = 0; i < NIT; i++) {
-        const int c = c0 + i * step;
-        if (c < D) {
-            if (a.h) load_weight<T, VEC>(a.post, a.w_f32, c, post[i]);
-            if (a.n) load_weight<T, VEC>(a.pre, a.w_f32, c, pre[i]);
-        }
-    }
+    R post, pre;
+    load_weight(post, a.h ? a.post : nullptr, a.w_f32, c0, step, D);
+    load_weight(pre, a.n ? a.pre : nullptr, a.w_f32, c0, step, D);
     RowPart<T, VEC, NIT> nx, nh, ng;
     float grow = 0.0f;
     auto fetch = [&](int64_t r) {
         const bool on = r < a.R;
         nx.load(a.x, r * a.sx, c0, step, D, on);
-        if (a.h) nh.load(a.h, r * a.sh, c0, step, D, on);
+        nh.load(a.h, r * a.sh, c0, step, D, on && a.h);
         if (full_gate) ng.load(a.gate, r * a.sg, c0, step, D, on);
         if (row_gate) grow = on ? to_f32(((const T *)a.gate)[r * a.sg]) : 0.0f;
     };
@@ -162,70 +218,52 @@ __global__ void __launch_bounds__(MAXT, MAXT == kNgThreads && VEC * NIT <= 8 ? 3
     for (int64_t r0 = blockIdx.x * groups; r0 < a.R; r0 += stride) {
         const int64_t r = r0 + g;
         const bool on = r < a.R;
-        float x[NIT][VEC];
-        float ss[1] = {0.0f};
-#pragma unroll
-        for (int i = 0; i < NIT; i++) nx.p[i].get(x[i]);
+        R x, h, gt;
+        nx.get(x);
+        nh.get(h);
+        if (full_gate) ng.get(gt);
+        const float arow = row_gate ? act_value(a.act, grow) : 1.0f;
+        fetch(r + stride);
         if (a.h) {
-            float h[NIT][VEC], av[NIT][VEC];
-            const float arow = row_gate ? act_value(a.act, grow, sigmoid(grow)) : 1.0f;
+            uint64_t s2 = 0;
 #pragma unroll
-            for (int i = 0; i < NIT; i++) {
-                nh.p[i].get(h[i]);
-                if (full_gate) ng.p[i].get(av[i]);
-            }
-            fetch(r + stride);
-#pragma unroll
-            for (int i = 0; i < NIT; i++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) ss[0] += h[i][e] * h[i][e];
+            for (int i = 0; i < P; i++) s2 = fma2(h.v[i], h.v[i], s2);
+            float ss[1] = {sum_of(s2)};
             row_sum(ss, tpr, sh, flip);
             const float rh = rsqrtf(ss[0] * inv_d + a.eps);
             if (on && lane == 0 && a.rstd) a.rstd[r] = rh;
             const float k = a.scale * rh * arow;
-            ss[0] = 0.0f;
+            const uint64_t kk = two(k, k);
 #pragma unroll
-            for (int i = 0; i < NIT; i++) {
-                const int c = c0 + i * step;
-                if (c < D) {
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) {
-                        float y = h[i][e] * post[i][e];
-                        if (full_gate) y *= act_value(a.act, av[i][e], sigmoid(av[i][e]));
-                        x[i][e] += k * y;
-                    }
-                    if (on) store_f32((T *)a.xo + r * a.D + c, x[i]);
-                }
+            for (int i = 0; i < P; i++) {
+                uint64_t y = mul2(h.v[i], post.v[i]);
+                if (full_gate) y = mul2(y, act_pair(act, gt.v[i], nullptr));
+                x.v[i] = fma2(kk, y, x.v[i]);
             }
-        } else {
-            fetch(r + stride);
+            if (on) store_row(x, a.xo, r * a.D, c0, step, D);
         }
         if (a.n) {
+            uint64_t s2 = 0;
 #pragma unroll
-            for (int i = 0; i < NIT; i++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) ss[0] += x[i][e] * x[i][e];
+            for (int i = 0; i < P; i++) s2 = fma2(x.v[i], x.v[i], s2);
+            float ss[1] = {sum_of(s2)};
             row_sum(ss, tpr, sh, flip);
             const float rx = rsqrtf(ss[0] * inv_d + a.eps);
             if (on && lane == 0 && a.rstd) a.rstd[a.R + r] = rx;
+            const uint64_t k = two(rx, rx);
 #pragma unroll
-            for (int i = 0; i < NIT; i++) {
-                const int c = c0 + i * step;
-                if (on && c < D) {
-                    float y[VEC];
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) y[e] = x[i][e] * rx * pre[i][e];
-                    store_f32((T *)a.n + r * a.D + c, y);
-                }
-            }
+            for (int i = 0; i < P; i++) x.v[i] = mul2(mul2(x.v[i], k), pre.v[i]);
+            if (on) store_row(x, a.n, r * a.D, c0, step, D);
         }
     }
 }
 
-template <typename T, int VEC, int NIT, int MAXT, int GATE>
-__global__ void __launch_bounds__(MAXT, MAXT == kNgThreads && VEC * NIT <= 8 ? 2 : 1)
+template <typename T, int VEC, int NIT, int MAXT, int GATE, int ACT>
+__global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT))
     k_norm_bwd(const __grid_constant__ NormArgs a, int tpr)
 {
+    using R = Row<T, VEC, NIT>;
+    constexpr int P = R::kPairs;
     __shared__ float sh[2 * 2 * 32];
     extern __shared__ float ng_part[];  // [groups][2][D], more than one group a block
     int flip = 0;
@@ -233,25 +271,20 @@ __global__ void __launch_bounds__(MAXT, MAXT == kNgThreads && VEC * NIT <= 8 ? 2
     const int64_t groups = blockDim.x / tpr, g = threadIdx.x / tpr, stride = gridDim.x * groups;
     const bool full_gate = GATE == 1 || (GATE < 0 && a.gate && !a.gate_row);
     const bool row_gate = GATE == 2 || (GATE < 0 && a.gate && a.gate_row);
+    const int act = ACT >= 0 ? ACT : a.act;
     const float inv_d = 1.0f / (float)a.D;
-    float post[NIT][VEC], pre[NIT][VEC], dpost[NIT][VEC], dpre[NIT][VEC];
+    R post, pre, dpost, dpre;
+    load_weight(post, a.h ? a.post : nullptr, a.w_f32, c0, step, D);
+    load_weight(pre, a.dn ? a.pre : nullptr, a.w_f32, c0, step, D);
 #pragma unroll
-    for (int i = 0; i < NIT; i++) {
-        const int c = c0 + i * step;
-#pragma unroll
-        for (int e = 0; e < VEC; e++) dpost[i][e] = dpre[i][e] = post[i][e] = pre[i][e] = 0.0f;
-        if (c < D) {
-            if (a.h) load_weight<T, VEC>(a.post, a.w_f32, c, post[i]);
-            if (a.dn) load_weight<T, VEC>(a.pre, a.w_f32, c, pre[i]);
-        }
-    }
+    for (int i = 0; i < P; i++) dpost.v[i] = dpre.v[i] = 0;
     RowPart<T, VEC, NIT> nt, nu, nx, nh, ng;
     float nrh = 0.0f, nrx = 0.0f, ngr = 0.0f;
     auto fetch = [&](int64_t r) {
         const bool on = r < a.R;
-        if (a.dn) nu.load(a.dn, r * a.sdn, c0, step, D, on);
-        if (a.dn) nx.load(a.x, r * a.sx, c0, step, D, on);
-        if (a.h) nh.load(a.h, r * a.sh, c0, step, D, on);
+        nu.load(a.dn, r * a.sdn, c0, step, D, on && a.dn);
+        nx.load(a.x, r * a.sx, c0, step, D, on && a.dn);
+        nh.load(a.h, r * a.sh, c0, step, D, on && a.h);
         if (full_gate) ng.load(a.gate, r * a.sg, c0, step, D, on);
         nt.load(a.dxo, r * a.sdx, c0, step, D, on && a.dxo);
         if (a.h) nrh = on ? a.rstd[r] : 0.0f;
@@ -262,106 +295,84 @@ __global__ void __launch_bounds__(MAXT, MAXT == kNgThreads && VEC * NIT <= 8 ? 2
     for (int64_t r0 = blockIdx.x * groups; r0 < a.R; r0 += stride) {
         const int64_t r = r0 + g;
         const bool on = r < a.R;
-        // t: dx', then the gradient of x'; hh: h r(h); gt: the gate; sg: its sigmoid
-        float t[NIT][VEC], hh[NIT][VEC], gt[NIT][VEC], sg[NIT][VEC], x[NIT][VEC], u[NIT][VEC];
+        // t: dx', then the gradient of x'; hh: h r(h); av, da: the gate's act and act'
+        R t, hh, av, da, x, u;
         const float rh = nrh, rx = nrx, grow = ngr;
-#pragma unroll
-        for (int i = 0; i < NIT; i++) {
-            nt.p[i].get(t[i]);
-            if (a.dn) nu.p[i].get(u[i]);
-            if (a.dn) nx.p[i].get(x[i]);
-            if (a.h) nh.p[i].get(hh[i]);
-            if (full_gate) ng.p[i].get(gt[i]);
-        }
+        nt.get(t);
+        nu.get(u);
+        nx.get(x);
+        nh.get(hh);
+        if (full_gate) ng.get(av);
         fetch(r + stride);
-        float arow = 1.0f, darow = 0.0f;
-        if (row_gate) {
-            const float s = sigmoid(grow);
-            arow = act_value(a.act, grow, s);
-            darow = act_grad(a.act, grow, s);
-        }
+        const float arow = row_gate ? act_value(a.act, grow) : 1.0f;
         if (a.h) {
+            const uint64_t k = two(rh, rh);
 #pragma unroll
-            for (int i = 0; i < NIT; i++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    hh[i][e] *= rh;
-                    if (full_gate) sg[i][e] = sigmoid(gt[i][e]);
-                }
+            for (int i = 0; i < P; i++) {
+                hh.v[i] = mul2(hh.v[i], k);
+                if (full_gate) av.v[i] = act_pair(act, av.v[i], &da.v[i]);
+            }
         }
         if (a.dn) {
-            float m[1] = {0.0f};
-            const float k = a.scale * arow;
+            const float kf = a.scale * arow;
+            const uint64_t k = two(kf, kf), kx = two(rx, rx);
+            uint64_t m2 = 0;
 #pragma unroll
-            for (int i = 0; i < NIT; i++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    if (a.h) {
-                        float y = hh[i][e] * post[i][e];
-                        if (full_gate) y *= act_value(a.act, gt[i][e], sg[i][e]);
-                        x[i][e] += k * y;
-                    }
-                    x[i][e] *= rx;
-                    dpre[i][e] += u[i][e] * x[i][e];
-                    u[i][e] *= pre[i][e];
-                    m[0] += u[i][e] * x[i][e];
+            for (int i = 0; i < P; i++) {
+                if (a.h) {
+                    uint64_t y = mul2(hh.v[i], post.v[i]);
+                    if (full_gate) y = mul2(y, av.v[i]);
+                    x.v[i] = fma2(k, y, x.v[i]);
                 }
-            row_sum(m, tpr, sh, flip);
-            const float mu = m[0] * inv_d;
-#pragma unroll
-            for (int i = 0; i < NIT; i++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) t[i][e] += rx * (u[i][e] - x[i][e] * mu);
-        }
-#pragma unroll
-        for (int i = 0; i < NIT; i++) {
-            const int c = c0 + i * step;
-            if (on && c < D && a.dx) store_f32((T *)a.dx + r * a.D + c, t[i]);
-        }
-        if (a.h) {
-            float m[2] = {0.0f, 0.0f};  // mean of w * hh; the row gate's sum of t * y
-#pragma unroll
-            for (int i = 0; i < NIT; i++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const float st = a.scale * t[i][e], sh_ = st * hh[i][e];
-                    float av = arow;
-                    if (full_gate) {
-                        av = act_value(a.act, gt[i][e], sg[i][e]);
-                        gt[i][e] = sh_ * post[i][e] * act_grad(a.act, gt[i][e], sg[i][e]);
-                    }
-                    if (row_gate) m[1] += sh_ * post[i][e];
-                    dpost[i][e] += av * sh_;
-                    t[i][e] = st * av * post[i][e];
-                    m[0] += t[i][e] * hh[i][e];
-                }
-            row_sum(m, tpr, sh, flip);
-            const float mw = m[0] * inv_d;
-#pragma unroll
-            for (int i = 0; i < NIT; i++) {
-                const int c = c0 + i * step;
-                if (!(on && c < D)) continue;
-                float d[VEC];
-#pragma unroll
-                for (int e = 0; e < VEC; e++) d[e] = rh * (t[i][e] - hh[i][e] * mw);
-                if (a.dh) store_f32((T *)a.dh + r * a.D + c, d);
-                if (full_gate && a.dgate) store_f32((T *)a.dgate + r * a.D + c, gt[i]);
+                x.v[i] = mul2(x.v[i], kx);
+                dpre.v[i] = fma2(u.v[i], x.v[i], dpre.v[i]);
+                u.v[i] = mul2(u.v[i], pre.v[i]);
+                m2 = fma2(u.v[i], x.v[i], m2);
             }
-            if (row_gate && a.dgate && on && lane == 0) ((T *)a.dgate)[r] = from_f32<T>(m[1] * darow);
+            float m[1] = {sum_of(m2)};
+            row_sum(m, tpr, sh, flip);
+            const float mu = -m[0] * inv_d;
+            const uint64_t mm = two(mu, mu);
+#pragma unroll
+            for (int i = 0; i < P; i++) t.v[i] = fma2(kx, fma2(x.v[i], mm, u.v[i]), t.v[i]);
+        }
+        if (on && a.dx) store_row(t, a.dx, r * a.D, c0, step, D);
+        if (a.h) {
+            const uint64_t k = two(a.scale, a.scale), ka = two(arow, arow);
+            uint64_t m2 = 0, row2 = 0;
+#pragma unroll
+            for (int i = 0; i < P; i++) {
+                const uint64_t st = mul2(t.v[i], k), sh_ = mul2(st, hh.v[i]), ty = mul2(sh_, post.v[i]);
+                const uint64_t ai = full_gate ? av.v[i] : ka;
+                if (full_gate) da.v[i] = mul2(ty, da.v[i]);
+                if (row_gate) row2 = add2(row2, ty);
+                dpost.v[i] = fma2(ai, sh_, dpost.v[i]);
+                t.v[i] = mul2(mul2(st, ai), post.v[i]);
+                m2 = fma2(t.v[i], hh.v[i], m2);
+            }
+            if (on && full_gate && a.dgate) store_row(da, a.dgate, r * a.D, c0, step, D);
+            float m[2] = {sum_of(m2), row_gate ? sum_of(row2) : 0.0f};
+            row_sum(m, tpr, sh, flip);
+            const float mw = -m[0] * inv_d;
+            const uint64_t mm = two(mw, mw), kh = two(rh, rh);
+#pragma unroll
+            for (int i = 0; i < P; i++) t.v[i] = mul2(kh, fma2(hh.v[i], mm, t.v[i]));
+            if (on && a.dh) store_row(t, a.dh, r * a.D, c0, step, D);
+            if (row_gate && a.dgate && on && lane == 0) ((T *)a.dgate)[r] = from_f32<T>(m[1] * act_grad(a.act, grow));
         }
     }
     if (!a.part) return;
     // the block's sums: its groups' parts added in order
     float *part = a.part + (int64_t)blockIdx.x * 2 * D, *mine = groups > 1 ? ng_part + g * 2 * D : part;
 #pragma unroll
-    for (int i = 0; i < NIT; i++) {
-        const int c = c0 + i * step;
+    for (int i = 0; i < VEC * NIT; i++) {
+        const int c = c0 + i / VEC * step + i % VEC;
+        float f[2], q[2];
+        both(dpost.v[i / 2], f[0], f[1]);
+        both(dpre.v[i / 2], q[0], q[1]);
         if (c < D) {
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                mine[c + e] = dpost[i][e];
-                mine[D + c + e] = dpre[i][e];
-            }
+            mine[c] = f[i % 2];
+            mine[D + c] = q[i % 2];
         }
     }
     if (groups > 1) {
@@ -438,18 +449,18 @@ bool norm_shape(int64_t D, bool wide, int elem, NormShape &s)
 int64_t norm_blocks(const NormShape &s, int64_t R, bool bwd)
 {
     const int64_t groups = s.threads / s.tpr;
-    const int64_t per_sm = s.threads == kNgMaxThreads || s.vec * s.nit > 8 ? 1 : bwd ? 2 : 3;
+    const int64_t per_sm = norm_blocks_per_sm(bwd, s.threads, s.vec, s.nit);
     return std::max<int64_t>(1, std::min<int64_t>((R + groups - 1) / groups, kNgSms * per_sm));
 }
 
-template <typename T, int VEC, int NIT, int MAXT, int GATE>
+template <typename T, int VEC, int NIT, int MAXT, int GATE, int ACT = -1>
 void norm_launch(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
 {
     const unsigned blocks = (unsigned)norm_blocks(sh, a.R, bwd);
     const size_t groups = sh.threads / sh.tpr, smem = groups > 1 && a.part ? groups * 2 * a.D * 4 : 0;  // 32 KB at most
     count_launches(1);
-    if (bwd) k_norm_bwd<T, VEC, NIT, MAXT, GATE><<<blocks, MAXT, smem, s>>>(a, sh.tpr);
-    else k_norm_fwd<T, VEC, NIT, MAXT, GATE><<<blocks, MAXT, 0, s>>>(a, sh.tpr);
+    if (bwd) k_norm_bwd<T, VEC, NIT, MAXT, GATE, ACT><<<blocks, MAXT, smem, s>>>(a, sh.tpr);
+    else k_norm_fwd<T, VEC, NIT, MAXT, GATE, ACT><<<blocks, MAXT, 0, s>>>(a, sh.tpr);
 }
 
 template <typename T, int VEC, int NIT>
@@ -463,8 +474,12 @@ void norm_gate(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
         norm_launch<T, VEC, NIT, kNgThreads, 0>(bwd, a, sh, s);
     } else if (a.gate_row) {
         norm_launch<T, VEC, NIT, kNgThreads, 2>(bwd, a, sh, s);
+    } else if (a.act == kActSilu) {
+        norm_launch<T, VEC, NIT, kNgThreads, 1, kActSilu>(bwd, a, sh, s);
+    } else if (a.act == kActSigmoid) {
+        norm_launch<T, VEC, NIT, kNgThreads, 1, kActSigmoid>(bwd, a, sh, s);
     } else {
-        norm_launch<T, VEC, NIT, kNgThreads, 1>(bwd, a, sh, s);
+        norm_launch<T, VEC, NIT, kNgThreads, 1, kActLinear>(bwd, a, sh, s);
     }
 }
 

@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import DTYPES, addr, check, need_cuda, on_device, stream_of
+from ._lib import DTYPES, addr, check, need_cuda, on_device, raw_stream
 
 
 def _forward(tokens, weight, scale):
@@ -22,7 +22,7 @@ def _forward(tokens, weight, scale):
     y = torch.empty(*tokens.shape, D, dtype=weight.dtype, device=weight.device)
     with on_device(weight):
         check(_lib.load().lifb_embed_fwd(addr(tokens), tokens.element_size(), addr(weight), addr(y), n, V, D,
-                                         max(weight.stride(0), D), scale, DTYPES[weight.dtype], stream_of(weight)),
+                                         max(weight.stride(0), D), scale, DTYPES[weight.dtype], raw_stream(weight)),
               "embedding")
     return y
 
@@ -49,7 +49,7 @@ class Embedding(torch.autograd.Function):
             nb = lib.lifb_embed_bwd_workspace_bytes(n, V, D)
             ws = torch.empty(nb, dtype=torch.uint8, device=dy.device)
             check(lib.lifb_embed_bwd(addr(tokens), tokens.element_size(), addr(dy), addr(dw), n, V, D,
-                                     max(dy.stride(0), D), scale, DTYPES[dtype], addr(ws), nb, stream_of(dy)),
+                                     max(dy.stride(0), D), scale, DTYPES[dtype], addr(ws), nb, raw_stream(dy)),
                   "embedding")
             _lib.poll_device("embedding")
         return None, dw, None

@@ -21,13 +21,13 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import DTYPES, addr, check, need_cuda, on_device, stream_of
+from ._lib import DTYPES, addr, check, need_cuda, on_device, raw_stream
 
 MAX_WIDTH = 128
 
 
 def _last_dense(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    return t if t.stride(-1) == 1 else t.contiguous()
 
 
 def _pack(q, k, v, log_decay, state, lengths, scale):
@@ -48,7 +48,7 @@ def _forward(q, k, v, log_decay, state, lengths, scale, return_state):
     with on_device(q):
         nb = lib.lifb_leaky_attn_workspace_bytes(args, 0)
         ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        check(lib.lifb_leaky_attn_fwd(args, addr(o), addr(out), addr(ws), nb, stream_of(q)), "leaky_attention")
+        check(lib.lifb_leaky_attn_fwd(args, addr(o), addr(out), addr(ws), nb, raw_stream(q)), "leaky_attention")
     return o, out
 
 
@@ -80,27 +80,33 @@ class LeakyAttention(torch.autograd.Function):
             nb = lib.lifb_leaky_attn_workspace_bytes(args, 1)
             ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
             check(lib.lifb_leaky_attn_bwd(args, addr(do), (_lib.c_i64 * 3)(*do.stride()[:3]), addr(dout), addr(dq),
-                                          addr(dk), addr(dv), addr(ds), addr(ws), nb, stream_of(q)),
+                                          addr(dk), addr(dv), addr(ds), addr(ws), nb, raw_stream(q)),
                   "leaky_attention")
             _lib.poll_device("leaky_attention")
         return dq, dk, dv, None, ds, None, None, None
 
 
+_SEQ_TYPES = (torch.float32, torch.bfloat16)
+_STEP_TYPES = tuple(DTYPES)
+
+
 def _check(what, q, k, v, log_decay, lead, types):
-    if q.dim() != lead + 2 or k.dim() != lead + 2 or v.dim() != lead + 2:
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if not len(qs) == len(ks) == len(vs) == lead + 2:
         raise ValueError(f"{what}: q, k and v must have {lead + 2} dimensions")
-    H, Dk = q.shape[lead:]
-    Hk, Dv = v.shape[lead:]
-    if k.shape[:lead] != q.shape[:lead] or v.shape[:lead] != q.shape[:lead] or k.shape[lead:] != (Hk, Dk):
-        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
-    if Hk == 0 and H > 0 or Hk > 0 and H % Hk:
+    H, Dk = qs[lead:]
+    Hk, Dv = vs[lead:]
+    if ks[:lead] != qs[:lead] or vs[:lead] != qs[:lead] or ks[lead] != Hk or ks[lead + 1] != Dk:
+        raise ValueError(f"{what}: q {tuple(qs)}, k {tuple(ks)} and v {tuple(vs)} do not fit")
+    if H % Hk if Hk else H:
         raise ValueError(f"{what}: {H} heads cannot share {Hk} key/value heads")
     if Dk > MAX_WIDTH or Dv > MAX_WIDTH:
         raise ValueError(f"{what}: head widths {Dk} and {Dv}; at most {MAX_WIDTH}")
-    if q.dtype not in types or k.dtype != q.dtype or v.dtype != q.dtype:
+    dt = q.dtype
+    if dt not in types or k.dtype != dt or v.dtype != dt:
         raise TypeError(f"{what}: q, k and v must share one of {', '.join(str(t) for t in types)}, got {q.dtype}, "
                         f"{k.dtype}, {v.dtype}")
-    if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
+    if log_decay.dim() != 1 or log_decay.shape[0] != H or log_decay.dtype != torch.float32:
         raise ValueError(f"{what}: log_decay must be [{H}] fp32, got {tuple(log_decay.shape)} {log_decay.dtype}")
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: the decay is a constant and gets no gradient: pass log_decay.detach()")
@@ -115,7 +121,7 @@ def leaky_attention(q, k, v, log_decay, state=None, lengths=None, scale=None, re
     zeros and leave the state alone.  scale: Dk ** -0.5 by default.  Gradients for
     q, k, v and state."""
     what = "leaky_attention"
-    H, _, Dk, Dv = _check(what, q, k, v, log_decay, 2, (torch.float32, torch.bfloat16))
+    H, _, Dk, Dv = _check(what, q, k, v, log_decay, 2, _SEQ_TYPES)
     need_cuda(what, q=q, k=k, v=v, log_decay=log_decay, state=state, lengths=lengths)
     B = q.shape[0]
     if state is not None:
@@ -146,7 +152,7 @@ def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     (None: its own index), at most one sequence to a slot; a place outside the
     cache (-1, say) is empty: zeros out, nothing changed.  Not differentiable."""
     what = "leaky_attention_step"
-    H, Hk, Dk, Dv = _check(what, q, k, v, log_decay, 1, tuple(DTYPES))
+    H, Hk, Dk, Dv = _check(what, q, k, v, log_decay, 1, _STEP_TYPES)
     need_cuda(what, q=q, k=k, v=v, log_decay=log_decay, state=state, slots=slots)
     B = q.shape[0]
     if state.dim() != 4 or state.shape[1:] != (H, Dk, Dv) or state.dtype != torch.float32:
@@ -165,10 +171,13 @@ def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
         raise RuntimeError(f"{what} is not differentiable: use leaky_attention, or torch.no_grad()")
     q, k, v, log_decay = _last_dense(q), _last_dense(k), _last_dense(v), log_decay.contiguous()
     scale = float(Dk) ** -0.5 if scale is None and Dk > 0 else float(scale or 0.0)
-    o = torch.empty(B, H, Dv, dtype=q.dtype, device=q.device)
-    args = _lib.LEAKY_ATTN_STEP.pack(addr(q), addr(k), addr(v), addr(log_decay), addr(slots), B, H, Hk, Dk, Dv,
-                                     state.shape[0], *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *st[:2],
-                                     scale, DTYPES[q.dtype])
+    o = q.new_empty((B, H, Dv))
+    q0, q1, _ = q.stride()
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
+    args = _lib.LEAKY_ATTN_STEP.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), addr(slots), B, H,
+                                     Hk, Dk, Dv, state.shape[0], q0, q1, k0, k1, v0, v1, st[0], st[1], scale,
+                                     DTYPES[q.dtype])
     with on_device(q):
-        check(_lib.load().lifb_leaky_attn_step(args, addr(o), addr(state), stream_of(q)), what)
+        check(_lib.load().lifb_leaky_attn_step(args, addr(o), addr(state), raw_stream(q)), what)
     return o

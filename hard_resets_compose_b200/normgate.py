@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import DTYPES, addr, check, need_cuda, on_device, stream_of
+from ._lib import DTYPES, addr, check, need_cuda, on_device, raw_stream
 
 ACTS = {"silu": 0, "sigmoid": 1, "none": 2}
 MAX_WIDTH = 8192
@@ -50,7 +50,7 @@ def _forward(x, h, gate, post, pre, scale, eps, act, keep):
     rstd = torch.empty(2, R, device=x.device) if keep else None
     with on_device(x):
         check(_lib.load().lifb_norm_gate_fwd(_pack(x, h, gate, post, pre, rstd, scale, eps, act), addr(xo), addr(n),
-                                             stream_of(x)), "norm_gate_residual")
+                                             raw_stream(x)), "norm_gate_residual")
     return xo, n, rstd
 
 
@@ -88,7 +88,7 @@ class NormGateResidual(torch.autograd.Function):
             check(lib.lifb_norm_gate_bwd(_pack(x, h, gate, post, pre, rstd, *ctx.cfg), addr(dxo),
                                          D if dxo is None else dxo.stride(0), addr(dn),
                                          D if dn is None else dn.stride(0), addr(dx), addr(dh), addr(dgate),
-                                         addr(dpost), addr(dpre), addr(ws), nb, stream_of(x)), "norm_gate_residual")
+                                         addr(dpost), addr(dpre), addr(ws), nb, raw_stream(x)), "norm_gate_residual")
         return dx, dh, dgate, dpost, dpre, None, None, None
 
 
