@@ -6,8 +6,8 @@
 // Both are bound by memory: the forward reads at most n rows and writes n, the
 // gradient reads n rows and writes all V.  The gradient's sums run in an order
 // that the tokens alone fix, so it gives the same bits each time: the token
-// positions are sorted by token (a stable radix sort: digits of up to 10
-// bits, one counting and one placing launch a digit), the sorted positions are
+// positions are sorted by token (a stable radix sort: digits of 8 to 10 bits, one
+// counting and one placing launch a digit, one alone for up to kEmMinTile tokens), the sorted positions are
 // cut into pieces of kEmPiece, and a piece adds its rows one after another in
 // fp32.  A token whose positions lie within a piece is finished there; one that
 // reaches over a piece's edge leaves that piece's part (fp32) to a last launch
@@ -26,9 +26,11 @@ namespace {
 
 constexpr int kEmThreads = 256;
 constexpr int kEmWarps = kEmThreads / 32;
-constexpr int kEmMaxBits = 10;       // digit size: 1024 bins, 4 a thread
-constexpr int kEmMaxBlocks = 128;    // sorting blocks: each sums the counts of all of them
-constexpr int kEmMinTile = 512;      // tokens a sorting block takes at least
+constexpr int kEmMaxBits = 10;       // digit size: at most 1024 bins, 4 a thread
+constexpr int kEmMinBits = 8;        // and at least 256, one a thread
+constexpr int kEmMaxBlocks = 64;     // sorting blocks: each sums the counts of all of them
+constexpr int kEmMinTile = 1024;     // tokens a sorting block takes at least
+constexpr int kEmRows = 4;           // rows of the forward a thread
 constexpr int kEmPiece = 64;         // sorted positions summed by one block
 
 struct EmbedPlan {
@@ -42,7 +44,7 @@ EmbedPlan plan_of(int64_t n, int64_t V)
     p.bits = 1;  // keys 0..V: V marks tokens without a row
     while ((int64_t(1) << p.bits) <= V) p.bits++;
     p.passes = (p.bits + kEmMaxBits - 1) / kEmMaxBits;
-    p.radix_bits = (p.bits + p.passes - 1) / p.passes;
+    p.radix_bits = std::max(kEmMinBits, (p.bits + p.passes - 1) / p.passes);
     p.tile = std::max<int64_t>(kEmMinTile, (n + kEmMaxBlocks - 1) / kEmMaxBlocks);
     p.tile = (p.tile + kEmThreads - 1) / kEmThreads * kEmThreads;
     p.blocks = (int)((n + p.tile - 1) / p.tile);
@@ -82,30 +84,50 @@ EmbedWs carve(void *base, int64_t n, int64_t V, int64_t D)
 
 }  // namespace
 
-// y = scale * W[token]; VEC elements a thread.  A token past the table gives
-// zeros and sets the device status.
+// y = scale * W[token]: a block has blockDim.x vectors of VEC columns by blockDim.y
+// rows, kEmRows of them a thread (their loads in flight together).  A token past the
+// table gives zeros and sets the device status.
 template <typename T, typename Tok, int VEC>
 __global__ void __launch_bounds__(256) k_embed_fwd(const Tok *__restrict__ tokens, const T *__restrict__ W,
                                                    T *__restrict__ Y, int64_t n, int64_t V, int64_t D,
                                                    int64_t w_stride, float scale, int *status)
 {
-    const int64_t per = D / VEC;
-    const int64_t step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; at < n * per; at += step) {
-        const int64_t row = at / per, c = (at - row * per) * VEC;
-        const int64_t tok = (int64_t)tokens[row];
-        float x[VEC];
-        if (tok >= 0 && tok < V) {
-            load_f32(W + tok * w_stride + c, x);
+    const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+    const int64_t r0 = (int64_t)blockIdx.x * blockDim.y * kEmRows + threadIdx.y;
+    int64_t tok[kEmRows];
 #pragma unroll
-            for (int i = 0; i < VEC; i++) x[i] *= scale;
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; i++) x[i] = 0.0f;
-            if (tok >= V && c == 0) atomicExch(status, kStatusTokenRange);
+    for (int i = 0; i < kEmRows; i++) {
+        const int64_t r = r0 + (int64_t)i * blockDim.y;
+        tok[i] = r < n ? (int64_t)tokens[r] : -1;
+        if (tok[i] >= V) {
+            if (c == 0) atomicExch(status, kStatusTokenRange);
+            tok[i] = -1;
         }
-        store_f32(Y + row * D + c, x);
     }
+    if (c >= D) return;
+    float x[kEmRows][VEC];
+#pragma unroll
+    for (int i = 0; i < kEmRows; i++) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) x[i][e] = 0.0f;
+        if (tok[i] >= 0) load_f32(W + tok[i] * w_stride + c, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kEmRows; i++) {
+        const int64_t r = r0 + (int64_t)i * blockDim.y;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) x[i][e] *= scale;
+        if (r < n) store_f32(Y + r * D + c, x[i]);
+    }
+}
+
+// A token's key: itself, or V where it has no row.
+template <typename Tok>
+__device__ __forceinline__ int32_t embed_key(const Tok *tokens, int64_t i, int64_t V, int *status)
+{
+    const int64_t tok = (int64_t)tokens[i];
+    if (tok >= V) atomicExch(status, kStatusTokenRange);
+    return tok >= 0 && tok < V ? (int32_t)tok : (int32_t)V;
 }
 
 // Counts the digits of each block's tokens: counts[block][digit].  The first
@@ -127,9 +149,7 @@ __global__ void __launch_bounds__(kEmThreads)
     for (int64_t i = i0 + threadIdx.x; i < i1; i += kEmThreads) {
         int32_t k;
         if (FIRST) {
-            const int64_t tok = (int64_t)tokens[i];
-            if (tok >= V) atomicExch(status, kStatusTokenRange);
-            k = tok >= 0 && tok < V ? (int32_t)tok : (int32_t)V;
+            k = embed_key(tokens, i, V, status);
             key[i] = k;
         } else {
             k = key[i];
@@ -143,37 +163,59 @@ __global__ void __launch_bounds__(kEmThreads)
 // Places each block's tokens, in order, at their digit's place: the number of
 // smaller digits, of this digit in earlier blocks, in earlier warps of the
 // block (each warp owns a contiguous part of the tile), and before it in the warp.
-template <bool FIRST, bool LAST>
+// PER digits a thread.  ALONE: one block has all tokens; it counts for itself (and in
+// the first digit's launch makes the keys and clears `present`).
+template <typename Tok, int PER, bool FIRST, bool ALONE>
 __global__ void __launch_bounds__(kEmThreads)
-    k_embed_place(const int32_t *__restrict__ key, const int32_t *__restrict__ pos, int32_t *__restrict__ key_out,
-                  int32_t *__restrict__ pos_out, const int32_t *__restrict__ counts, uint8_t *__restrict__ present,
-                  int64_t n, int64_t V, int64_t tile, int shift, int radix_bits)
+    k_embed_place(const Tok *__restrict__ tokens, const int32_t *__restrict__ key, const int32_t *__restrict__ pos,
+                  int32_t *__restrict__ key_out, int32_t *__restrict__ pos_out, const int32_t *__restrict__ counts,
+                  uint8_t *__restrict__ present, int64_t n, int64_t V, int64_t tile, int shift, int last, int *status)
 {
+    constexpr int radix = PER * kEmThreads;
     extern __shared__ int32_t em_smem[];
-    const int radix = 1 << radix_bits;
-    int32_t *base = em_smem;           // [radix]
-    int32_t *whist = em_smem + radix;  // [warps][radix]
+    int32_t *whist = em_smem;  // [warps][radix]
     __shared__ int32_t warp_sum[kEmWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto key_at = [&](int64_t i) {
+        if constexpr (FIRST && ALONE) return embed_key(tokens, i, V, status);
+        else return key[i];
+    };
     for (int i = tid; i < kEmWarps * radix; i += kEmThreads) whist[i] = 0;
+    if (FIRST && ALONE)
+        for (int64_t v = tid; v < V; v += kEmThreads) present[v] = 0;
+    __syncthreads();
 
-    // counts of this digit in all blocks and in the earlier ones; per = 4 at most
-    const int per = (radix + kEmThreads - 1) / kEmThreads;
-    int32_t total[(1 << kEmMaxBits) / kEmThreads], before[(1 << kEmMaxBits) / kEmThreads];
-    int32_t mine = 0;
+    // digits of each warp's part
+    const int64_t part = tile / kEmWarps;  // a multiple of 32
+    const int64_t i0 = blockIdx.x * tile + warp * part, i1 = min(n, i0 + part);
+    int32_t *wh = whist + warp * radix;
+    for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&wh[(key_at(i) >> shift) & (radix - 1)], 1);
+
+    // counts of this thread's digits in all blocks and in the earlier ones
+    struct alignas(4 * PER) Counts {
+        int32_t c[PER];
+    };
+    Counts total = {}, before = {};
+    if (ALONE) {
+        __syncthreads();
+        for (int w = 0; w < kEmWarps; w++)
 #pragma unroll
-    for (int e = 0; e < (1 << kEmMaxBits) / kEmThreads; e++) {
-        total[e] = before[e] = 0;
-        const int d = tid * per + e;
-        if (e < per && d < radix) {
-            for (int b = 0; b < (int)gridDim.x; b++) {
-                const int32_t c = counts[(int64_t)b * radix + d];
-                total[e] += c;
-                if (b < (int)blockIdx.x) before[e] += c;
+            for (int e = 0; e < PER; e++) total.c[e] += whist[w * radix + tid * PER + e];
+    } else {
+        const Counts *at = reinterpret_cast<const Counts *>(counts) + tid;
+#pragma unroll 8
+        for (int b = 0; b < (int)gridDim.x; b++) {
+            const Counts x = at[(int64_t)b * kEmThreads];
+#pragma unroll
+            for (int e = 0; e < PER; e++) {
+                total.c[e] += x.c[e];
+                if (b < (int)blockIdx.x) before.c[e] += x.c[e];
             }
         }
-        mine += total[e];
     }
+    int32_t mine = 0;
+#pragma unroll
+    for (int e = 0; e < PER; e++) mine += total.c[e];
     int32_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -184,22 +226,12 @@ __global__ void __launch_bounds__(kEmThreads)
     __syncthreads();
     int32_t start = incl - mine;
     for (int w = 0; w < warp; w++) start += warp_sum[w];
-#pragma unroll
-    for (int e = 0; e < (1 << kEmMaxBits) / kEmThreads; e++) {
-        const int d = tid * per + e;
-        if (e < per && d < radix) base[d] = start + before[e];
-        start += total[e];
-    }
-
-    // digits of each warp's part
-    const int64_t part = tile / kEmWarps;  // a multiple of 32
-    const int64_t i0 = blockIdx.x * tile + warp * part, i1 = min(n, i0 + part);
-    int32_t *wh = whist + warp * radix;
-    for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&wh[(key[i] >> shift) & (radix - 1)], 1);
-    __syncthreads();
     // each warp's first place of each digit
-    for (int d = tid; d < radix; d += kEmThreads) {
-        int32_t s = base[d];
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+        const int d = tid * PER + e;
+        int32_t s = start + before.c[e];
+        start += total.c[e];
         for (int w = 0; w < kEmWarps; w++) {
             const int32_t c = whist[w * radix + d];
             whist[w * radix + d] = s;
@@ -209,7 +241,7 @@ __global__ void __launch_bounds__(kEmThreads)
     __syncthreads();
     for (int64_t i = i0; i < i1; i += 32) {  // uniform over the warp
         const bool on = i + lane < i1;
-        const int32_t k = on ? key[i + lane] : 0;
+        const int32_t k = on ? key_at(i + lane) : 0;
         const int d = on ? (k >> shift) & (radix - 1) : -1;
         const unsigned same = __match_any_sync(~0u, d);
         const int rank = __popc(same & ((1u << lane) - 1));
@@ -221,7 +253,7 @@ __global__ void __launch_bounds__(kEmThreads)
         if (on) {
             key_out[at] = k;
             pos_out[at] = FIRST ? (int32_t)(i + lane) : pos[i + lane];
-            if (LAST && k < V) present[k] = 1;
+            if (last && k < V) present[k] = 1;
         }
     }
 }
@@ -238,13 +270,19 @@ __global__ void __launch_bounds__(256)
     __shared__ int32_t s_key[kEmPiece + 2], s_pos[kEmPiece];
     const int tid = threadIdx.x;
     if (blockIdx.x >= pieces) {
+        // 32 rows' marks at a time
         const int64_t per = D / VEC, nz = gridDim.x - pieces, z = blockIdx.x - pieces;
+        const int lane = tid & 31;
         float zero[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; i++) zero[i] = 0.0f;
-        for (int64_t v = z; v < V; v += nz) {
-            if (present[v]) continue;
-            for (int64_t c = tid; c < per; c += blockDim.x) store_f32(dW + v * D + c * VEC, zero);
+        for (int64_t v0 = z * 32; v0 < V; v0 += nz * 32) {
+            unsigned absent = __ballot_sync(~0u, v0 + lane < V && !present[min(v0 + lane, V - 1)]);
+            while (absent) {
+                const int64_t v = v0 + __ffs(absent) - 1;
+                absent &= absent - 1;
+                for (int64_t c = tid; c < per; c += blockDim.x) store_f32(dW + v * D + c * VEC, zero);
+            }
         }
         return;
     }
@@ -310,6 +348,7 @@ __global__ void __launch_bounds__(256)
     __shared__ int64_t s_last;
     if (threadIdx.x == 0) {  // the last piece that it reaches: the first one after whose end key is not k
         int64_t lo = p + 1, hi = pieces - 1;
+        if (key[min(n, (p + 2) * kEmPiece) - 1] != k) hi = lo;  // mostly
         while (lo < hi) {
             const int64_t mid = (lo + hi) / 2;
             if (key[min(n, (mid + 1) * kEmPiece) - 1] == k) lo = mid + 1;
@@ -323,6 +362,7 @@ __global__ void __launch_bounds__(256)
     for (int64_t c = (int64_t)threadIdx.x * VEC; c < D; c += (int64_t)blockDim.x * VEC) {
         float acc[VEC];
         load_f32(tail + p * D + c, acc);
+#pragma unroll 8
         for (int64_t q = p + 1; q <= last; q++) {
             float x[VEC];
             load_f32(head + q * D + c, x);
@@ -346,10 +386,12 @@ template <typename T, typename Tok, int VEC>
 void embed_fwd(const void *tokens, const void *W, void *Y, int64_t n, int64_t V, int64_t D, int64_t w_stride,
                float scale, cudaStream_t s)
 {
-    const int64_t blocks = std::min<int64_t>((n * (D / VEC) + 255) / 256, 148 * 64);
+    const int64_t vecs = (D + VEC - 1) / VEC;
+    const unsigned x = vecs >= 256 ? 256 : round_threads(vecs), y = 256 / x;
+    const dim3 grid((unsigned)((n + y * kEmRows - 1) / (y * kEmRows)), (unsigned)((vecs + x - 1) / x));
     count_launches(1);
-    k_embed_fwd<T, Tok, VEC><<<(unsigned)blocks, 256, 0, s>>>((const Tok *)tokens, (const T *)W, (T *)Y, n, V, D,
-                                                              w_stride, scale, device_status_ptr());
+    k_embed_fwd<T, Tok, VEC><<<grid, dim3(x, y), 0, s>>>((const Tok *)tokens, (const T *)W, (T *)Y, n, V, D, w_stride,
+                                                         scale, device_status_ptr());
 }
 
 template <typename T, int VEC>
@@ -357,7 +399,7 @@ void embed_sum(const EmbedWs &w, int last, const EmbedPlan &p, const void *dY, v
                int64_t D, int64_t dy_stride, float scale, cudaStream_t s)
 {
     const unsigned threads = round_threads((D + VEC - 1) / VEC);
-    const int64_t zero_blocks = std::min<int64_t>(V, 148 * 8);
+    const int64_t zero_blocks = std::min<int64_t>((V + 31) / 32, 148 * 8);
     count_launches(2);
     k_embed_sum<T, VEC><<<(unsigned)(p.pieces + zero_blocks), threads, 0, s>>>(
         w.key[last], w.pos[last], (const T *)dY, (T *)dW, w.head, w.tail, w.present, n, V, D, dy_stride, p.pieces,
@@ -366,29 +408,38 @@ void embed_sum(const EmbedWs &w, int last, const EmbedPlan &p, const void *dY, v
                                                                 p.pieces, scale);
 }
 
-template <typename Tok>
+template <typename Tok, int PER>
 int embed_sort(const EmbedWs &w, const EmbedPlan &p, const void *tokens, int64_t n, int64_t V, cudaStream_t s)
 {
-    const size_t smem = (size_t)(1 + kEmWarps) * (1 << p.radix_bits) * 4;  // 36 KB at most
+    const size_t smem = (size_t)kEmWarps * (1 << p.radix_bits) * 4;  // 32 KB at most
     int cur = 0;
     for (int pass = 0; pass < p.passes; pass++) {
         const int shift = pass * p.radix_bits;
-        const bool first = pass == 0, last = pass == p.passes - 1;
-        count_launches(2);
-        if (first)
-            k_embed_count<Tok, true><<<p.blocks, kEmThreads, 0, s>>>((const Tok *)tokens, w.key[cur], w.counts, w.present,
-                                                                     n, V, p.tile, shift, p.radix_bits,
-                                                                     device_status_ptr());
-        else
-            k_embed_count<Tok, false><<<p.blocks, kEmThreads, 0, s>>>(nullptr, w.key[cur], w.counts, w.present, n, V,
-                                                                      p.tile, shift, p.radix_bits, nullptr);
-        auto place = first ? (last ? k_embed_place<true, true> : k_embed_place<true, false>)
-                           : (last ? k_embed_place<false, true> : k_embed_place<false, false>);
-        place<<<p.blocks, kEmThreads, smem, s>>>(w.key[cur], w.pos[cur], w.key[cur ^ 1], w.pos[cur ^ 1], w.counts,
-                                                 w.present, n, V, p.tile, shift, p.radix_bits);
+        const bool first = pass == 0, alone = p.blocks == 1;
+        const Tok *tok = (const Tok *)tokens;
+        if (!alone) {
+            count_launches(1);
+            auto count = first ? k_embed_count<Tok, true> : k_embed_count<Tok, false>;
+            count<<<p.blocks, kEmThreads, 0, s>>>(tok, w.key[cur], w.counts, w.present, n, V, p.tile, shift,
+                                                  p.radix_bits, device_status_ptr());
+        }
+        auto place = first ? (alone ? k_embed_place<Tok, PER, true, true> : k_embed_place<Tok, PER, true, false>)
+                           : (alone ? k_embed_place<Tok, PER, false, true> : k_embed_place<Tok, PER, false, false>);
+        count_launches(1);
+        place<<<p.blocks, kEmThreads, smem, s>>>(tok, w.key[cur], w.pos[cur], w.key[cur ^ 1], w.pos[cur ^ 1], w.counts,
+                                                 w.present, n, V, p.tile, shift, pass == p.passes - 1,
+                                                 device_status_ptr());
         cur ^= 1;
     }
     return cur;
+}
+
+template <typename Tok>
+int embed_sort(const EmbedWs &w, const EmbedPlan &p, const void *tokens, int64_t n, int64_t V, cudaStream_t s)
+{
+    return p.radix_bits == 8   ? embed_sort<Tok, 1>(w, p, tokens, n, V, s)
+           : p.radix_bits == 9 ? embed_sort<Tok, 2>(w, p, tokens, n, V, s)
+                               : embed_sort<Tok, 4>(w, p, tokens, n, V, s);
 }
 
 int embed_check(const char *what, const void *tokens, int token_bytes, const void *a, const void *b, int64_t n,
