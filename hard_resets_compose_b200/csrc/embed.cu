@@ -28,7 +28,10 @@ constexpr int kEmThreads = 256;
 constexpr int kEmWarps = kEmThreads / 32;
 constexpr int kEmMaxBits = 10;       // digit size: at most 1024 bins, 4 a thread
 constexpr int kEmMinBits = 8;        // and at least 256, one a thread
-constexpr int kEmMaxBlocks = 64;     // sorting blocks: each sums the counts of all of them
+// Sorting blocks: each reads the counts of all of them, from the same lines of L2 (64
+// blocks of 1024 digits: 27 us of it), so few, and more only where tokens are many.
+constexpr int kEmBlocks = 32, kEmBlocksMany = 64;
+constexpr int64_t kEmMany = 1 << 17;
 constexpr int kEmMinTile = 1024;     // tokens a sorting block takes at least
 constexpr int kEmRows = 4;           // rows of the forward a thread
 constexpr int kEmPiece = 64;         // sorted positions summed by one block
@@ -45,7 +48,8 @@ EmbedPlan plan_of(int64_t n, int64_t V)
     while ((int64_t(1) << p.bits) <= V) p.bits++;
     p.passes = (p.bits + kEmMaxBits - 1) / kEmMaxBits;
     p.radix_bits = std::max(kEmMinBits, (p.bits + p.passes - 1) / p.passes);
-    p.tile = std::max<int64_t>(kEmMinTile, (n + kEmMaxBlocks - 1) / kEmMaxBlocks);
+    const int most = n > kEmMany ? kEmBlocksMany : kEmBlocks;
+    p.tile = std::max<int64_t>(kEmMinTile, (n + most - 1) / most);
     p.tile = (p.tile + kEmThreads - 1) / kEmThreads * kEmThreads;
     p.blocks = (int)((n + p.tile - 1) / p.tile);
     p.pieces = (n + kEmPiece - 1) / kEmPiece;
@@ -146,6 +150,7 @@ __global__ void __launch_bounds__(kEmThreads)
             present[v] = 0;
     __syncthreads();
     const int64_t i0 = blockIdx.x * tile, i1 = min(n, i0 + tile);
+#pragma unroll 4
     for (int64_t i = i0 + threadIdx.x; i < i1; i += kEmThreads) {
         int32_t k;
         if (FIRST) {
@@ -189,7 +194,18 @@ __global__ void __launch_bounds__(kEmThreads)
     const int64_t part = tile / kEmWarps;  // a multiple of 32
     const int64_t i0 = blockIdx.x * tile + warp * part, i1 = min(n, i0 + part);
     int32_t *wh = whist + warp * radix;
-    for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&wh[(key_at(i) >> shift) & (radix - 1)], 1);
+    constexpr int U = 8;  // tokens of a lane loaded together
+    int32_t k8[U];
+    auto load_keys = [&](int64_t i) {
+#pragma unroll
+        for (int j = 0; j < U; j++) k8[j] = i + 32 * j + lane < i1 ? key_at(i + 32 * j + lane) : -1;
+    };
+    for (int64_t i = i0; i < i1; i += 32 * U) {
+        load_keys(i);
+#pragma unroll
+        for (int j = 0; j < U; j++)
+            if (k8[j] >= 0) atomicAdd(&wh[(k8[j] >> shift) & (radix - 1)], 1);
+    }
 
     // counts of this thread's digits in all blocks and in the earlier ones
     struct alignas(4 * PER) Counts {
@@ -239,21 +255,30 @@ __global__ void __launch_bounds__(kEmThreads)
         }
     }
     __syncthreads();
-    for (int64_t i = i0; i < i1; i += 32) {  // uniform over the warp
-        const bool on = i + lane < i1;
-        const int32_t k = on ? key_at(i + lane) : 0;
-        const int d = on ? (k >> shift) & (radix - 1) : -1;
-        const unsigned same = __match_any_sync(~0u, d);
-        const int rank = __popc(same & ((1u << lane) - 1));
-        int32_t at = 0;
-        if (on) at = wh[d] + rank;
-        __syncwarp();
-        if (on && rank == 0) wh[d] += __popc(same);
-        __syncwarp();
-        if (on) {
-            key_out[at] = k;
-            pos_out[at] = FIRST ? (int32_t)(i + lane) : pos[i + lane];
-            if (last && k < V) present[k] = 1;
+    for (int64_t i = i0; i < i1; i += 32 * U) {  // uniform over the warp
+        if (i1 - i0 > 32 * U) load_keys(i);      // else still there
+        int32_t from[U];
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const int64_t at = i + 32 * j + lane;
+            from[j] = FIRST ? (int32_t)at : k8[j] >= 0 ? pos[at] : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const bool on = k8[j] >= 0;
+            const int d = on ? (k8[j] >> shift) & (radix - 1) : -1;
+            const unsigned same = __match_any_sync(~0u, d);
+            const int rank = __popc(same & ((1u << lane) - 1));
+            int32_t at = 0;
+            if (on) at = wh[d] + rank;
+            __syncwarp();
+            if (on && rank == 0) wh[d] += __popc(same);
+            __syncwarp();
+            if (on) {
+                key_out[at] = k8[j];
+                pos_out[at] = from[j];
+                if (last && k8[j] < V) present[k8[j]] = 1;
+            }
         }
     }
 }
@@ -300,19 +325,21 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
         for (int e = 0; e < VEC; e++) acc[e] = 0.0f;
         int first = 0;  // where the current token's run starts in the piece
-        constexpr int U = 8;
+        constexpr int U = 16;  // rows in flight
         for (int i = 0; i < m; i += U) {
-            float x[U][VEC];
+            Pack<T, VEC> raw[U];
 #pragma unroll
             for (int u = 0; u < U; u++)
-                if (i + u < m && s_key[i + u + 1] < V) load_f32(dY + (int64_t)s_pos[i + u] * dy_stride + c, x[u]);
+                if (i + u < m && s_key[i + u + 1] < V) raw[u].load(dY + (int64_t)s_pos[i + u] * dy_stride + c);
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 if (i + u >= m) break;
                 const int32_t k = s_key[i + u + 1];
                 if (k >= V) break;  // the tokens without a row are last
+                float x[VEC];
+                raw[u].get(x);
 #pragma unroll
-                for (int e = 0; e < VEC; e++) acc[e] += x[u][e];
+                for (int e = 0; e < VEC; e++) acc[e] += x[e];
                 if (s_key[i + u + 2] != k || i + u == m - 1) {  // the run's end, or the piece's
                     if (first == 0 && from_before) {
                         store_f32(head + p * D + c, acc);
@@ -342,20 +369,27 @@ __global__ void __launch_bounds__(256)
 {
     const int64_t p = blockIdx.x, end = (p + 1) * kEmPiece;
     if (end >= n) return;
-    const int32_t k = key[end - 1];
-    if (k >= V || key[end] != k) return;                     // nothing goes on past this piece
-    if (p > 0 && key[p * kEmPiece - 1] == k) return;         // it starts in an earlier piece
+    const int32_t k = key[end - 1], after = key[end], before = p > 0 ? key[p * kEmPiece - 1] : -1;
+    if (k >= V || after != k) return;  // nothing goes on past this piece
+    if (before == k && key[p * kEmPiece] == k) return;  // it starts in an earlier piece
     __shared__ int64_t s_last;
-    if (threadIdx.x == 0) {  // the last piece that it reaches: the first one after whose end key is not k
+    if (threadIdx.x < 32) {
+        // The last piece that it reaches: the first one after p whose end is not k, if that
+        // begins with k (32 of them tested at a time).
         int64_t lo = p + 1, hi = pieces - 1;
-        if (key[min(n, (p + 2) * kEmPiece) - 1] != k) hi = lo;  // mostly
         while (lo < hi) {
-            const int64_t mid = (lo + hi) / 2;
-            if (key[min(n, (mid + 1) * kEmPiece) - 1] == k) lo = mid + 1;
-            else hi = mid;
+            const int64_t step = (hi - lo + 31) / 32, at = lo + threadIdx.x * step;
+            const unsigned past = __ballot_sync(~0u, at >= hi || key[min(n, (at + 1) * kEmPiece) - 1] != k);
+            const int first = __ffs(past) - 1;  // lane 31 is at or past hi only if step covers it
+            if (past == 0) {
+                lo = lo + 31 * step + 1;
+            } else {
+                const int64_t f = min(hi, lo + first * step);
+                lo = first == 0 ? lo : lo + (first - 1) * step + 1;
+                hi = f;
+            }
         }
-        // lo: the first piece from p + 1 on that does not end in k, or the last piece
-        s_last = key[lo * kEmPiece] == k ? lo : lo - 1;
+        if (threadIdx.x == 0) s_last = key[lo * kEmPiece] == k ? lo : lo - 1;
     }
     __syncthreads();
     const int64_t last = s_last;
