@@ -459,6 +459,7 @@ Split split_time(int64_t chains, int64_t T, int64_t room)
 int64_t attn_room(int64_t dq, int64_t dv, int dtype)
 {
     if (dtype == LIFB_BF16 && dq % 8 == 0 && dv % 8 == 0) return kAtSms;
+    if (dtype == LIFB_F32 && dq % 4 == 0 && dv % 4 == 0 && dq <= 64 && dv <= 64) return kAtSms;
     return kAtSms * 2 / std::max<int64_t>(1, (dv + kAtTile - 1) / kAtTile);
 }
 
@@ -511,9 +512,11 @@ int at_check(const char *what, const lifb_leaky_attn *p)
 
 bool run_passes(AttnArgs &a, int passes, int dtype, cudaStream_t s)
 {
-    const bool tc = attn_tc_applies(a, passes, dtype);
+    const bool tc = attn_tc_applies(a, passes, dtype), tc32 = attn_tc32_applies(a, passes, dtype);
     auto run = [&](bool state_only) {
-        return tc ? attn_tc(a, passes, state_only, s) : attn_simt(a, passes, dtype, state_only, s);
+        return tc     ? attn_tc(a, passes, state_only, s)
+               : tc32 ? attn_tc32(a, passes, state_only, s)
+                      : attn_simt(a, passes, dtype, state_only, s);
     };
     if (a.nseg > 1) {
         if (!run(true)) return false;

@@ -89,5 +89,8 @@ bool attn_simt(const AttnArgs &a, int passes, int dtype, bool state_only, cudaSt
 // can load (16-byte aligned strides, widths multiples of 8).
 bool attn_tc_applies(const AttnArgs &a, int passes, int dtype);
 bool attn_tc(const AttnArgs &a, int passes, bool state_only, cudaStream_t s);
+// leaky_attn_tc32.cu: the same for fp32 operands in 16-byte aligned vectors, widths up to 64.
+bool attn_tc32_applies(const AttnArgs &a, int passes, int dtype);
+bool attn_tc32(const AttnArgs &a, int passes, bool state_only, cudaStream_t s);
 
 }  // namespace lifb
