@@ -18,12 +18,12 @@ from ._lib import DTYPES, addr, check, need_cuda, on_device, raw_stream
 
 
 def _forward(tokens, weight, scale):
-    n, (V, D) = tokens.numel(), weight.shape
-    y = torch.empty(*tokens.shape, D, dtype=weight.dtype, device=weight.device)
+    V, D = weight.shape
+    y = weight.new_empty(tokens.shape + (D,))
     with on_device(weight):
-        check(_lib.load().lifb_embed_fwd(addr(tokens), tokens.element_size(), addr(weight), addr(y), n, V, D,
-                                         max(weight.stride(0), D), scale, DTYPES[weight.dtype], raw_stream(weight)),
-              "embedding")
+        check(_lib.load().lifb_embed_fwd(tokens.data_ptr(), tokens.element_size(), weight.data_ptr(), y.data_ptr(),
+                                         tokens.numel(), V, D, max(weight.stride(0), D), scale, DTYPES[weight.dtype],
+                                         raw_stream(weight)), "embedding")
     return y
 
 
@@ -40,16 +40,19 @@ class Embedding(torch.autograd.Function):
         tokens, = ctx.saved_tensors
         (V, D), dtype, scale = ctx.cfg
         n = tokens.numel()
-        dy = dy.reshape(n, D)
-        if dy.stride(-1) != 1 or dy.stride(0) < D:
+        if dy.dim() != 2:
+            dy = dy.reshape(n, D)
+        s0, s1 = dy.stride()
+        if s1 != 1 or s0 < D:
             dy = dy.contiguous()
-        dw = torch.empty(V, D, dtype=dtype, device=dy.device)
+            s0 = D
+        dw = dy.new_empty((V, D))
         lib = _lib.load()
         with on_device(dy):
             nb = lib.lifb_embed_bwd_workspace_bytes(n, V, D)
-            ws = torch.empty(nb, dtype=torch.uint8, device=dy.device)
+            ws = dy.new_empty(nb, dtype=torch.uint8)
             check(lib.lifb_embed_bwd(addr(tokens), tokens.element_size(), addr(dy), addr(dw), n, V, D,
-                                     max(dy.stride(0), D), scale, DTYPES[dtype], addr(ws), nb, raw_stream(dy)),
+                                     max(s0, D), scale, DTYPES[dtype], ws.data_ptr(), nb, raw_stream(dy)),
                   "embedding")
             _lib.poll_device("embedding")
         return None, dw, None

@@ -40,14 +40,13 @@ def _pack(q, k, v, log_decay, state, lengths, scale):
 def _forward(q, k, v, log_decay, state, lengths, scale, return_state):
     B, T, H, Dk = q.shape
     Dv = v.shape[3]
-    dev = q.device
-    o = torch.empty(B, T, H, Dv, dtype=q.dtype, device=dev)
-    out = torch.empty(B, H, Dk, Dv, device=dev) if return_state else None
+    o = q.new_empty((B, T, H, Dv))
+    out = q.new_empty((B, H, Dk, Dv), dtype=torch.float32) if return_state else None
     lib = _lib.load()
     args = _pack(q, k, v, log_decay, state, lengths, scale)
     with on_device(q):
         nb = lib.lifb_leaky_attn_workspace_bytes(args, 0)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
         check(lib.lifb_leaky_attn_fwd(args, addr(o), addr(out), addr(ws), nb, raw_stream(q)), "leaky_attention")
     return o, out
 
@@ -72,13 +71,13 @@ class LeakyAttention(torch.autograd.Function):
             do = torch.zeros(*q.shape[:3], v.shape[3], dtype=q.dtype, device=dev)
         do = _last_dense(do)
         dout = None if dout is None else dout.contiguous()
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
         ds = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
         lib = _lib.load()
         args = _pack(q, k, v, log_decay, state, lengths, ctx.scale)
         with on_device(q):
             nb = lib.lifb_leaky_attn_workspace_bytes(args, 1)
-            ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+            ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
             check(lib.lifb_leaky_attn_bwd(args, addr(do), (_lib.c_i64 * 3)(*do.stride()[:3]), addr(dout), addr(dq),
                                           addr(dk), addr(dv), addr(ds), addr(ws), nb, raw_stream(q)),
                   "leaky_attention")

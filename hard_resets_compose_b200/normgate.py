@@ -29,102 +29,104 @@ def _rows(t, D):
     """t as [R, D] rows with a row stride, without a copy where it has one."""
     if t.dim() != 2:
         t = t.reshape(-1, D)
-    if t.shape[0] > 1 and t.stride(0) < D or D > 1 and t.stride(1) != 1:
+    s0, s1 = t.stride()
+    if s1 != 1 and D > 1 or s0 < D and t.shape[0] > 1:
         t = t.contiguous()
     return t
 
 
 def _pack(x, h, gate, post, pre, rstd, scale, eps, act):
     R, D = x.shape
-    cols = 0 if gate is None else gate.shape[1]
     w = post if post is not None else pre
-    return _lib.NORM_GATE.pack(addr(x), addr(h), addr(gate), addr(post), addr(pre), addr(rstd), R, D, x.stride(0),
-                               0 if h is None else h.stride(0), 0 if gate is None else gate.stride(0), cols, scale,
-                               eps, act, DTYPES[x.dtype], DTYPES[w.dtype])
+    return _lib.NORM_GATE.pack(x.data_ptr(), addr(h), addr(gate), addr(post), addr(pre), addr(rstd), R, D,
+                               x.stride(0), 0 if h is None else h.stride(0), 0 if gate is None else gate.stride(0),
+                               0 if gate is None else gate.shape[1], scale, eps, act, DTYPES[x.dtype],
+                               DTYPES[w.dtype])
 
 
 def _forward(x, h, gate, post, pre, scale, eps, act, keep):
-    R, D = x.shape
-    xo = None if h is None else torch.empty(R, D, dtype=x.dtype, device=x.device)
-    n = None if pre is None else torch.empty(R, D, dtype=x.dtype, device=x.device)
-    rstd = torch.empty(2, R, device=x.device) if keep else None
+    """x' and n in x's shape, and (keep) what the backward needs: the operands as
+    rows and each row's two factors."""
+    shape, D = x.shape, x.shape[-1]
+    xo = None if h is None else x.new_empty(shape)
+    n = None if pre is None else x.new_empty(shape)
+    x = _rows(x, D)
+    h = None if h is None else _rows(h, D)
+    gate = None if gate is None else _rows(gate, gate.shape[-1])
+    rstd = x.new_empty((2, x.shape[0]), dtype=torch.float32) if keep else None
     with on_device(x):
         check(_lib.load().lifb_norm_gate_fwd(_pack(x, h, gate, post, pre, rstd, scale, eps, act), addr(xo), addr(n),
                                              raw_stream(x)), "norm_gate_residual")
-    return xo, n, rstd
+    return xo, n, (x, h, gate, rstd)
 
 
 class NormGateResidual(torch.autograd.Function):
-    """Over rows: x [R, D], h [R, D] or None, gate [R, D], [R, 1] or None."""
+    """x [..., D], h [..., D] or None, gate [..., D], [..., 1] or None."""
 
     @staticmethod
     def forward(ctx, x, h, gate, post, pre, scale, eps, act):
-        xo, n, rstd = _forward(x, h, gate, post, pre, scale, eps, act, True)
-        ctx.save_for_backward(x, h, gate, post, pre, rstd)
+        xo, n, (x2, h2, g2, rstd) = _forward(x, h, gate, post, pre, scale, eps, act, True)
+        ctx.save_for_backward(x2, h2, g2, post, pre, rstd)
         ctx.cfg = (scale, eps, act)
+        ctx.shapes = (x.shape, None if gate is None else gate.shape)
         ctx.set_materialize_grads(False)
         return xo, n
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dxo, dn):
-        x, h, gate, post, pre, rstd = ctx.saved_tensors
-        R, D = x.shape
-        dev = x.device
         if dxo is None and dn is None:
             return (None,) * 8
+        x, h, gate, post, pre, rstd = ctx.saved_tensors
+        R, D = x.shape
+        shape, gate_shape = ctx.shapes
         dxo = None if dxo is None else _rows(dxo, D)
         dn = None if dn is None else _rows(dn, D)
         need = ctx.needs_input_grad
-
-        def out(i, t):
-            return torch.empty(t.shape, dtype=t.dtype, device=dev) if t is not None and need[i] else None
-
-        dx, dh, dgate, dpost, dpre = out(0, x), out(1, h), out(2, gate), out(3, post), out(4, pre)
+        dx = x.new_empty(shape) if need[0] else None
+        dh = x.new_empty(shape) if need[1] else None
+        dgate = x.new_empty(gate_shape) if need[2] else None
+        dpost = torch.empty_like(post) if need[3] else None
+        dpre = torch.empty_like(pre) if need[4] else None
         lib = _lib.load()
         with on_device(x):
-            nb = lib.lifb_norm_gate_bwd_workspace_bytes(R, D, DTYPES[x.dtype])
-            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+            nb = lib.lifb_norm_gate_bwd_workspace_bytes(R, D, DTYPES[x.dtype]) if need[3] or need[4] else 0
+            ws = x.new_empty(nb, dtype=torch.uint8)
             check(lib.lifb_norm_gate_bwd(_pack(x, h, gate, post, pre, rstd, *ctx.cfg), addr(dxo),
                                          D if dxo is None else dxo.stride(0), addr(dn),
                                          D if dn is None else dn.stride(0), addr(dx), addr(dh), addr(dgate),
-                                         addr(dpost), addr(dpre), addr(ws), nb, raw_stream(x)), "norm_gate_residual")
+                                         addr(dpost), addr(dpre), ws.data_ptr(), nb, raw_stream(x)),
+                  "norm_gate_residual")
         return dx, dh, dgate, dpost, dpre, None, None, None
 
 
 def _run(what, x, h, gate, post, pre, scale, eps, act):
-    D = x.shape[-1] if x.dim() else 0
-    if x.dtype not in DTYPES:
-        raise TypeError(f"{what}: x must be fp32, bf16 or fp16, got {x.dtype}")
+    shape, dt = x.shape, x.dtype
+    D = shape[-1] if shape else 0
+    if dt not in DTYPES:
+        raise TypeError(f"{what}: x must be fp32, bf16 or fp16, got {dt}")
     need_cuda(what, x=x, h=h, gate=gate, post_weight=post, pre_weight=pre)
     for name, t in (("h", h), ("gate", gate)):
         if t is not None:
-            if t.dtype != x.dtype:
-                raise TypeError(f"{what}: {name} must be {x.dtype} like x, got {t.dtype}")
-            if t.shape != x.shape and not (name == "gate" and t.shape == x.shape[:-1] + (1,)):
-                raise ValueError(f"{what}: {name} {tuple(t.shape)} does not fit x {tuple(x.shape)}")
+            if t.dtype != dt:
+                raise TypeError(f"{what}: {name} must be {dt} like x, got {t.dtype}")
+            if t.shape != shape and not (name == "gate" and t.shape == shape[:-1] + (1,)):
+                raise ValueError(f"{what}: {name} {tuple(t.shape)} does not fit x {tuple(shape)}")
     wd = None
     for name, w in (("post_weight", post), ("pre_weight", pre)):
         if w is not None:
-            if w.shape != (D,):
+            if w.dim() != 1 or w.shape[0] != D:
                 raise ValueError(f"{what}: {name} must be [{D}], got {tuple(w.shape)}")
-            if w.dtype not in (torch.float32, x.dtype) or wd not in (None, w.dtype):
-                raise TypeError(f"{what}: the weights must both be fp32 or both {x.dtype}")
+            if w.dtype not in (torch.float32, dt) or wd not in (None, w.dtype):
+                raise TypeError(f"{what}: the weights must both be fp32 or both {dt}")
             wd = w.dtype
     if D > MAX_WIDTH:
         raise ValueError(f"{what}: rows of {D} elements; at most {MAX_WIDTH}")
-    shape = x.shape
-    x = _rows(x, D)
-    h = None if h is None else _rows(h, D)
-    gate = None if gate is None else _rows(gate, gate.shape[-1])
     post = None if post is None else post.contiguous()
     pre = None if pre is None else pre.contiguous()
-    args = (x, h, gate, post, pre, float(scale), float(eps), act)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, h, gate, post, pre)):
-        xo, n = NormGateResidual.apply(*args)
-    else:
-        xo, n, _ = _forward(*args, False)
-    return (None if xo is None else xo.view(shape)), (None if n is None else n.view(shape))
+        return NormGateResidual.apply(x, h, gate, post, pre, float(scale), float(eps), act)
+    return _forward(x, h, gate, post, pre, float(scale), float(eps), act, False)[:2]
 
 
 def norm_gate_residual(x, h, gate, post_weight, pre_weight=None, residual_scale=1.0, act="silu", eps=1e-6):
