@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kAtThreads) k_attn_simt(const __grid_constant_
         if (u == 0) {
             if (p.s_in) s_in = p.s_in + bh * mat;
         } else {
-            s_in = p.seg + (bh * a.nseg + u) * mat;
+            s_in = p.seg + (bh * (a.nseg + 1) + u) * mat;
             row = p.dv;
             col = 1;
         }
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kAtThreads) k_attn_simt(const __grid_constant_
     __syncthreads();
     float *s_out = nullptr;
     if (state_only) {
-        s_out = p.seg + (bh * a.nseg + u + 1) * mat;
+        s_out = p.seg + (bh * (a.nseg + 1) + u + 1) * mat;
         row = p.dv;
         col = 1;
     } else if (u == a.nseg - 1 && p.s_out) {
@@ -276,8 +276,9 @@ __global__ void __launch_bounds__(kAtThreads) k_attn_simt(const __grid_constant_
 }
 
 // Segments' own end states to starting states: seg[u] += b^n(u - 1) seg[u - 1],
-// seg[0] the pass's initial state.  One element a thread, in the order of the pass.
-__global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnArgs a)
+// seg[0] the pass's initial state; `finish`: the final state from the last one too.
+// One element a thread, in the order of the pass.
+__global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnArgs a, int finish)
 {
     const AttnPass &p = a.p[blockIdx.z];
     const int64_t mat = (int64_t)p.dq * p.dv, bh = blockIdx.y, e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -287,13 +288,14 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnA
     const DecayFactor full(ld, a.seg_tokens);
     const int64_t r = e / p.dv, c = e - r * p.dv;
     float s = p.s_in ? p.s_in[bh * mat + r * p.s_row + c * p.s_col] : 0.0f;
-    float *at = p.seg + bh * a.nseg * mat + e;
-    for (int u = 1; u < a.nseg; u++) {
+    float *at = p.seg + bh * (a.nseg + 1) * mat + e;
+    for (int u = 1; u < a.nseg + (finish && p.s_out); u++) {
         const int64_t seg = p.rev ? a.nseg - u : u - 1;  // in time, the one before
         const int64_t s0 = seg * a.seg_tokens, s1 = min(a.T, s0 + a.seg_tokens);
         const int64_t n = max((int64_t)0, min(s1, len) - s0);
         s = (n == a.seg_tokens ? full : DecayFactor(ld, n)).times(s) + at[u * mat];
-        at[u * mat] = s;
+        if (u == a.nseg) p.s_out[bh * mat + r * p.s_row + c * p.s_col] = s;
+        else at[u * mat] = s;
     }
 }
 
@@ -479,8 +481,9 @@ AttnWs carve(void *base, const lifb_leaky_attn &p, bool bwd, const Split &sp)
         return r;
     };
     const size_t mat = (size_t)p.B * p.H * p.Dk * p.Dv * 4;
-    if (sp.nseg > 1)
-        for (int i = 0; i < (bwd ? 3 : 1); i++) w.seg[i] = take(mat * sp.nseg);
+    // one segment: room for the final state of a pass that returns one
+    for (int i = 0; i < (bwd ? 3 : 1); i++)
+        if (sp.nseg > 1 || (p.dtype == LIFB_BF16 && (!bwd || i == 2))) w.seg[i] = take(mat * (sp.nseg + 1));
     if (bwd && p.Hk != p.H) {
         w.part[0] = take((size_t)p.B * p.T * p.H * p.Dk * 4);
         w.part[1] = take((size_t)p.B * p.T * p.H * p.Dv * 4);
@@ -513,19 +516,26 @@ int at_check(const char *what, const lifb_leaky_attn *p)
 bool run_passes(AttnArgs &a, int passes, int dtype, cudaStream_t s)
 {
     const bool tc = attn_tc_applies(a, passes, dtype), tc32 = attn_tc32_applies(a, passes, dtype);
-    auto run = [&](bool state_only) {
-        return tc     ? attn_tc(a, passes, state_only, s)
-               : tc32 ? attn_tc32(a, passes, state_only, s)
-                      : attn_simt(a, passes, dtype, state_only, s);
-    };
-    if (a.nseg > 1) {
-        if (!run(true)) return false;
+    // on the tensor cores a returned state comes from the state's own kernel, except where
+    // the main one has it at hand
+    bool finish = false;
+    if (tc)
+        for (int i = 0; i < passes; i++)
+            finish = finish || (a.p[i].s_out && (a.nseg > 1 || !attn_tc_returns_state(a.p[i].dq, a.p[i].dv)));
+    if (a.nseg > 1 || finish) {
+        const bool ok = tc     ? attn_state(a, passes, finish, s)
+                        : tc32 ? attn_tc32(a, passes, true, s)
+                               : attn_simt(a, passes, dtype, true, s);
+        if (!ok) return false;
         int64_t mat = 0;
         for (int i = 0; i < passes; i++) mat = std::max<int64_t>(mat, (int64_t)a.p[i].dq * a.p[i].dv);
         count_launches(1);
-        k_attn_join<<<dim3((unsigned)((mat + 255) / 256), (unsigned)(a.B * a.H), (unsigned)passes), 256, 0, s>>>(a);
+        k_attn_join<<<dim3((unsigned)((mat + 255) / 256), (unsigned)(a.B * a.H), (unsigned)passes), 256, 0, s>>>(a,
+                                                                                                           finish);
+        if (finish)
+            for (int i = 0; i < passes; i++) a.p[i].s_out = nullptr;
     }
-    return run(false);
+    return tc ? attn_tc(a, passes, s) : tc32 ? attn_tc32(a, passes, false, s) : attn_simt(a, passes, dtype, false, s);
 }
 
 void strides_of(int64_t (&st)[3], const int64_t *from) { st[0] = from[0], st[1] = from[1], st[2] = from[2]; }

@@ -19,6 +19,7 @@
 // one power of b less on the carried term and one more on the new one (`shift`).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -38,7 +39,8 @@ struct AttnPass {
     int64_t s_row, s_col;         // their strides: row (q's width), column (v's)
     float p_scale, i_scale, w_scale;  // of the chunk's products, the carried term, and the state's update
     int shift, rev, o_f32;
-    float *seg;                   // [B*H][nseg][dq][dv]: each time segment's starting state (0's unused)
+    float *seg;                   // [B*H][nseg + 1][dq][dv]: each time segment's starting state (0's unused);
+                                  // the last is what the final state is joined from
 };
 
 constexpr int kAttnMaxPasses = 3;
@@ -88,7 +90,15 @@ bool attn_simt(const AttnArgs &a, int passes, int dtype, bool state_only, cudaSt
 // leaky_attn_tc.cu: chunks of 128 tokens on the tensor cores, bf16 operands that TMA
 // can load (16-byte aligned strides, widths multiples of 8).
 bool attn_tc_applies(const AttnArgs &a, int passes, int dtype);
-bool attn_tc(const AttnArgs &a, int passes, bool state_only, cudaStream_t s);
+bool attn_tc(const AttnArgs &a, int passes, cudaStream_t s);
+// leaky_attn_state.cu: the segments' own end states for them (the last segment's where the
+// pass returns its state).
+bool attn_state(const AttnArgs &a, int passes, bool finish, cudaStream_t s);
+// A tensor map of an operand in tiles of 64 columns by 128 tokens.
+bool attn_operand_map(CUtensorMap *m, const void *base, const int64_t (&st)[3], int d, int64_t T, int64_t heads,
+                      int64_t B);
+// Whether attn_tc returns this pass's state itself.
+bool attn_tc_returns_state(int dq, int dv);
 // leaky_attn_tc32.cu: the same for fp32 operands in 16-byte aligned vectors, widths up to 64.
 bool attn_tc32_applies(const AttnArgs &a, int passes, int dtype);
 bool attn_tc32(const AttnArgs &a, int passes, bool state_only, cudaStream_t s);

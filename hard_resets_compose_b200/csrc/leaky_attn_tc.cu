@@ -38,20 +38,15 @@
 // Registers are moved from the other warpgroups to the state's (setmaxnreg).
 // Every wait is bounded (status 101).
 #include <algorithm>
-#include <type_traits>
 
-#include "leaky_attn.h"
+#include "leaky_attn_tc.cuh"
 #include "lifb_common.cuh"
 #include "lifb_internal.h"
 #include "seq_types.cuh"
-#include "tc.cuh"
 
 namespace lifb {
 
 namespace {
-
-constexpr int kTcC = 128;           // tokens of a chunk
-constexpr int kTcBlock = kTcC * 128;  // bytes of 128 rows of 64 bf16
 
 // Tensor maps of the passes of one launch.
 struct AttnMaps {
@@ -66,11 +61,9 @@ struct TcLayout {
     static constexpr uint32_t kQ = DQ / 64 * kTcBlock, kV = DV / 64 * kTcBlock, kS = DV / 64 * DQ * 128;
     static constexpr bool small = DQ == 64 && DV == 64;
     static constexpr int np = small ? 2 : 1;  // P's in flight, in tensor memory
-    // tiles in flight: of q one more than P's, so that the next Q K^T need not wait for
-    // Q S (where three pieces of 128 columns leave no room for it, it does)
-    static constexpr int nq = DQ == 128 && DV == 128 && NP == 3 ? 1 : np + 1, nk = np;
-    static constexpr int nv = DQ == 128 && (DV == 128 || NP == 3) ? 1 : 2, nm = small ? 2 : 1;  // nm: sets of pieces
-    static constexpr bool early = nq > np;
+    // tiles in flight: of q one more than P's, so that the next Q K^T need not wait for Q S
+    static constexpr int nq = np + 1, nk = np;
+    static constexpr int nv = DQ == 128 && DV == 128 ? 1 : 2, nm = small ? 2 : 1;  // nm: sets of pieces
     static constexpr uint32_t pieces = 0, k = nm * NP * kQ, q = k + nk * kQ, v = q + nq * kQ, s = v + nv * kV,
                               bytes = s + kS;
     static_assert(bytes + 1024 + 512 <= 227 * 1024, "tiles fit an SM");
@@ -93,17 +86,6 @@ struct TcBars {
     uint64_t q_full[3], q_free[3], k_full[2], k_free[2], v_full[2], v_free[2];
     uint64_t p_full[2], p_ready[2], kw_ready[2], s_ready, s_free, o_full, o_free, ds_full, ds_free, done;
 };
-
-template <int N>
-__device__ __forceinline__ void regs_inc()
-{
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_dec()
-{
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
 
 }  // namespace
 
@@ -175,49 +157,7 @@ __device__ __forceinline__ void store_32_bytes(void *p, const uint32_t (&m)[8])
                  : "memory");
 }
 
-// A token's weight, as the pieces of its weighted key need it: two bf16 values
-// (each twice in a word) whose sum is w to 2^-18, or w itself.
-template <int NP>
-struct TokenWeight {
-    uint32_t wh, wm;
-    __device__ __forceinline__ void set(float w)
-    {
-        wh = NP == 2 ? pack_bf16(w, w) : __float_as_uint(w);
-        wm = NP == 2 ? pack_bf16(w - bf16_lo(wh), w - bf16_lo(wh)) : 0;
-    }
-    // w * x for eight bf16 elements x (four words) as NP bf16 pieces.  Two pieces: hi =
-    // x wh rounded; what that dropped is exact in bf16 (the product has 16 bits), so
-    // mid = x wm + it.
-    __device__ __forceinline__ void split(const uint4 &x4, uint4 &hi4, uint4 &mid4, uint4 &lo4) const
-    {
-        const uint32_t in[4] = {x4.x, x4.y, x4.z, x4.w};
-        uint32_t hi[4], mid[4], lo[4] = {};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if constexpr (NP == 2) {
-                const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&in[e]);
-                const __nv_bfloat162 h2 = *reinterpret_cast<const __nv_bfloat162 *>(&wh);
-                const __nv_bfloat162 m2 = *reinterpret_cast<const __nv_bfloat162 *>(&wm);
-                const __nv_bfloat162 h = __hmul2_rn(x, h2);
-                const __nv_bfloat162 m = __hfma2(x, m2, __hfma2(x, h2, __hneg2(h)));
-                hi[e] = *reinterpret_cast<const uint32_t *>(&h);
-                mid[e] = *reinterpret_cast<const uint32_t *>(&m);
-            } else {
-                const float w = __uint_as_float(wh);
-                const float f0 = bf16_lo(in[e]) * w, f1 = bf16_hi(in[e]) * w;
-                hi[e] = pack_bf16(f0, f1);
-                const float g0 = f0 - bf16_lo(hi[e]), g1 = f1 - bf16_hi(hi[e]);
-                mid[e] = pack_bf16(g0, g1);
-                lo[e] = pack_bf16(g0 - bf16_lo(mid[e]), g1 - bf16_hi(mid[e]));
-            }
-        }
-        hi4 = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        mid4 = make_uint4(mid[0], mid[1], mid[2], mid[3]);
-        lo4 = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-};
-
-template <int DQ, int DV, int NP, bool STATE_ONLY>
+template <int DQ, int DV, int NP>
 __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     k_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps maps, int *status)
 {
@@ -231,7 +171,6 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     const AttnPass &p = a.p[pi];
     const int64_t bh = blockIdx.x / a.nseg;
     const int u = (int)(blockIdx.x - bh * a.nseg);  // in the order of the pass
-    if (STATE_ONLY && u == a.nseg - 1) return;      // nothing starts from the last one
     const int64_t b = bh / a.H, h = bh - b * a.H;
     const int64_t len = attn_length(a.lengths, b, a.T);
     const float ld = a.log_decay[h];
@@ -250,7 +189,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.k_full[i], 1);
-            mbar_init(&bars.k_free[i], (STATE_ONLY ? 0 : 1) + 128 * L::state_groups);
+            mbar_init(&bars.k_free[i], 1 + 128 * L::state_groups);
             mbar_init(&bars.v_full[i], 1);
             mbar_init(&bars.v_free[i], 1);
             mbar_init(&bars.p_full[i], 1);
@@ -288,7 +227,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             // ---- loads
             prefetch_tmap(&maps.k[pi]);
             prefetch_tmap(&maps.v[pi]);
-            if (!STATE_ONLY) prefetch_tmap(&maps.q[pi]);
+            prefetch_tmap(&maps.q[pi]);
             const int hq = (int)(h / p.qg), hk = (int)(h / p.kg), hv = (int)(h / p.vg), ib = (int)b;
             // tile c of an operand with N buffers of `bytes` from `at`; false: gave up
             auto load = [&](const CUtensorMap *m, uint32_t at, uint32_t bytes, int N, int c, int head, uint64_t *full,
@@ -304,10 +243,8 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             for (int c = 0; c < chunks; c++) {
                 if (!load(&maps.k[pi], L::k, L::kQ, L::nk, c, hk, bars.k_full, bars.k_free)) break;
                 nk++;
-                if (!STATE_ONLY) {
-                    if (!load(&maps.q[pi], L::q, L::kQ, L::nq, c, hq, bars.q_full, bars.q_free)) break;
-                    nq++;
-                }
+                if (!load(&maps.q[pi], L::q, L::kQ, L::nq, c, hq, bars.q_full, bars.q_free)) break;
+                nq++;
                 if (!load(&maps.v[pi], L::v, L::kV, L::nv, c, hv, bars.v_full, bars.v_free)) break;
                 nv++;
             }
@@ -351,7 +288,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                                      k > 0);
                     umma_arrive(&bars.q_free[c % L::nq]);
                     umma_arrive(&bars.s_free);
-                    if (L::early) umma_arrive(&bars.o_full);
+                    umma_arrive(&bars.o_full);
                 }
                 return true;
             };
@@ -370,12 +307,9 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                             umma_bf16_ss(tmem + L::ds, dk + k * 128, dv + k * 128, kIdS, piece > 0 || k > 0);
                     }
                     umma_arrive(&bars.ds_full);
-                    if (STATE_ONLY) umma_arrive(&bars.v_free[c % L::nv]);
                 }
-                if (STATE_ONLY) return true;
                 if (!wait_warp(&bars.p_ready[c % L::np], c / L::np)) return false;
                 if (c > 0 && !wait_warp(&bars.o_free, c - 1)) return false;
-                if (!L::early && !carried(c)) return false;
                 tcgen05_after();
                 const uint32_t pb = p_cols(c) + (p.rev ? 0u : 64u);  // P in bf16
                 if (elect_lane()) {
@@ -383,18 +317,16 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                     for (int k = 0; k < kTcC / 16; k++)
                         umma_bf16_ts(tmem + L::o1, pb + k * 8, dv + k * 128, kIdO, k > 0);
                     umma_arrive(&bars.v_free[c % L::nv]);
-                    if (!L::early) umma_arrive(&bars.o_full);
                 }
                 if (c + L::np < chunks) {
                     // P V is done: P's columns are free
                     if (!wait_warp(&bars.v_free[c % L::nv], c / L::nv)) return false;
                     if (!scores(c + L::np)) return false;
                 }
-                return !L::early || carried(c);
+                return carried(c);
             };
             bool ok = true;
-            if (!STATE_ONLY)
-                for (int c = 0; ok && c < L::np && c < chunks; c++) ok = scores(c);
+            for (int c = 0; ok && c < L::np && c < chunks; c++) ok = scores(c);
             for (int c = 0; ok && c < chunks; c++) ok = body(c);
             if (elect_lane()) {  // nothing of the tensor cores is left running
                 umma_arrive(&bars.done);
@@ -404,106 +336,102 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     } else if (group < L::score_groups) {
         // ---- P: one token a thread
         regs_dec<L::score_regs>();
-        if (!STATE_ONLY) {
-            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            const float b1 = decay_pow(ld, 1.0f);
-            uint64_t pw[8];
-            float b16 = 1.0f;
-            {
-                float f[16];
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const float b1 = decay_pow(ld, 1.0f);
+        uint64_t pw[8];
+        float b16 = 1.0f;
+        {
+            float f[16];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    f[i] = b16;
-                    b16 *= b1;
-                }
+            for (int i = 0; i < 16; i++) {
+                f[i] = b16;
+                b16 *= b1;
+            }
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    pw[i] = p.rev ? two(f[2 * i], f[2 * i + 1]) : two(f[15 - 2 * i], f[14 - 2 * i]);
-            }
-            for (int c = group; c < chunks; c += L::np) {
-                const int n = min(kTcC, end - (t_first + c * t_step));
-                if (!wait_warp(&bars.p_full[group], c / L::np)) break;
-                tcgen05_after();
-                const uint32_t cols = tmem + lanes + group * 128;
-                if (p.rev) attn_scores<true>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
-                else attn_scores<false>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
-                tcgen05_before();
-                mbar_arrive(&bars.p_ready[group]);
-            }
+            for (int i = 0; i < 8; i++)
+                pw[i] = p.rev ? two(f[2 * i], f[2 * i + 1]) : two(f[15 - 2 * i], f[14 - 2 * i]);
+        }
+        for (int c = group; c < chunks; c += L::np) {
+            const int n = min(kTcC, end - (t_first + c * t_step));
+            if (!wait_warp(&bars.p_full[group], c / L::np)) break;
+            tcgen05_after();
+            const uint32_t cols = tmem + lanes + group * 128;
+            if (p.rev) attn_scores<true>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
+            else attn_scores<false>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
+            tcgen05_before();
+            mbar_arrive(&bars.p_ready[group]);
         }
     } else if (group == L::output_group) {
         // ---- O: one token a thread
         regs_dec<L::output_regs>();
-        if (!STATE_ONLY) {
-            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            const int row = tid & 127;
-            const int64_t o_at = b * p.os[0] + h * p.os[2];
-            const bool sectors = p.dv % 16 == 0 && (uintptr_t)p.o % 32 == 0;  // rows of whole 32-byte sectors
-            for (int c = 0; c < chunks; c++) {
-                const int t0 = t_first + c * t_step, n = min(kTcC, end - t0);
-                const int r = p.rev ? n - 1 - row : row;
-                const float w = row < n ? p.i_scale * decay_pow(ld, (float)(r + 1 - p.shift)) : 0.0f;
-                if (!wait_warp(&bars.o_full, c)) break;
-                tcgen05_after();
-                const uint64_t ww = two(w, w);
-                char *o_row = (char *)p.o + (o_at + (int64_t)(t0 + row) * p.os[1]) * (p.o_f32 ? 4 : 2);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int row = tid & 127;
+        const int64_t o_at = b * p.os[0] + h * p.os[2];
+        const bool sectors = p.dv % 16 == 0 && (uintptr_t)p.o % 32 == 0;  // rows of whole 32-byte sectors
+        for (int c = 0; c < chunks; c++) {
+            const int t0 = t_first + c * t_step, n = min(kTcC, end - t0);
+            const int r = p.rev ? n - 1 - row : row;
+            const float w = row < n ? p.i_scale * decay_pow(ld, (float)(r + 1 - p.shift)) : 0.0f;
+            if (!wait_warp(&bars.o_full, c)) break;
+            tcgen05_after();
+            const uint64_t ww = two(w, w);
+            char *o_row = (char *)p.o + (o_at + (int64_t)(t0 + row) * p.os[1]) * (p.o_f32 ? 4 : 2);
 #pragma unroll 1
-                for (int g = 0; g < DV; g += 32) {
-                    uint32_t x[32], y[32];
-                    tmem_load32(tmem + lanes + L::o1 + g, x);
-                    tmem_load32(tmem + lanes + L::o2 + g, y);
-                    tmem_wait_ld();
-                    if (g == DV - 32) {
-                        tcgen05_before();
-                        mbar_arrive(&bars.o_free);
-                    }
-                    uint64_t o[16];
+            for (int g = 0; g < DV; g += 32) {
+                uint32_t x[32], y[32];
+                tmem_load32(tmem + lanes + L::o1 + g, x);
+                tmem_load32(tmem + lanes + L::o2 + g, y);
+                tmem_wait_ld();
+                if (g == DV - 32) {
+                    tcgen05_before();
+                    mbar_arrive(&bars.o_free);
+                }
+                uint64_t o[16];
 #pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        o[e] = fma2(ww, two(y[2 * e], y[2 * e + 1]), two(x[2 * e], x[2 * e + 1]));
-                    if (row >= n) {
+                for (int e = 0; e < 16; e++)
+                    o[e] = fma2(ww, two(y[2 * e], y[2 * e + 1]), two(x[2 * e], x[2 * e + 1]));
+                if (row >= n) {
 #pragma unroll
-                        for (int e = 0; e < 16; e++) o[e] = 0;
-                    }
-                    if (t0 + row < s1) {
-                        if (!p.o_f32) {
-                            __nv_bfloat16 *dst = (__nv_bfloat16 *)o_row + g;
+                    for (int e = 0; e < 16; e++) o[e] = 0;
+                }
+                if (t0 + row < s1) {
+                    if (!p.o_f32) {
+                        __nv_bfloat16 *dst = (__nv_bfloat16 *)o_row + g;
 #pragma unroll
-                            for (int e = 0; e < 16; e += 8) {
-                                const uint32_t m[8] = {pack2_bf16(o[e]),     pack2_bf16(o[e + 1]), pack2_bf16(o[e + 2]),
-                                                       pack2_bf16(o[e + 3]), pack2_bf16(o[e + 4]), pack2_bf16(o[e + 5]),
-                                                       pack2_bf16(o[e + 6]), pack2_bf16(o[e + 7])};
-                                if (sectors && g + 2 * e < p.dv) {
-                                    store_32_bytes(dst + 2 * e, m);
-                                } else {
-                                    if (g + 2 * e < p.dv)
-                                        *reinterpret_cast<uint4 *>(dst + 2 * e) = make_uint4(m[0], m[1], m[2], m[3]);
-                                    if (g + 2 * e + 8 < p.dv)
-                                        *reinterpret_cast<uint4 *>(dst + 2 * e + 8) = make_uint4(m[4], m[5], m[6], m[7]);
-                                }
-                            }
-                        } else {
-                            float *dst = (float *)o_row + g;
-#pragma unroll
-                            for (int e = 0; e < 16; e += 2)
+                        for (int e = 0; e < 16; e += 8) {
+                            const uint32_t m[8] = {pack2_bf16(o[e]),     pack2_bf16(o[e + 1]), pack2_bf16(o[e + 2]),
+                                                   pack2_bf16(o[e + 3]), pack2_bf16(o[e + 4]), pack2_bf16(o[e + 5]),
+                                                   pack2_bf16(o[e + 6]), pack2_bf16(o[e + 7])};
+                            if (sectors && g + 2 * e < p.dv) {
+                                store_32_bytes(dst + 2 * e, m);
+                            } else {
                                 if (g + 2 * e < p.dv)
-                                    *reinterpret_cast<ulonglong2 *>(dst + 2 * e) = make_ulonglong2(o[e], o[e + 1]);
+                                    *reinterpret_cast<uint4 *>(dst + 2 * e) = make_uint4(m[0], m[1], m[2], m[3]);
+                                if (g + 2 * e + 8 < p.dv)
+                                    *reinterpret_cast<uint4 *>(dst + 2 * e + 8) = make_uint4(m[4], m[5], m[6], m[7]);
+                            }
                         }
+                    } else {
+                        float *dst = (float *)o_row + g;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2)
+                            if (g + 2 * e < p.dv)
+                                *reinterpret_cast<ulonglong2 *>(dst + 2 * e) = make_ulonglong2(o[e], o[e + 1]);
                     }
-                    __syncwarp();
                 }
+                __syncwarp();
             }
-            // tokens past the sequence's end in chunks that have none of it
-            const int z0 = s0 + chunks * kTcC;
-            const int64_t nz = (int64_t)max(0, s1 - z0) * (p.dv / 8);
-            for (int64_t i = row; i < nz; i += 128) {
-                const int64_t r = i / (p.dv / 8), at = o_at + (z0 + r) * p.os[1] + (i - r * (p.dv / 8)) * 8;
-                if (p.o_f32) {
-                    *reinterpret_cast<float4 *>((float *)p.o + at) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    *reinterpret_cast<float4 *>((float *)p.o + at + 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                } else {
-                    *reinterpret_cast<uint4 *>((__nv_bfloat16 *)p.o + at) = make_uint4(0, 0, 0, 0);
-                }
+        }
+        // tokens past the sequence's end in chunks that have none of it
+        const int z0 = s0 + chunks * kTcC;
+        const int64_t nz = (int64_t)max(0, s1 - z0) * (p.dv / 8);
+        for (int64_t i = row; i < nz; i += 128) {
+            const int64_t r = i / (p.dv / 8), at = o_at + (z0 + r) * p.os[1] + (i - r * (p.dv / 8)) * 8;
+            if (p.o_f32) {
+                *reinterpret_cast<float4 *>((float *)p.o + at) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                *reinterpret_cast<float4 *>((float *)p.o + at + 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            } else {
+                *reinterpret_cast<uint4 *>((__nv_bfloat16 *)p.o + at) = make_uint4(0, 0, 0, 0);
             }
         }
     } else if (group < L::last_group) {
@@ -518,14 +446,12 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
         {
             const float *s_in = nullptr;
             int64_t row = p.s_row, col = p.s_col;
-            if (!STATE_ONLY) {
-                if (u == 0) {
-                    if (p.s_in) s_in = p.s_in + bh * mat;
-                } else {
-                    s_in = p.seg + (bh * a.nseg + u) * mat;
-                    row = p.dv;
-                    col = 1;
-                }
+            if (u == 0) {
+                if (p.s_in) s_in = p.s_in + bh * mat;
+            } else {
+                s_in = p.seg + (bh * (a.nseg + 1) + u) * mat;
+                row = p.dv;
+                col = 1;
             }
 #pragma unroll
             for (int j = 0; j < SC; j += 2) {
@@ -548,7 +474,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             fence_proxy_async_shared();
             mbar_arrive(&bars.s_ready);
         };
-        if (!STATE_ONLY && chunks > 0) put_state();
+        if (chunks > 0) put_state();
         const DecayFactor full(ld, kTcC);
         // the weights of the tokens whose columns this thread scales
         constexpr int NW = 8 / NB;
@@ -629,16 +555,12 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             mbar_arrive(&bars.ds_free);
             if (c + 1 == chunks) break;
             if (L::nm == 1 && !weigh(c + 1)) break;
-            if (!STATE_ONLY) {
-                if (!wait_warp(&bars.s_free, c)) break;
-                put_state();
-            }
+            if (!wait_warp(&bars.s_free, c)) break;
+            put_state();
         }
         float *s_out = nullptr;
         int64_t row = p.dv, col = 1;
-        if (STATE_ONLY) {
-            s_out = p.seg + (bh * a.nseg + u + 1) * mat;
-        } else if (u == a.nseg - 1 && p.s_out) {
+        if (u == a.nseg - 1 && p.s_out) {
             s_out = p.s_out + bh * mat;
             row = p.s_row;
             col = p.s_col;
@@ -664,22 +586,23 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     }
 }
 
-namespace {
-
-int width_class(int d) { return d <= 64 ? 64 : 128; }
-
-bool operand_map(CUtensorMap *m, const void *base, const int64_t (&st)[3], int d, int64_t T, int64_t heads, int64_t B)
+bool attn_operand_map(CUtensorMap *m, const void *base, const int64_t (&st)[3], int d, int64_t T, int64_t heads,
+                      int64_t B)
 {
     const int64_t dims[4] = {d, T, heads, B}, strides[3] = {st[1], st[2], st[0]};
     return make_tmap_4d_bf16(m, base, dims, strides, 64, kTcC);
 }
 
+namespace {
+
+int width_class(int d) { return d <= 64 ? 64 : 128; }
+
 template <int DQ, int DV, int NP>
-bool launch_tc(const AttnArgs &a, const AttnMaps &m, int passes, bool state_only, cudaStream_t s)
+bool launch_tc(const AttnArgs &a, const AttnMaps &m, int passes, cudaStream_t s)
 {
     using L = TcLayout<DQ, DV, NP>;
     const size_t smem = L::bytes + 1024;
-    auto kern = state_only ? k_attn_tc<DQ, DV, NP, true> : k_attn_tc<DQ, DV, NP, false>;
+    auto kern = k_attn_tc<DQ, DV, NP>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
     count_launches(1);
     kern<<<dim3((unsigned)(a.B * a.H * a.nseg), (unsigned)passes), L::threads, smem, s>>>(a, m, device_status_ptr());
@@ -695,15 +618,17 @@ bool attn_tc_applies(const AttnArgs &a, int passes, int dtype)
         const AttnPass &p = a.p[i];
         if (p.dq % 8 || p.dv % 8 || p.dq > kAttnMaxDim || p.dv > kAttnMaxDim || !aligned16(p.o)) return false;
         CUtensorMap m;
-        if (!operand_map(&m, p.q, p.qs, p.dq, a.T, a.H / p.qg, a.B) ||
-            !operand_map(&m, p.k, p.ks, p.dq, a.T, a.H / p.kg, a.B) ||
-            !operand_map(&m, p.v, p.vs, p.dv, a.T, a.H / p.vg, a.B))
+        if (!attn_operand_map(&m, p.q, p.qs, p.dq, a.T, a.H / p.qg, a.B) ||
+            !attn_operand_map(&m, p.k, p.ks, p.dq, a.T, a.H / p.kg, a.B) ||
+            !attn_operand_map(&m, p.v, p.vs, p.dv, a.T, a.H / p.vg, a.B))
             return false;
     }
     return true;
 }
 
-bool attn_tc(const AttnArgs &a, int passes, bool state_only, cudaStream_t s)
+bool attn_tc_returns_state(int dq, int dv) { return width_class(dq) == 64 && width_class(dv) == 64; }
+
+bool attn_tc(const AttnArgs &a, int passes, cudaStream_t s)
 {
     // passes of one pair of width classes, and with a returned state or without, share a launch
     bool launched[kAttnMaxPasses] = {};
@@ -719,21 +644,17 @@ bool attn_tc(const AttnArgs &a, int passes, bool state_only, cudaStream_t s)
             if (launched[j] || width_class(p.dq) != dq || width_class(p.dv) != dv ||
                 (p.s_out != nullptr) != exact_state)
                 continue;
-            if (!operand_map(&m.q[n], p.q, p.qs, p.dq, a.T, a.H / p.qg, a.B) ||
-                !operand_map(&m.k[n], p.k, p.ks, p.dq, a.T, a.H / p.kg, a.B) ||
-                !operand_map(&m.v[n], p.v, p.vs, p.dv, a.T, a.H / p.vg, a.B))
+            if (!attn_operand_map(&m.q[n], p.q, p.qs, p.dq, a.T, a.H / p.qg, a.B) ||
+                !attn_operand_map(&m.k[n], p.k, p.ks, p.dq, a.T, a.H / p.kg, a.B) ||
+                !attn_operand_map(&m.v[n], p.v, p.vs, p.dv, a.T, a.H / p.vg, a.B))
                 return false;
             launched[j] = true;
             b.p[n++] = p;
         }
-        auto run = [&](auto np) {
-            constexpr int NP = decltype(np)::value;
-            return dq == 64 ? (dv == 64 ? launch_tc<64, 64, NP>(b, m, n, state_only, s)
-                                        : launch_tc<64, 128, NP>(b, m, n, state_only, s))
-                            : (dv == 64 ? launch_tc<128, 64, NP>(b, m, n, state_only, s)
-                                        : launch_tc<128, 128, NP>(b, m, n, state_only, s));
-        };
-        const bool ok = exact_state ? run(std::integral_constant<int, 3>()) : run(std::integral_constant<int, 2>());
+        const bool ok = dq == 64 ? (dv != 64      ? launch_tc<64, 128, 2>(b, m, n, s)
+                                    : exact_state ? launch_tc<64, 64, 3>(b, m, n, s)
+                                                  : launch_tc<64, 64, 2>(b, m, n, s))
+                                 : (dv == 64 ? launch_tc<128, 64, 2>(b, m, n, s) : launch_tc<128, 128, 2>(b, m, n, s));
         if (!ok) return false;
     }
     return true;

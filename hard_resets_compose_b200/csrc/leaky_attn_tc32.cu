@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
                 if (u == 0) {
                     if (p.s_in) s_in = p.s_in + bh * mat;
                 } else {
-                    s_in = p.seg + (bh * a.nseg + u) * mat;
+                    s_in = p.seg + (bh * (a.nseg + 1) + u) * mat;
                     row = p.dv;
                     col = 1;
                 }
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
         float *s_out = nullptr;
         int64_t row = p.dv, col = 1;
         if (STATE_ONLY) {
-            s_out = p.seg + (bh * a.nseg + u + 1) * mat;
+            s_out = p.seg + (bh * (a.nseg + 1) + u + 1) * mat;
         } else if (u == a.nseg - 1 && p.s_out) {
             s_out = p.s_out + bh * mat;
             row = p.s_row;
