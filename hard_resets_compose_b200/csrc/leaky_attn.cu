@@ -289,13 +289,22 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnA
     const int64_t r = e / p.dv, c = e - r * p.dv;
     float s = p.s_in ? p.s_in[bh * mat + r * p.s_row + c * p.s_col] : 0.0f;
     float *at = p.seg + bh * (a.nseg + 1) * mat + e;
-    for (int u = 1; u < a.nseg + (finish && p.s_out); u++) {
-        const int64_t seg = p.rev ? a.nseg - u : u - 1;  // in time, the one before
-        const int64_t s0 = seg * a.seg_tokens, s1 = min(a.T, s0 + a.seg_tokens);
-        const int64_t n = max((int64_t)0, min(s1, len) - s0);
-        s = (n == a.seg_tokens ? full : DecayFactor(ld, n)).times(s) + at[u * mat];
-        if (u == a.nseg) p.s_out[bh * mat + r * p.s_row + c * p.s_col] = s;
-        else at[u * mat] = s;
+    const int last = a.nseg + (finish && p.s_out);
+    for (int u0 = 1; u0 < last; u0 += 8) {  // eight loads in flight
+        float own[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) own[j] = u0 + j < last ? at[(u0 + j) * mat] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int u = u0 + j;
+            if (u >= last) break;
+            const int64_t seg = p.rev ? a.nseg - u : u - 1;  // in time, the one before
+            const int64_t s0 = seg * a.seg_tokens, s1 = min(a.T, s0 + a.seg_tokens);
+            const int64_t n = max((int64_t)0, min(s1, len) - s0);
+            s = (n == a.seg_tokens ? full : DecayFactor(ld, n)).times(s) + own[j];
+            if (u == a.nseg) p.s_out[bh * mat + r * p.s_row + c * p.s_col] = s;
+            else at[u * mat] = s;
+        }
     }
 }
 
