@@ -454,12 +454,13 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 col = 1;
             }
 #pragma unroll
-            for (int j = 0; j < SC; j += 2) {
-                float f[2] = {0.0f, 0.0f};
+            for (int j = 0; j < SC / 2; j++) S[j] = 0;
+            // (a branch, not a condition of each load: what is not there is not fetched either)
+            if (s_in && st < p.dq) {
+                s_in += st * row + c0 * col;
 #pragma unroll
-                for (int e = 0; e < 2; e++)
-                    if (s_in && st < p.dq && c0 + j + e < p.dv) f[e] = s_in[st * row + (c0 + j + e) * col];
-                S[j / 2] = two(f[0], f[1]);
+                for (int j = 0; j < SC; j += 2)
+                    if (c0 + j < p.dv) S[j / 2] = two(s_in[j * col], s_in[(j + 1) * col]);
             }
         }
         auto put_state = [&] {  // its bf16 copy, the B operand of Q S

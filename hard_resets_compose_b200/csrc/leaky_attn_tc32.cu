@@ -339,12 +339,13 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
                 }
             }
 #pragma unroll
-            for (int j = 0; j < kT32W; j += 2) {
-                float f[2] = {0.0f, 0.0f};
+            for (int j = 0; j < kT32W / 2; j++) S[j] = 0;
+            // (a branch, not a condition of each load: what is not there is not fetched either)
+            if (s_in && st < p.dq) {
+                s_in += st * row;
 #pragma unroll
-                for (int e = 0; e < 2; e++)
-                    if (s_in && st < p.dq && j + e < p.dv) f[e] = s_in[st * row + (j + e) * col];
-                S[j / 2] = two(f[0], f[1]);
+                for (int j = 0; j < kT32W; j += 2)
+                    if (j < p.dv) S[j / 2] = two(s_in[j * col], s_in[(j + 1) * col]);
             }
         }
         const DecayFactor full(ld, kT32C);
