@@ -323,20 +323,45 @@ __global__ void __launch_bounds__(256) k_attn_group(const float *__restrict__ pa
     }
 }
 
+// A state's elements, read once and written once: not kept in the caches.
+template <int VEC>
+__device__ __forceinline__ void load_once(const float *p, float (&x)[VEC])
+{
+    if constexpr (VEC == 4) {
+        const float4 f = __ldcs(reinterpret_cast<const float4 *>(p));
+        x[0] = f.x;
+        x[1] = f.y;
+        x[2] = f.z;
+        x[3] = f.w;
+    } else {
+        x[0] = __ldcs(p);
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void store_once(float *p, const float (&x)[VEC])
+{
+    if constexpr (VEC == 4) __stcs(reinterpret_cast<float4 *>(p), make_float4(x[0], x[1], x[2], x[3]));
+    else __stcs(p, x[0]);
+}
+
 // One token: S = b S + k v^T in place, o = scale * S^T q.  A block has one
 // (sequence, head) and CV * VEC columns of the state; its threads are CV columns
 // (VEC elements each) by row groups that walk the rows, and the groups' sums of
 // q_r S_r are added at the end.  Bound by memory: the state is read and written
-// once, 8 dk dv bytes.
+// once, 8 dk dv bytes.  What it takes is enough bytes in flight: eight rows a thread
+// are on their way before q and k are (190 sequences of 16 heads of 128 x 128: 80 us
+// with the rows after them, 68 us so, 62 us at the copy rate), and blocks of 128
+// threads, 16 vectors wide, so that heads of 64 x 64 do too (512 x 16 of them: 60 us
+// with 256 threads, 48 us so, floor 42 us).
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kAtThreads)
     k_attn_step(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, T *__restrict__ o,
                 const float *__restrict__ log_decay, float *__restrict__ state, const int32_t *__restrict__ slots,
                 int64_t n_slots, int H, int group, int dk, int dv, int cv, int64_t q_b, int64_t q_h, int64_t k_b,
                 int64_t k_h, int64_t v_b, int64_t v_h, int64_t s_slot, int64_t s_h, float scale)
 {
     __shared__ float sq[kAttnMaxDim], sk[kAttnMaxDim];
-    __shared__ float part[256 * VEC];
+    __shared__ float part[kAtThreads * VEC];
     const int64_t b = blockIdx.x / H, h = blockIdx.x - b * H;
     const int tid = threadIdx.x, groups = blockDim.x / cv, rg = tid / cv;
     const int c = (blockIdx.y * cv + tid % cv) * VEC;
@@ -359,20 +384,32 @@ __global__ void __launch_bounds__(256)
     for (int e = 0; e < VEC; e++) x[e] = acc[e] = 0.0f;
     float *st = state + slot * s_slot + h * s_h + c;
     const bool in = c < dv && rg < groups;
+    // rows rg, rg + groups, ..., U of them in flight; the first ones before q and k are there
+    constexpr int U = 8;
+    float y[U][VEC];
+    auto load = [&](int r0) {
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const int r = r0 + j * groups;
+            if (in && r < dk) load_once(st + (int64_t)r * dv, y[j]);
+        }
+    };
+    load(rg);
     if (in) load_f32(v + b * v_b + (h / group) * v_h + c, x);
     __syncthreads();
-    if (in) {
-#pragma unroll 8
-        for (int r = rg; r < dk; r += groups) {
-            float y[VEC];
-            load_f32(st + (int64_t)r * dv, y);
+    for (int r0 = rg; r0 < dk; r0 += U * groups) {
+        if (r0 != rg) load(r0);
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const int r = r0 + j * groups;
+            if (!in || r >= dk) break;
             const float kr = sk[r], qr = sq[r];
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                y[e] = beta * y[e] + kr * x[e];
-                acc[e] += qr * y[e];
+                y[j][e] = beta * y[j][e] + kr * x[e];
+                acc[e] += qr * y[j][e];
             }
-            store_f32(st + (int64_t)r * dv, y);
+            store_once(st + (int64_t)r * dv, y[j]);
         }
     }
 #pragma unroll
@@ -716,7 +753,7 @@ void step_launch(const lifb_leaky_attn_step_args &p, void *o, float *state, cuda
                       p.v_strides[0] % 4 == 0 && p.v_strides[1] % 4 == 0 && (uintptr_t)p.v % (4 * sizeof(T)) == 0 &&
                       (uintptr_t)o % (4 * sizeof(T)) == 0;
     const int vec = wide ? 4 : 1, cols = (int)(p.Dv + vec - 1) / vec;
-    const int cv = std::min(cols, 32), threads = 256 / cv * cv;
+    const int cv = std::min(cols, 16), threads = kAtThreads / cv * cv;
     const dim3 grid((unsigned)(p.B * p.H), (unsigned)((cols + cv - 1) / cv));
     auto kern = wide ? k_attn_step<T, 4> : k_attn_step<T, 1>;
     count_launches(1);
