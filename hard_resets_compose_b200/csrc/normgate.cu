@@ -60,7 +60,7 @@ struct NormArgs {
 __host__ __device__ constexpr int norm_blocks_per_sm(bool bwd, int threads, int vec, int nit)
 {
     const int elems = vec == 1 ? 2 * nit : vec * nit;
-    return threads > kNgThreads || elems > 16 ? 1 : elems > 8 ? (bwd ? 1 : 2) : elems > 4 ? (bwd ? 2 : 4) : (bwd ? 4 : 5);
+    return threads > kNgThreads || elems > 16 ? 1 : elems > 8 ? 2 : elems > 4 ? (bwd ? 2 : 4) : (bwd ? 4 : 5);
 }
 
 }  // namespace
@@ -258,26 +258,42 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(false, MAXT, VEC, NIT
     }
 }
 
+// The weights and the sums of their gradients lie in shared memory in vectors of four
+// elements, vector q of a row's thread `lane` at (q * tpr + lane) * 4: registers are
+// what limits the rows in flight.
 template <typename T, int VEC, int NIT, int MAXT, int GATE, int ACT>
 __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT))
     k_norm_bwd(const __grid_constant__ NormArgs a, int tpr)
 {
     using R = Row<T, VEC, NIT>;
-    constexpr int P = R::kPairs;
+    constexpr int P = R::kPairs, Q = P / 2;
+    constexpr bool kAhead = VEC * NIT <= 8;  // the next row's loads before this one's sums
     __shared__ float sh[2 * 2 * 32];
-    extern __shared__ float ng_part[];  // [groups][2][D], more than one group a block
+    extern __shared__ float4 ng_smem[];
     int flip = 0;
     const int lane = threadIdx.x & (tpr - 1), c0 = lane * VEC, step = tpr * VEC, D = (int)a.D;
-    const int64_t groups = blockDim.x / tpr, g = threadIdx.x / tpr, stride = gridDim.x * groups;
+    const int groups = blockDim.x / tpr, g = threadIdx.x / tpr;
+    const int64_t stride = (int64_t)gridDim.x * groups;
     const bool full_gate = GATE == 1 || (GATE < 0 && a.gate && !a.gate_row);
     const bool row_gate = GATE == 2 || (GATE < 0 && a.gate && a.gate_row);
     const int act = ACT >= 0 ? ACT : a.act;
     const float inv_d = 1.0f / (float)a.D;
-    R post, pre, dpost, dpre;
-    load_weight(post, a.h ? a.post : nullptr, a.w_f32, c0, step, D);
-    load_weight(pre, a.dn ? a.pre : nullptr, a.w_f32, c0, step, D);
-#pragma unroll
-    for (int i = 0; i < P; i++) dpost.v[i] = dpre.v[i] = 0;
+    float4 *post = ng_smem + lane, *pre = post + Q * tpr, *dpost = pre + (1 + 2 * g) * Q * tpr, *dpre = dpost + Q * tpr;
+    if (g == 0) {
+        R w;
+        load_weight(w, a.h ? a.post : nullptr, a.w_f32, c0, step, D);
+        for (int q = 0; q < Q; q++) reinterpret_cast<ulonglong2 *>(post)[q * tpr] = make_ulonglong2(w.v[2 * q], w.v[2 * q + 1]);
+        load_weight(w, a.dn ? a.pre : nullptr, a.w_f32, c0, step, D);
+        for (int q = 0; q < Q; q++) reinterpret_cast<ulonglong2 *>(pre)[q * tpr] = make_ulonglong2(w.v[2 * q], w.v[2 * q + 1]);
+    }
+    for (int q = 0; q < Q; q++) dpost[q * tpr] = dpre[q * tpr] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __syncthreads();
+    auto four = [&](const float4 *p, int q) { return *reinterpret_cast<const ulonglong2 *>(p + q * tpr); };
+    auto add_four = [&](float4 *p, int q, uint64_t a0, uint64_t b0, uint64_t a1, uint64_t b1) {
+        ulonglong2 *at = reinterpret_cast<ulonglong2 *>(p + q * tpr);
+        const ulonglong2 z = *at;
+        *at = make_ulonglong2(fma2(a0, b0, z.x), fma2(a1, b1, z.y));
+    };
     RowPart<T, VEC, NIT> nt, nu, nx, nh, ng;
     float nrh = 0.0f, nrx = 0.0f, ngr = 0.0f;
     auto fetch = [&](int64_t r) {
@@ -291,10 +307,11 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT)
         if (a.dn) nrx = on ? a.rstd[a.R + r] : 0.0f;
         if (row_gate) ngr = on ? to_f32(((const T *)a.gate)[r * a.sg]) : 0.0f;
     };
-    fetch(blockIdx.x * groups + g);
+    if (kAhead) fetch(blockIdx.x * groups + g);
     for (int64_t r0 = blockIdx.x * groups; r0 < a.R; r0 += stride) {
         const int64_t r = r0 + g;
         const bool on = r < a.R;
+        if (!kAhead) fetch(r);
         // t: dx', then the gradient of x'; hh: h r(h); av, da: the gate's act and act'
         R t, hh, av, da, x, u;
         const float rh = nrh, rx = nrx, grow = ngr;
@@ -303,7 +320,7 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT)
         nx.get(x);
         nh.get(hh);
         if (full_gate) ng.get(av);
-        fetch(r + stride);
+        if (kAhead) fetch(r + stride);
         const float arow = row_gate ? act_value(a.act, grow) : 1.0f;
         if (a.h) {
             const uint64_t k = two(rh, rh);
@@ -318,16 +335,27 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT)
             const uint64_t k = two(kf, kf), kx = two(rx, rx);
             uint64_t m2 = 0;
 #pragma unroll
-            for (int i = 0; i < P; i++) {
-                if (a.h) {
-                    uint64_t y = mul2(hh.v[i], post.v[i]);
-                    if (full_gate) y = mul2(y, av.v[i]);
-                    x.v[i] = fma2(k, y, x.v[i]);
+            for (int q = 0; q < Q; q++) {
+                const ulonglong2 wp = four(pre, q);
+                ulonglong2 ws = make_ulonglong2(0, 0);
+                if (a.h) ws = four(post, q);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int i = 2 * q + j;
+                    if (a.h) {
+                        uint64_t y = mul2(hh.v[i], j ? ws.y : ws.x);
+                        if (full_gate) y = mul2(y, av.v[i]);
+                        x.v[i] = fma2(k, y, x.v[i]);
+                    }
+                    x.v[i] = mul2(x.v[i], kx);
                 }
-                x.v[i] = mul2(x.v[i], kx);
-                dpre.v[i] = fma2(u.v[i], x.v[i], dpre.v[i]);
-                u.v[i] = mul2(u.v[i], pre.v[i]);
-                m2 = fma2(u.v[i], x.v[i], m2);
+                add_four(dpre, q, u.v[2 * q], x.v[2 * q], u.v[2 * q + 1], x.v[2 * q + 1]);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int i = 2 * q + j;
+                    u.v[i] = mul2(u.v[i], j ? wp.y : wp.x);
+                    m2 = fma2(u.v[i], x.v[i], m2);
+                }
             }
             float m[1] = {sum_of(m2)};
             row_sum(m, tpr, sh, flip);
@@ -341,14 +369,22 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT)
             const uint64_t k = two(a.scale, a.scale), ka = two(arow, arow);
             uint64_t m2 = 0, row2 = 0;
 #pragma unroll
-            for (int i = 0; i < P; i++) {
-                const uint64_t st = mul2(t.v[i], k), sh_ = mul2(st, hh.v[i]), ty = mul2(sh_, post.v[i]);
-                const uint64_t ai = full_gate ? av.v[i] : ka;
-                if (full_gate) da.v[i] = mul2(ty, da.v[i]);
-                if (row_gate) row2 = add2(row2, ty);
-                dpost.v[i] = fma2(ai, sh_, dpost.v[i]);
-                t.v[i] = mul2(mul2(st, ai), post.v[i]);
-                m2 = fma2(t.v[i], hh.v[i], m2);
+            for (int q = 0; q < Q; q++) {
+                const ulonglong2 w = four(post, q);
+                uint64_t ai[2], sh_[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int i = 2 * q + j;
+                    const uint64_t wj = j ? w.y : w.x, st = mul2(t.v[i], k);
+                    sh_[j] = mul2(st, hh.v[i]);
+                    const uint64_t ty = mul2(sh_[j], wj);
+                    ai[j] = full_gate ? av.v[i] : ka;
+                    if (full_gate) da.v[i] = mul2(ty, da.v[i]);
+                    if (row_gate) row2 = add2(row2, ty);
+                    t.v[i] = mul2(mul2(st, ai[j]), wj);
+                    m2 = fma2(t.v[i], hh.v[i], m2);
+                }
+                add_four(dpost, q, ai[0], sh_[0], ai[1], sh_[1]);
             }
             if (on && full_gate && a.dgate) store_row(da, a.dgate, r * a.D, c0, step, D);
             float m[2] = {sum_of(m2), row_gate ? sum_of(row2) : 0.0f};
@@ -362,26 +398,18 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT)
         }
     }
     if (!a.part) return;
-    // the block's sums: its groups' parts added in order
-    float *part = a.part + (int64_t)blockIdx.x * 2 * D, *mine = groups > 1 ? ng_part + g * 2 * D : part;
-#pragma unroll
-    for (int i = 0; i < VEC * NIT; i++) {
-        const int c = c0 + i / VEC * step + i % VEC;
-        float f[2], q[2];
-        both(dpost.v[i / 2], f[0], f[1]);
-        both(dpre.v[i / 2], q[0], q[1]);
-        if (c < D) {
-            mine[c] = f[i % 2];
-            mine[D + c] = q[i % 2];
-        }
-    }
-    if (groups > 1) {
-        __syncthreads();
-        for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) {
-            float v = 0.0f;
-            for (int j = 0; j < (int)groups; j++) v += ng_part[j * 2 * D + c];
-            part[c] = v;
-        }
+    // the block's sums: its groups' parts added in order, dpost then dpre
+    __syncthreads();
+    float *part = a.part + (int64_t)blockIdx.x * 2 * D;
+    const float *sums = reinterpret_cast<const float *>(ng_smem + 2 * Q * tpr);  // [groups][2][Q][tpr][4]
+    for (int j = threadIdx.x; j < 2 * 4 * Q * tpr; j += blockDim.x) {
+        const int which = j / (4 * Q * tpr), k = j - which * (4 * Q * tpr);
+        const int f = k / (4 * tpr) * 4 + k % 4, l = k / 4 % tpr;  // the element of thread l
+        const int c = l * VEC + f / VEC * step + f % VEC;
+        if (c >= D) continue;
+        float v = 0.0f;
+        for (int i = 0; i < groups; i++) v += sums[(int64_t)i * 8 * Q * tpr + j];
+        part[which * D + c] = v;
     }
 }
 
@@ -420,9 +448,11 @@ struct NormShape {
     int vec, nit, tpr, threads;
 };
 
-// A row that a warp can hold stays in one warp (no block barrier); a longer one
-// takes a thread for each vector up to a block of kNgThreads, then more vectors
-// a thread, then a block of kNgMaxThreads.
+// A row that a warp can hold at kNgMaxElems a thread stays in one warp (no block
+// barrier); a longer one takes as few threads as hold it so, since a row costs each
+// thread some 250 instructions besides its elements (bf16 rows of 2048: forward 150 us
+// with 8 elements a thread, 121 us with 16); rows that are read element by element
+// take more threads instead.
 bool norm_shape(int64_t D, bool wide, int elem, NormShape &s)
 {
     s.vec = wide ? 16 / elem : 1;
@@ -440,7 +470,7 @@ bool norm_shape(int64_t D, bool wide, int elem, NormShape &s)
         if (tpr >= vecs) return spread(tpr);
     if (spread(32)) return true;
     for (int tpr = 64; tpr <= kNgThreads; tpr *= 2)
-        if (tpr >= vecs) return spread(tpr);
+        if (wide ? spread(tpr) : tpr >= vecs) return spread(tpr);
     if (spread(kNgThreads)) return true;
     s.threads = kNgMaxThreads;
     return spread(kNgMaxThreads);
@@ -457,10 +487,16 @@ template <typename T, int VEC, int NIT, int MAXT, int GATE, int ACT = -1>
 void norm_launch(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
 {
     const unsigned blocks = (unsigned)norm_blocks(sh, a.R, bwd);
-    const size_t groups = sh.threads / sh.tpr, smem = groups > 1 && a.part ? groups * 2 * a.D * 4 : 0;  // 32 KB at most
     count_launches(1);
-    if (bwd) k_norm_bwd<T, VEC, NIT, MAXT, GATE, ACT><<<blocks, MAXT, smem, s>>>(a, sh.tpr);
-    else k_norm_fwd<T, VEC, NIT, MAXT, GATE, ACT><<<blocks, MAXT, 0, s>>>(a, sh.tpr);
+    if (bwd) {
+        // weights, and each group's sums: 2 * (1 + groups) rows of tpr * VEC * NIT floats
+        const size_t smem = (size_t)2 * (1 + sh.threads / sh.tpr) * sh.tpr * VEC * NIT * 4;  // 128 KB at most
+        auto kern = k_norm_bwd<T, VEC, NIT, MAXT, GATE, ACT>;
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        kern<<<blocks, MAXT, smem, s>>>(a, sh.tpr);
+    } else {
+        k_norm_fwd<T, VEC, NIT, MAXT, GATE, ACT><<<blocks, MAXT, 0, s>>>(a, sh.tpr);
+    }
 }
 
 template <typename T, int VEC, int NIT>
