@@ -60,36 +60,44 @@ struct NormArgs {
 __host__ __device__ constexpr int norm_blocks_per_sm(bool bwd, int threads, int vec, int nit)
 {
     const int elems = vec == 1 ? 2 * nit : vec * nit;
-    return threads > kNgThreads || elems > 16 ? 1 : elems > 8 ? 2 : elems > 4 ? (bwd ? 2 : 4) : (bwd ? 4 : 5);
+    return threads > kNgThreads || elems > 16 ? 1 : elems > 8 ? 2 : elems > 4 ? (bwd ? 2 : 3) : (bwd ? 4 : 5);
 }
 
 }  // namespace
 
-// Sums NV values over the TPR threads of a row; every thread gets them.
-// `sh`: NV * warps of the block floats, used twice alternately by `flip`.
+// Sums NV values over the tpr threads of a row (a power of two); every thread gets
+// them.  `sh`: 2 * NV * 32 floats, halves used alternately by `flip`.
 template <int NV>
 __device__ __forceinline__ void row_sum(float (&v)[NV], int tpr, float *sh, int &flip)
 {
-    const int in_warp = tpr < 32 ? tpr : 32;
-    for (int o = in_warp >> 1; o > 0; o >>= 1) {
+    if (tpr >= 32) {
 #pragma unroll
-        for (int i = 0; i < NV; i++) v[i] += __shfl_xor_sync(~0u, v[i], o);
+        for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) v[i] += __shfl_xor_sync(~0u, v[i], o);
+        }
+    } else {
+        for (int o = tpr >> 1; o > 0; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) v[i] += __shfl_xor_sync(~0u, v[i], o);
+        }
     }
     if (tpr > 32) {
         // rows of one block reduce in lockstep: every group makes the same calls
-        const int warp = threadIdx.x >> 5, wpr = tpr >> 5, w0 = warp / wpr * wpr;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wpr = tpr >> 5;
         float *buf = sh + flip * NV * 32;
         flip ^= 1;
-        if ((threadIdx.x & 31) == 0) {
+        if (lane == 0) {
 #pragma unroll
             for (int i = 0; i < NV; i++) buf[i * 32 + warp] = v[i];
         }
         __syncthreads();
+        const int at = (warp & -wpr) + (lane & (wpr - 1));
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            float s = 0.0f;
-            for (int w = 0; w < wpr; w++) s += buf[i * 32 + w0 + w];
-            v[i] = s;
+        for (int i = 0; i < NV; i++) v[i] = buf[i * 32 + at];
+        for (int o = wpr >> 1; o > 0; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) v[i] += __shfl_xor_sync(~0u, v[i], o);
         }
     }
 }
@@ -135,18 +143,21 @@ struct Row {
 };
 
 // A row's vectors of one tensor, as they are in memory: loaded for the next row
-// while the present one waits for its sums.  Absent tensors and columns are zero.
+// while the present one waits for its sums.  Absent tensors and columns are zero and
+// never loaded; a row past the last is loaded as the last one and then cleared.
 template <typename T, int VEC, int NIT>
 struct RowPart {
     Pack<T, VEC> p[NIT];
-    __device__ __forceinline__ void load(const void *base, int64_t at, int c0, int step, int D, bool on)
+    __device__ __forceinline__ void clear()
     {
 #pragma unroll
-        for (int i = 0; i < NIT; i++) {
-            const int c = c0 + i * step;
-            p[i].zero();
-            if (on && c < D) p[i].load((const T *)base + at + c);
-        }
+        for (int i = 0; i < NIT; i++) p[i].zero();
+    }
+    __device__ __forceinline__ void load(const void *row, int step, const bool (&in)[NIT])
+    {
+#pragma unroll
+        for (int i = 0; i < NIT; i++)
+            if (in[i]) p[i].load((const T *)row + i * step);
     }
     __device__ __forceinline__ void get(Row<T, VEC, NIT> &x) const
     {
@@ -159,14 +170,16 @@ struct RowPart {
 };
 
 template <typename T, int VEC, int NIT>
-__device__ __forceinline__ void store_row(const Row<T, VEC, NIT> &x, void *base, int64_t at, int c0, int step, int D)
+__device__ __forceinline__ void store_row(const Row<T, VEC, NIT> &x, void *base, int64_t at, int step,
+                                          const bool (&in)[NIT])
 {
+    T *row = (T *)base + at;
     float f[NIT][VEC];
 #pragma unroll
     for (int i = 0; i < VEC * NIT; i += 2) both(x.v[i / 2], f[i / VEC][i % VEC], f[(i + 1) / VEC][(i + 1) % VEC]);
 #pragma unroll
     for (int i = 0; i < NIT; i++)
-        if (c0 + i * step < D) store_f32((T *)base + at + c0 + i * step, f[i]);
+        if (in[i]) store_f32(row + i * step, f[i]);
 }
 
 // A weight's elements of this thread, zero past the row's end.
@@ -204,14 +217,20 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(false, MAXT, VEC, NIT
     R post, pre;
     load_weight(post, a.h ? a.post : nullptr, a.w_f32, c0, step, D);
     load_weight(pre, a.n ? a.pre : nullptr, a.w_f32, c0, step, D);
+    bool in[NIT];
+#pragma unroll
+    for (int i = 0; i < NIT; i++) in[i] = c0 + i * step < D;
     RowPart<T, VEC, NIT> nx, nh, ng;
+    nx.clear();
+    nh.clear();
+    ng.clear();
     float grow = 0.0f;
     auto fetch = [&](int64_t r) {
-        const bool on = r < a.R;
-        nx.load(a.x, r * a.sx, c0, step, D, on);
-        nh.load(a.h, r * a.sh, c0, step, D, on && a.h);
-        if (full_gate) ng.load(a.gate, r * a.sg, c0, step, D, on);
-        if (row_gate) grow = on ? to_f32(((const T *)a.gate)[r * a.sg]) : 0.0f;
+        r = min(r, a.R - 1);
+        nx.load((const T *)a.x + r * a.sx + c0, step, in);
+        if (a.h) nh.load((const T *)a.h + r * a.sh + c0, step, in);
+        if (full_gate) ng.load((const T *)a.gate + r * a.sg + c0, step, in);
+        if (row_gate) grow = to_f32(((const T *)a.gate)[r * a.sg]);
     };
     fetch(blockIdx.x * groups + g);
     // every group of a block makes the same number of rounds
@@ -240,7 +259,7 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(false, MAXT, VEC, NIT
                 if (full_gate) y = mul2(y, act_pair(act, gt.v[i], nullptr));
                 x.v[i] = fma2(kk, y, x.v[i]);
             }
-            if (on) store_row(x, a.xo, r * a.D, c0, step, D);
+            if (on) store_row(x, a.xo, r * a.D + c0, step, in);
         }
         if (a.n) {
             uint64_t s2 = 0;
@@ -253,7 +272,7 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(false, MAXT, VEC, NIT
             const uint64_t k = two(rx, rx);
 #pragma unroll
             for (int i = 0; i < P; i++) x.v[i] = mul2(mul2(x.v[i], k), pre.v[i]);
-            if (on) store_row(x, a.n, r * a.D, c0, step, D);
+            if (on) store_row(x, a.n, r * a.D + c0, step, in);
         }
     }
 }
@@ -294,18 +313,43 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT)
         const ulonglong2 z = *at;
         *at = make_ulonglong2(fma2(a0, b0, z.x), fma2(a1, b1, z.y));
     };
+    bool in[NIT];
+#pragma unroll
+    for (int i = 0; i < NIT; i++) in[i] = c0 + i * step < D;
     RowPart<T, VEC, NIT> nt, nu, nx, nh, ng;
+    nt.clear();
+    nu.clear();
+    nx.clear();
+    nh.clear();
+    ng.clear();
     float nrh = 0.0f, nrx = 0.0f, ngr = 0.0f;
-    auto fetch = [&](int64_t r) {
-        const bool on = r < a.R;
-        nu.load(a.dn, r * a.sdn, c0, step, D, on && a.dn);
-        nx.load(a.x, r * a.sx, c0, step, D, on && a.dn);
-        nh.load(a.h, r * a.sh, c0, step, D, on && a.h);
-        if (full_gate) ng.load(a.gate, r * a.sg, c0, step, D, on);
-        nt.load(a.dxo, r * a.sdx, c0, step, D, on && a.dxo);
-        if (a.h) nrh = on ? a.rstd[r] : 0.0f;
-        if (a.dn) nrx = on ? a.rstd[a.R + r] : 0.0f;
-        if (row_gate) ngr = on ? to_f32(((const T *)a.gate)[r * a.sg]) : 0.0f;
+    auto fetch = [&](int64_t row) {
+        const int64_t r = min(row, a.R - 1);
+        if (!kAhead) {  // nothing of a row lives past it
+            nt.clear();
+            nu.clear();
+            nx.clear();
+            nh.clear();
+            ng.clear();
+        }
+        if (a.dn) {
+            nu.load((const T *)a.dn + r * a.sdn + c0, step, in);
+            nx.load((const T *)a.x + r * a.sx + c0, step, in);
+            nrx = a.rstd[a.R + r];
+        }
+        if (a.h) {
+            nh.load((const T *)a.h + r * a.sh + c0, step, in);
+            nrh = a.rstd[r];
+        }
+        if (full_gate) ng.load((const T *)a.gate + r * a.sg + c0, step, in);
+        if (a.dxo) nt.load((const T *)a.dxo + r * a.sdx + c0, step, in);
+        if (row_gate) ngr = to_f32(((const T *)a.gate)[r * a.sg]);
+        if (row >= a.R) {  // adds nothing to the sums
+            nt.clear();
+            nu.clear();
+            nx.clear();
+            nh.clear();
+        }
     };
     if (kAhead) fetch(blockIdx.x * groups + g);
     for (int64_t r0 = blockIdx.x * groups; r0 < a.R; r0 += stride) {
@@ -364,7 +408,7 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT)
 #pragma unroll
             for (int i = 0; i < P; i++) t.v[i] = fma2(kx, fma2(x.v[i], mm, u.v[i]), t.v[i]);
         }
-        if (on && a.dx) store_row(t, a.dx, r * a.D, c0, step, D);
+        if (on && a.dx) store_row(t, a.dx, r * a.D + c0, step, in);
         if (a.h) {
             const uint64_t k = two(a.scale, a.scale), ka = two(arow, arow);
             uint64_t m2 = 0, row2 = 0;
@@ -386,14 +430,14 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT)
                 }
                 add_four(dpost, q, ai[0], sh_[0], ai[1], sh_[1]);
             }
-            if (on && full_gate && a.dgate) store_row(da, a.dgate, r * a.D, c0, step, D);
+            if (on && full_gate && a.dgate) store_row(da, a.dgate, r * a.D + c0, step, in);
             float m[2] = {sum_of(m2), row_gate ? sum_of(row2) : 0.0f};
             row_sum(m, tpr, sh, flip);
             const float mw = -m[0] * inv_d;
             const uint64_t mm = two(mw, mw), kh = two(rh, rh);
 #pragma unroll
             for (int i = 0; i < P; i++) t.v[i] = mul2(kh, fma2(hh.v[i], mm, t.v[i]));
-            if (on && a.dh) store_row(t, a.dh, r * a.D, c0, step, D);
+            if (on && a.dh) store_row(t, a.dh, r * a.D + c0, step, in);
             if (row_gate && a.dgate && on && lane == 0) ((T *)a.dgate)[r] = from_f32<T>(m[1] * act_grad(a.act, grow));
         }
     }
@@ -448,32 +492,27 @@ struct NormShape {
     int vec, nit, tpr, threads;
 };
 
-// A row that a warp can hold at kNgMaxElems a thread stays in one warp (no block
-// barrier); a longer one takes as few threads as hold it so, since a row costs each
-// thread some 250 instructions besides its elements (bf16 rows of 2048: forward 150 us
-// with 8 elements a thread, 121 us with 16); rows that are read element by element
-// take more threads instead.
-bool norm_shape(int64_t D, bool wide, int elem, NormShape &s)
+// A row takes as few threads as hold it at 16 (fp32 forward: 8) elements each,
+// in one warp if it can: a row costs each thread some 150 instructions besides its
+// elements (bf16 rows of 2048: forward 150 us with 8 elements a thread, 109 us with 16).
+// Rows that are read element by element take more threads instead.
+bool norm_shape(int64_t D, bool wide, int elem, bool bwd, NormShape &s)
 {
     s.vec = wide ? 16 / elem : 1;
     const int64_t vecs = (D + s.vec - 1) / s.vec;
-    const int most = kNgMaxElems / s.vec;
-    auto spread = [&](int tpr) {
+    auto spread = [&](int tpr, int elems) {
         s.tpr = tpr;
-        s.nit = 1;
-        // one element a vector: 4 or 16 of them, whichever is enough
-        while (s.nit < most && ((int64_t)s.tpr * s.nit < vecs || (!wide && s.nit < 4) || (!wide && s.nit == 8))) s.nit *= 2;
+        s.nit = wide ? 1 : 4;  // one element a vector: 4 or 16 of them
+        while (s.nit * s.vec < elems && (int64_t)s.tpr * s.nit < vecs) s.nit *= wide ? 2 : 4;
         return (int64_t)s.tpr * s.nit >= vecs;
     };
     s.threads = kNgThreads;
-    for (int tpr = 8; tpr < 32; tpr *= 2)
-        if (tpr >= vecs) return spread(tpr);
-    if (spread(32)) return true;
-    for (int tpr = 64; tpr <= kNgThreads; tpr *= 2)
-        if (wide ? spread(tpr) : tpr >= vecs) return spread(tpr);
-    if (spread(kNgThreads)) return true;
+    for (int tpr = 8; tpr <= kNgThreads; tpr *= 2)
+        if (spread(tpr, tpr < 32 ? s.vec : !wide ? (tpr == 32 ? kNgMaxElems : 4) : elem == 2 || bwd ? kNgMaxElems : 8))
+            return true;
+    if (spread(kNgThreads, kNgMaxElems)) return true;
     s.threads = kNgMaxThreads;
-    return spread(kNgMaxThreads);
+    return spread(kNgMaxThreads, kNgMaxElems);
 }
 
 int64_t norm_blocks(const NormShape &s, int64_t R, bool bwd)
@@ -594,7 +633,7 @@ extern "C" int lifb_norm_gate_fwd(const lifb_norm_gate *p, void *xo, void *n, vo
     if (n) wide = wide && aligned16(a.pre);
     if (a.gate && !a.gate_row) wide = wide && a.sg % vec == 0 && aligned16(a.gate);
     NormShape sh;
-    if (!norm_shape(a.D, wide, (int)dtype_bytes(p->dtype), sh))
+    if (!norm_shape(a.D, wide, (int)dtype_bytes(p->dtype), false, sh))
         return norm_fail(LIFB_ERR_UNSUPPORTED, what, "rows longer than 8192 elements");
     LIFB_BY_DTYPE(p->dtype, T, norm_run<T>(false, a, sh, (cudaStream_t)stream));
     if (cudaGetLastError() != cudaSuccess) return norm_fail(LIFB_ERR_CUDA, what, "launch failed");
@@ -609,7 +648,7 @@ extern "C" size_t lifb_norm_gate_bwd_workspace_bytes(int64_t R, int64_t D, int d
     size_t most = 0;  // of the vector and the element form
     for (int wide = 0; wide < 2; wide++) {
         NormShape sh;
-        if (norm_shape(D, wide != 0, (int)dtype_bytes(dtype), sh))
+        if (norm_shape(D, wide != 0, (int)dtype_bytes(dtype), true, sh))
             most = std::max(most, (size_t)norm_blocks(sh, R, true) * 2 * D * 4);
     }
     return most;
@@ -653,7 +692,7 @@ extern "C" int lifb_norm_gate_bwd(const lifb_norm_gate *p, const void *dxo, int6
     if (a.h) wide = wide && a.sh % vec == 0 && aligned16(a.h) && aligned16(a.post);
     if (a.gate && !a.gate_row) wide = wide && a.sg % vec == 0 && aligned16(a.gate) && aligned16(dgate);
     NormShape sh;
-    if (!norm_shape(a.D, wide, (int)dtype_bytes(p->dtype), sh))
+    if (!norm_shape(a.D, wide, (int)dtype_bytes(p->dtype), true, sh))
         return norm_fail(LIFB_ERR_UNSUPPORTED, what, "rows longer than 8192 elements");
     LIFB_BY_DTYPE(p->dtype, T, norm_run<T>(true, a, sh, s));
     if (weights) {
