@@ -10,6 +10,7 @@ import ctypes
 import os
 import struct
 import threading
+import time
 
 import torch
 
@@ -263,16 +264,16 @@ def addr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-# The current stream's handle: torch's own raw accessor where it has one (a tenth of
-# the time of building a Stream object), else the Stream object's.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# The current stream's handle and the current device: torch's own raw accessors where
+# it has them (a tenth of the time of a Stream object), else the public ones.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda i: torch.cuda.current_stream(i).cuda_stream)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def raw_stream(t: torch.Tensor) -> int:
     """Handle of the current stream of the tensor's device."""
-    if _raw_stream is not None:
-        return _raw_stream(t.device.index)
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return _raw_stream(t.get_device())
 
 
 class _Here:
@@ -288,22 +289,38 @@ _here = _Here()
 
 def on_device(t: torch.Tensor):
     """torch.cuda.device(t.device) where that is not the current device already."""
-    return _here if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _here if t.get_device() == _raw_device() else torch.cuda.device(t.device)
 
 
-def need_cuda(what: str, **tensors) -> None:
-    """Raises unless every tensor given (None: absent) is on one CUDA device."""
+def need_cuda(what: str, names: str, *tensors) -> None:
+    """Raises unless every tensor given (None: absent) is on one CUDA device; `names`:
+    what they are called, in order."""
     dev = None
-    for name, t in tensors.items():
+    for t in tensors:
         if t is None:
             continue
-        d = t.device
-        if d.type != "cuda":
-            raise RuntimeError(f"{what}: {name} must be a CUDA tensor")
+        d = t.get_device()
         if dev is None:
             dev = d
-        elif d != dev:
-            raise RuntimeError(f"{what}: {name} is on {d}, not {dev}")
+        if d < 0 or d != dev:
+            break
+    else:
+        return
+    name = names.split()[[x is t for x in tensors].index(True)]
+    raise RuntimeError(f"{what}: {name} must be a CUDA tensor" if d < 0 else
+                       f"{what}: {name} is on {t.device}, not cuda:{dev}")
+
+
+_poll_again = 0.0  # when the next poll is due
+
+
+def poll_device_sometimes(what: str) -> None:
+    """poll_device, at most every 20 ms: for calls as short as the poll itself."""
+    global _poll_again
+    now = time.monotonic()
+    if now >= _poll_again:
+        _poll_again = now + 0.02
+        poll_device(what)
 
 
 class Stats(ctypes.Structure):

@@ -54,7 +54,7 @@ class Embedding(torch.autograd.Function):
             check(lib.lifb_embed_bwd(addr(tokens), tokens.element_size(), addr(dy), addr(dw), n, V, D,
                                      max(s0, D), scale, DTYPES[dtype], ws.data_ptr(), nb, raw_stream(dy)),
                   "embedding")
-            _lib.poll_device("embedding")
+            _lib.poll_device_sometimes("embedding")
         return None, dw, None
 
 
@@ -67,9 +67,9 @@ def embedding(tokens, weight, scale=1.0):
         raise TypeError(f"embedding: weight must be fp32, bf16 or fp16, got {weight.dtype}")
     if tokens.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"embedding: tokens must be int32 or int64, got {tokens.dtype}")
-    need_cuda("embedding", tokens=tokens, weight=weight)
+    need_cuda("embedding", "tokens weight", tokens, weight)
     tokens = tokens.contiguous()
-    if weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
+    if not weight.is_contiguous() and (weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]):
         weight = weight.contiguous()
     if weight.requires_grad and torch.is_grad_enabled():
         return Embedding.apply(tokens, weight, float(scale))

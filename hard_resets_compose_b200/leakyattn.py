@@ -81,7 +81,7 @@ class LeakyAttention(torch.autograd.Function):
             check(lib.lifb_leaky_attn_bwd(args, addr(do), (_lib.c_i64 * 3)(*do.stride()[:3]), addr(dout), addr(dq),
                                           addr(dk), addr(dv), addr(ds), addr(ws), nb, raw_stream(q)),
                   "leaky_attention")
-            _lib.poll_device("leaky_attention")
+            _lib.poll_device_sometimes("leaky_attention")
         return dq, dk, dv, None, ds, None, None, None
 
 
@@ -121,7 +121,7 @@ def leaky_attention(q, k, v, log_decay, state=None, lengths=None, scale=None, re
     q, k, v and state."""
     what = "leaky_attention"
     H, _, Dk, Dv = _check(what, q, k, v, log_decay, 2, _SEQ_TYPES)
-    need_cuda(what, q=q, k=k, v=v, log_decay=log_decay, state=state, lengths=lengths)
+    need_cuda(what, "q k v log_decay state lengths", q, k, v, log_decay, state, lengths)
     B = q.shape[0]
     if state is not None:
         if state.shape != (B, H, Dk, Dv) or state.dtype != torch.float32:
@@ -152,7 +152,7 @@ def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     cache (-1, say) is empty: zeros out, nothing changed.  Not differentiable."""
     what = "leaky_attention_step"
     H, Hk, Dk, Dv = _check(what, q, k, v, log_decay, 1, _STEP_TYPES)
-    need_cuda(what, q=q, k=k, v=v, log_decay=log_decay, state=state, slots=slots)
+    need_cuda(what, "q k v log_decay state slots", q, k, v, log_decay, state, slots)
     B = q.shape[0]
     if state.dim() != 4 or state.shape[1:] != (H, Dk, Dv) or state.dtype != torch.float32:
         raise ValueError(f"{what}: state must be [slots, {H}, {Dk}, {Dv}] fp32, got {tuple(state.shape)} {state.dtype}")

@@ -29,6 +29,8 @@ def _rows(t, D):
     """t as [R, D] rows with a row stride, without a copy where it has one."""
     if t.dim() != 2:
         t = t.reshape(-1, D)
+    if t.is_contiguous():
+        return t
     s0, s1 = t.stride()
     if s1 != 1 and D > 1 or s0 < D and t.shape[0] > 1:
         t = t.contiguous()
@@ -105,7 +107,7 @@ def _run(what, x, h, gate, post, pre, scale, eps, act):
     D = shape[-1] if shape else 0
     if dt not in DTYPES:
         raise TypeError(f"{what}: x must be fp32, bf16 or fp16, got {dt}")
-    need_cuda(what, x=x, h=h, gate=gate, post_weight=post, pre_weight=pre)
+    need_cuda(what, "x h gate post_weight pre_weight", x, h, gate, post, pre)
     for name, t in (("h", h), ("gate", gate)):
         if t is not None:
             if t.dtype != dt:
