@@ -225,48 +225,64 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
     } else if (group == kScores) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kT32Regs[kScores]));
         if (!STATE_ONLY) {
-            float pw[16];  // b^i
+            uint64_t pw[8];  // of 16 columns in their order, from the one nearest the diagonal
 #pragma unroll
-            for (int i = 0; i < 16; i++) pw[i] = decay_pow(ld, (float)i);
+            for (int i = 0; i < 8; i++) {
+                const float lo = decay_pow(ld, (float)(p.rev ? 2 * i : 15 - 2 * i));
+                const float hi = decay_pow(ld, (float)(p.rev ? 2 * i + 1 : 14 - 2 * i));
+                pw[i] = two(lo, hi);
+            }
             const float near = decay_pow(ld, (float)lane);
             const int w4 = warp & 3;
             for (int c = 0; c < chunks; c++) {
                 const int n = min(kT32C, end - (t_first + c * t_step));
                 if (!wait(&bars.p_full, c)) break;
                 tcgen05_after();
-                uint32_t x[16];
 #pragma unroll 1
                 for (int s = 0; s < 8; s++) {
                     const int c0 = s * 16, blk = s >> 1;
                     const bool past = p.rev ? blk < w4 : blk > w4;  // on the other side of the diagonal
-                    uint32_t out[3][8] = {};
-                    if (!past) {
-                        tmem_load16(tmem + lanes + c0, x);
-                        tmem_wait_ld();
-                        if (blk == w4) {
+                    if (past) {
+                        const uint32_t zero[8] = {};
 #pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                const int d = p.rev ? c0 + e - st : st - c0 - e;  // -31 .. 31
-                                const float f = __shfl_sync(~0u, near, d & 31);
-                                x[e] = d >= 0 && c0 + e < n ? __float_as_uint(__uint_as_float(x[e]) * (p.p_scale * f)) : 0u;
-                            }
-                        } else {
-                            // the nearest column's distance, then pw of the others' from there
-                            const float f = p.p_scale * decay_pow(ld, (float)(p.rev ? c0 - st : st - c0 - 15));
+                        for (int q = 0; q < 3; q++) tmem_store8(tmem + lanes + kT32Pa + q * 64 + s * 8, zero);
+                        continue;
+                    }
+                    uint32_t x[16];
+                    tmem_load16(tmem + lanes + c0, x);
+                    // the nearest column's power, then pw's of the others from there
+                    const float f = p.p_scale * decay_pow(ld, (float)max(0, p.rev ? c0 - st : st - c0 - 15));
+                    tmem_wait_ld();
+                    if (blk == w4) {
 #pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                const float g = p.rev ? pw[e] : pw[15 - e];
-                                x[e] = c0 + e < n ? __float_as_uint(__uint_as_float(x[e]) * (f * g)) : 0u;
-                            }
+                        for (int e = 0; e < 16; e++) {
+                            const int d = p.rev ? c0 + e - st : st - c0 - e;  // -31 .. 31
+                            const float g = __shfl_sync(~0u, near, d & 31);
+                            x[e] = d >= 0 && c0 + e < n ? __float_as_uint(__uint_as_float(x[e]) * (p.p_scale * g)) : 0u;
                         }
+                    } else {
+                        const uint64_t ff = two(f, f);
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
-                            uint64_t r = two(x[2 * i], x[2 * i + 1]);
+                            float lo, hi;
+                            both(mul2(two(x[2 * i], x[2 * i + 1]), mul2(pw[i], ff)), lo, hi);
+                            x[2 * i] = __float_as_uint(lo);
+                            x[2 * i + 1] = __float_as_uint(hi);
+                        }
+                        if (c0 + 16 > n) {
 #pragma unroll
-                            for (int q = 0; q < 3; q++) {
-                                out[q][i] = pack2_bf16(r);
-                                if (q < 2) r = fma2(two(bf16_lo(out[q][i]), bf16_hi(out[q][i])), two(-1.0f, -1.0f), r);
-                            }
+                            for (int e = 0; e < 16; e++)
+                                if (c0 + e >= n) x[e] = 0;
+                        }
+                    }
+                    uint32_t out[3][8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        uint64_t r = two(x[2 * i], x[2 * i + 1]);
+#pragma unroll
+                        for (int q = 0; q < 3; q++) {
+                            out[q][i] = pack2_bf16(r);
+                            if (q < 2) r = fma2(two(bf16_lo(out[q][i]), bf16_hi(out[q][i])), two(-1.0f, -1.0f), r);
                         }
                     }
 #pragma unroll
