@@ -561,6 +561,7 @@ int at_check(const char *what, const lifb_leaky_attn *p)
 
 bool run_passes(AttnArgs &a, int passes, int dtype, cudaStream_t s)
 {
+    a.passes = passes;
     const bool tc = attn_tc_applies(a, passes, dtype), tc32 = attn_tc32_applies(a, passes, dtype);
     // on the tensor cores a returned state comes from the state's own kernel, except where
     // the main one has it at hand

@@ -50,6 +50,8 @@ struct AttnArgs {
     const float *log_decay;       // [H]
     const int32_t *lengths;       // [B], or NULL: every sequence has T tokens
     int64_t B, T, H;
+    int passes;                   // of this launch: the fastest part of the block's number, so that the
+                                  // passes over one head run together and share its operands in L2
     int nseg;                     // time segments, each with a multiple of kAttnSegGrain tokens
     int64_t seg_tokens;
 };

@@ -61,10 +61,10 @@ __global__ void __launch_bounds__((StateLayout<DQ, DV, NP>::threads), 1)
     __shared__ StateBars bars;
     __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0), group = warp >> 2;
-    const int pi = blockIdx.y;
+    const int pi = blockIdx.x % a.passes, item = blockIdx.x / a.passes;
     const AttnPass &p = a.p[pi];
-    const int64_t bh = blockIdx.x / a.nseg;
-    const int u = (int)(blockIdx.x - bh * a.nseg);                // in the order of the pass
+    const int64_t bh = item / a.nseg;
+    const int u = (int)(item - bh * a.nseg);                // in the order of the pass
     if (u == a.nseg - 1 && !(finish && p.s_out)) return;          // nothing starts from the last one
     const int64_t b = bh / a.H, h = bh - b * a.H;
     const int64_t len = attn_length(a.lengths, b, a.T);
@@ -278,7 +278,7 @@ bool launch_state(const AttnArgs &a, const StateMaps &m, int passes, bool finish
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes + 1024) != cudaSuccess)
             return false;
         count_launches(1);
-        kern<<<dim3((unsigned)(a.B * a.H * a.nseg), (unsigned)passes), threads, bytes + 1024, s>>>(a, m, finish,
+        kern<<<(unsigned)(a.B * a.H * a.nseg * passes), threads, bytes + 1024, s>>>(a, m, finish,
                                                                                                  device_status_ptr());
         return true;
     };
@@ -308,6 +308,7 @@ bool attn_state(const AttnArgs &a, int passes, bool finish, cudaStream_t s)
             launched[j] = true;
             b.p[n++] = p;
         }
+        b.passes = n;
         const bool ok = wq ? (wv ? launch_state<128, 128>(b, m, n, finish, s) : launch_state<128, 64>(b, m, n, finish, s))
                            : (wv ? launch_state<64, 128>(b, m, n, finish, s) : launch_state<64, 64>(b, m, n, finish, s));
         if (!ok) return false;

@@ -167,10 +167,10 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     __shared__ TcBars bars;
     __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0), group = warp >> 2;
-    const int pi = blockIdx.y;
+    const int pi = blockIdx.x % a.passes, item = blockIdx.x / a.passes;
     const AttnPass &p = a.p[pi];
-    const int64_t bh = blockIdx.x / a.nseg;
-    const int u = (int)(blockIdx.x - bh * a.nseg);  // in the order of the pass
+    const int64_t bh = item / a.nseg;
+    const int u = (int)(item - bh * a.nseg);  // in the order of the pass
     const int64_t b = bh / a.H, h = bh - b * a.H;
     const int64_t len = attn_length(a.lengths, b, a.T);
     const float ld = a.log_decay[h];
@@ -606,7 +606,7 @@ bool launch_tc(const AttnArgs &a, const AttnMaps &m, int passes, cudaStream_t s)
     auto kern = k_attn_tc<DQ, DV, NP>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
     count_launches(1);
-    kern<<<dim3((unsigned)(a.B * a.H * a.nseg), (unsigned)passes), L::threads, smem, s>>>(a, m, device_status_ptr());
+    kern<<<(unsigned)(a.B * a.H * a.nseg * passes), L::threads, smem, s>>>(a, m, device_status_ptr());
     return true;
 }
 
@@ -652,6 +652,7 @@ bool attn_tc(const AttnArgs &a, int passes, cudaStream_t s)
             launched[j] = true;
             b.p[n++] = p;
         }
+        b.passes = n;
         const bool ok = dq == 64 ? (dv != 64      ? launch_tc<64, 128, 2>(b, m, n, s)
                                     : exact_state ? launch_tc<64, 64, 3>(b, m, n, s)
                                                   : launch_tc<64, 64, 2>(b, m, n, s))

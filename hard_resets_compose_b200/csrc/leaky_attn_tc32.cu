@@ -120,9 +120,10 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
     __shared__ T32Bars bars;
     __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0), group = warp >> 2;
-    const AttnPass &p = a.p[blockIdx.y];
-    const int64_t bh = blockIdx.x / a.nseg;
-    const int u = (int)(blockIdx.x - bh * a.nseg);  // in the order of the pass
+    const int item = blockIdx.x / a.passes;
+    const AttnPass &p = a.p[blockIdx.x % a.passes];
+    const int64_t bh = item / a.nseg;
+    const int u = (int)(item - bh * a.nseg);  // in the order of the pass
     if (STATE_ONLY && u == a.nseg - 1) return;      // nothing starts from the last one
     const int64_t b = bh / a.H, h = bh - b * a.H;
     const int64_t len = attn_length(a.lengths, b, a.T);
@@ -502,7 +503,7 @@ bool attn_tc32(const AttnArgs &a, int passes, bool state_only, cudaStream_t s)
     const size_t smem = kT32Bytes + 1024;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
     count_launches(1);
-    kern<<<dim3((unsigned)(a.B * a.H * a.nseg), (unsigned)passes), kT32Threads, smem, s>>>(a, device_status_ptr());
+    kern<<<(unsigned)(a.B * a.H * a.nseg * passes), kT32Threads, smem, s>>>(a, device_status_ptr());
     return true;
 }
 
