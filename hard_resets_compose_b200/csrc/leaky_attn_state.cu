@@ -15,7 +15,7 @@
 //   one for each 64 columns of the state: registers += MMA result (two in tensor memory);
 //   one warp TMA loads, one the MMAs.
 // Measured: segments of 15 chunks of 16 heads (144 blocks) 56 us with these steps one
-// after another in the main kernel's roles.
+// after another in the main kernel's roles, 35 us so.
 // Every wait is bounded (status 101).
 #include <algorithm>
 

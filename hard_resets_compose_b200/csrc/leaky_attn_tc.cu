@@ -16,26 +16,29 @@
 // itself stays in fp32 registers of its warps, one row of the state a thread.  A
 // rounded weighted k would put 2^-9 into the fp32 state, so b^(C-1-r) k is split
 // into bf16 pieces that as many MMAs add up: two (2^-18) where the state only feeds
-// further bf16 products, three (24 bits) where it is returned.
+// further bf16 products, three (24 bits) where heads of 64 x 64 return it (wider ones
+// have it from leaky_attn_state.cu).
 //
 // Per chunk and head at dq = dv = 128: q, k, v, o are 128 KB, 4800 cycles of the
 // memory that 128 busy SMs share; the MMAs are 5 x 128^3 multiply-adds, 2560 cycles
 // at 4096 a cycle and SM, but an MMA with both operands in shared memory reads 8 KB
 // in 64 cycles, all that shared memory can give (128 bytes a cycle): with the loads
-// and the element-wise writes 512 KB pass through it, 4000 cycles.  So no stage may wait
-// for another (measured: with P, k's pieces, O and S done by 12 warps one after
-// another 7400 cycles a chunk):
+// and the element-wise writes 512 KB pass through it, 4000 cycles.  So no stage may
+// wait for another (measured: with P, k's pieces, O and S done by 12 warps one after
+// another 7400 cycles a chunk, spilling states 14000, as below 5200: B 8, T 4096, H 16
+// in 103 us, 83 us at the copy rate):
 //   scores      P: tensor memory -> decay, bf16 -> tensor memory (A operand of P V).
-//               A thread owns a token.  Two warpgroups where dv = 64 leaves tensor
-//               memory for two P's, in turn.
+//               A thread owns a token.  Two warpgroups where heads of 64 x 64 leave
+//               tensor memory for two P's, in turn.
 //   output      the epilogue to global memory.  A thread owns a token.
-//   state       k's pieces in shared memory (the first in k's place), then the state:
-//               registers += MMA result, its bf16 copy to shared memory.  One warpgroup
-//               for each 64 columns.
+//   state       the weighted k's pieces in shared memory, then the state: registers +=
+//               MMA result, its bf16 copy to shared memory.  One warpgroup for each 64
+//               columns.
 //   one warp    TMA loads, as far ahead as there are tiles.
-//   one warp    issues all MMAs: Q S of a chunk first (the last state is there),
-//               then the state's while the scores are worked on, P V, the next Q K^T.
-// Registers are moved from the other warpgroups to the state's (setmaxnreg).
+//   one warp    issues all MMAs: the state's, P V, the next Q K^T, Q S.
+// Registers are moved from the other warpgroups to the state's (setmaxnreg).  What
+// starts a block up (12 us before its first chunk was out, 8 us now) is mostly code
+// fetched for the first time, so loops stay rolled where that costs nothing.
 // Every wait is bounded (status 101).
 #include <algorithm>
 

@@ -78,7 +78,8 @@ uint64_t lifb_kernel_launches(void);
 /* Device-side status of the current CUDA device: 0 when no kernel of this
  * library has reported a problem, else the code of the first one (101 = a
  * bounded wait for an asynchronous copy expired; the kernel stopped early and
- * its outputs are incomplete).  Synchronous (reads device memory); reset != 0
+ * its outputs are incomplete; 102 = a token id past the embedding table, whose
+ * row is zeros).  Synchronous (reads device memory); reset != 0
  * clears the word afterwards.  Returns -1 if the read itself failed. */
 int lifb_device_status(int reset);
 
