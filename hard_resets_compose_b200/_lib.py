@@ -209,6 +209,32 @@ def load(build_if_missing: bool = True):
         return _lib
 
 
+_fast = None
+
+
+def fast():
+    """The host binding of the sequence-model operators (csrc/host/seq_binding.cpp), over
+    the loaded library: torch autograd nodes without Python in them.  Its functions
+    return None for calls that they leave to the Python functions of the same names."""
+    global _fast
+    if _fast is None:
+        import importlib.util
+        L = load()
+        with _lock:
+            try:
+                path = _build.build_binding()
+            except (RuntimeError, OSError) as e:  # no g++: use the prebuilt binding if present
+                path = _build.binding_path()
+                if not os.path.exists(path):
+                    raise RuntimeError(f"{os.path.basename(path)} is missing and cannot be built: {e}") from e
+            spec = importlib.util.spec_from_file_location("lifb_seq", path)
+            m = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(m)
+            m.bind({name: ctypes.cast(getattr(L, name), c_void_p).value for name in SIGNATURES}, check)
+            _fast = m
+    return _fast
+
+
 def check(status: int, what: str, lib=None) -> None:
     if status != 0:
         L = lib or load(False)

@@ -82,5 +82,46 @@ def build(force: bool = False, verbose: bool = False, defines=(), out: str = Non
     return target
 
 
+# ---- the host binding of the sequence-model operators (csrc/host): torch's C++ autograd
+
+BINDING_SRC = os.path.join(CSRC, "host", "seq_binding.cpp")
+
+
+def binding_path() -> str:
+    """Where the binding is built: one for each torch, whose C++ interface it uses."""
+    import torch
+    return os.path.join(LIBDIR, "lifb_seq-" + torch.__version__.replace("+", "_") + ".so")
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """Compile csrc/host/seq_binding.cpp (g++, about a minute) if it is missing or stale."""
+    import sysconfig
+
+    import torch
+    target = binding_path()
+    deps = [BINDING_SRC] + glob.glob(os.path.join(INCLUDE, "*.h"))
+    if not force and os.path.exists(target) and all(os.path.getmtime(d) <= os.path.getmtime(target) for d in deps):
+        return target
+    gxx = os.environ.get("CXX") or shutil.which("g++")
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    if not gxx:
+        raise RuntimeError("g++ not found: set CXX or put it on PATH")
+    os.makedirs(LIBDIR, exist_ok=True)
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(cuda, "include"), INCLUDE]
+    tmp = f"{target}.{os.getpid()}.tmp"
+    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-DTORCH_EXTENSION_NAME=lifb_seq",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[x for d in inc for x in ("-isystem", d)],
+           BINDING_SRC, "-o", tmp, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+           "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, target)
+    return target
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose=True))
+    print(build_binding(force="--force" in sys.argv, verbose=True))

@@ -61,6 +61,9 @@ class Embedding(torch.autograd.Function):
 def embedding(tokens, weight, scale=1.0):
     """scale * weight[tokens]: tokens of any shape (int32 or int64, negative:
     padding), weight [V, D] (fp32, bf16 or fp16); returns [*tokens.shape, D]."""
+    y = _lib.fast().embedding(tokens, weight, scale)
+    if y is not None:
+        return y
     if weight.dim() != 2:
         raise ValueError(f"embedding: weight must be [V, D], got {tuple(weight.shape)}")
     if weight.dtype not in DTYPES:

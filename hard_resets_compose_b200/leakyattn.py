@@ -119,6 +119,9 @@ def leaky_attention(q, k, v, log_decay, state=None, lengths=None, scale=None, re
     lengths [B] int32: tokens at and past a sequence's length are not read, give
     zeros and leave the state alone.  scale: Dk ** -0.5 by default.  Gradients for
     q, k, v and state."""
+    out = _lib.fast().attention(q, k, v, log_decay, state, lengths, scale, return_state)
+    if out is not None:
+        return out
     what = "leaky_attention"
     H, _, Dk, Dv = _check(what, q, k, v, log_decay, 2, _SEQ_TYPES)
     need_cuda(what, "q k v log_decay state lengths", q, k, v, log_decay, state, lengths)
@@ -150,6 +153,9 @@ def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     head's matrix contiguous; slots [B] int32: the place of each sequence's state
     (None: its own index), at most one sequence to a slot; a place outside the
     cache (-1, say) is empty: zeros out, nothing changed.  Not differentiable."""
+    o = _lib.fast().attention_step(q, k, v, log_decay, state, slots, scale)
+    if o is not None:
+        return o
     what = "leaky_attention_step"
     H, Hk, Dk, Dv = _check(what, q, k, v, log_decay, 1, _STEP_TYPES)
     need_cuda(what, "q k v log_decay state slots", q, k, v, log_decay, state, slots)

@@ -141,6 +141,9 @@ def norm_gate_residual(x, h, gate, post_weight, pre_weight=None, residual_scale=
         raise ValueError(f"norm_gate_residual: unknown act {act!r}")
     if h is None or post_weight is None:
         raise ValueError("norm_gate_residual: needs the block's output h and its post_weight (rms_norm has neither)")
+    out = _lib.fast().norm_gate(x, h, gate, post_weight, pre_weight, residual_scale, eps, ACTS[act])
+    if out is not None:
+        return out
     xo, n = _run("norm_gate_residual", x, h, gate, post_weight, pre_weight, residual_scale, eps, ACTS[act])
     return xo if pre_weight is None else (xo, n)
 
@@ -149,4 +152,7 @@ def rms_norm(x, weight, eps=1e-6):
     """x / sqrt(mean(x^2) + eps) * weight over the last dimension."""
     if weight is None:
         raise ValueError("rms_norm: needs a weight")
+    n = _lib.fast().norm_gate(x, None, None, None, weight, 1.0, eps, 2)
+    if n is not None:
+        return n
     return _run("rms_norm", x, None, None, None, weight, 1.0, eps, 2)[1]
