@@ -12,12 +12,14 @@
 // decays), so they are applied where the values are: to P between its two MMAs, to
 // Q S in the epilogue, to k before the state's MMA, to S in registers.
 //
-// Precision: P and S enter their MMAs rounded to bf16, like the inputs are; S
-// itself stays in fp32 registers of its warps, one row of the state a thread.  A
-// rounded weighted k would put 2^-9 into the fp32 state, so b^(C-1-r) k is split
-// into bf16 pieces that as many MMAs add up: two (2^-18) where the state only feeds
-// further bf16 products, three (24 bits) where heads of 64 x 64 return it (wider ones
-// have it from leaky_attn_state.cu).
+// Precision: P and S enter their MMAs rounded to bf16, like the inputs are; sequences
+// of one chunk or less use two pieces of each (a few tokens' roundings need not average
+// out, up to 1.55 times the output's own; such a call's time is latency).  S itself
+// stays in fp32 registers of its warps, one row of the state a thread.  A rounded
+// weighted k would put 2^-9 into the fp32 state, so b^(C-1-r) k is split into bf16
+// pieces that as many MMAs add up: two (2^-18) where the state only feeds further bf16
+// products, three (24 bits) where heads of 64 x 64 return it (wider ones have it from
+// leaky_attn_state.cu).
 //
 // Per chunk and head at dq = dv = 128: q, k, v, o are 128 KB, 4800 cycles of the
 // memory that 128 busy SMs share; the MMAs are 5 x 128^3 multiply-adds, 2560 cycles
@@ -69,6 +71,9 @@ struct TcLayout {
     static constexpr int nv = DQ == 128 && DV == 128 ? 1 : 2, nm = small ? 2 : 1;  // nm: sets of pieces
     static constexpr uint32_t pieces = 0, k = nm * NP * kQ, q = k + nk * kQ, v = q + nq * kQ, s = v + nv * kV,
                               bytes = s + kS;
+    // S's second piece, where there is one: in q's second tile, which one chunk leaves unused
+    static constexpr uint32_t s_fine = q + kQ;
+    static_assert(nq > 1 && kS <= kQ, "it fits there");
     static_assert(bytes + 1024 + 512 <= 227 * 1024, "tiles fit an SM");
     // columns of tensor memory
     static constexpr uint32_t tmem_cols = 512, o1 = np * 128, o2 = o1 + DV, ds = o2 + DV;
@@ -97,20 +102,24 @@ struct TcBars {
 // packed to bf16 into 64 of the same 128 columns.  Powers of b run from the
 // diagonal outwards (pw: of 16 columns, in their order).  Forward passes walk the columns
 // downwards and pack into the upper half, backward passes the other way round, so
-// that nothing unread is overwritten.
-template <bool REV>
+// that nothing unread is overwritten.  FINE: two bf16 pieces (2^-18) in place of one,
+// each 16 columns of scores becoming 8 of the first and 8 of the second.
+template <bool REV, bool FINE>
 __device__ __forceinline__ void attn_scores(uint32_t lane_cols, int warp, int lane, int n, float b, float b16,
                                             const uint64_t (&pw)[8], float p_scale)
 {
     float d = 0.0f;
     auto col = [&](int s) { return (REV ? s : 7 - s) * 16; };
-    auto out = [&](int s) { return lane_cols + (REV ? 0 : 64) + col(s) / 2; };
+    auto out = [&](int s) { return lane_cols + (FINE ? col(s) : (REV ? 0 : 64) + col(s) / 2); };
     uint32_t x[2][16];
     const int first = 2 * (REV ? warp : 3 - warp);  // before it all columns are on the other side of the diagonal
     tmem_load16(lane_cols + col(first), x[0]);
     {
         const uint32_t zero[8] = {};
-        for (int s = 0; s < first; s++) tmem_store8(out(s), zero);
+        for (int s = 0; s < first; s++) {
+            tmem_store8(out(s), zero);
+            if (FINE) tmem_store8(out(s) + 8, zero);
+        }
     }
     // the two column blocks with the diagonal, then the ones past it, two at a time
 #pragma unroll 1
@@ -120,7 +129,11 @@ __device__ __forceinline__ void attn_scores(uint32_t lane_cols, int warp, int la
             tmem_wait_ld();
             if (half == 0) tmem_load16(lane_cols + col(s + 1), x[1]);
             else if (s < 6) tmem_load16(lane_cols + col(s + 2), x[0]);
-            uint32_t w[8];
+            uint32_t w[8], fine[8];
+            auto pack = [&](int i, uint64_t v) {
+                w[i] = pack2_bf16(v);
+                if (FINE) fine[i] = pack2_bf16(fma2(two(-1.0f, -1.0f), two(bf16_lo(w[i]), bf16_hi(w[i])), v));
+            };
             if (s == first) {
 #pragma unroll
                 for (int t = 0; t < 16; t++) {
@@ -130,23 +143,27 @@ __device__ __forceinline__ void attn_scores(uint32_t lane_cols, int warp, int la
                     x[half][e] = on ? __float_as_uint(__uint_as_float(x[half][e]) * d) : 0u;
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = pack2_bf16(two(x[half][2 * i], x[half][2 * i + 1]));
+                for (int i = 0; i < 8; i++) pack(i, two(x[half][2 * i], x[half][2 * i + 1]));
                 if (half == 1) d *= b;  // of the next block's nearest column
             } else {
                 const uint64_t dd = two(d, d);
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    w[i] = pack2_bf16(mul2(two(x[half][2 * i], x[half][2 * i + 1]), mul2(pw[i], dd)));
+                    pack(i, mul2(two(x[half][2 * i], x[half][2 * i + 1]), mul2(pw[i], dd)));
                 if (REV && n < kTcC) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        if (col(s + half) + 2 * i >= n) w[i] = 0;
-                        else if (col(s + half) + 2 * i + 1 >= n) w[i] &= 0xFFFFu;
+                        const uint32_t on = col(s + half) + 2 * i >= n       ? 0u
+                                            : col(s + half) + 2 * i + 1 >= n ? 0xFFFFu
+                                                                             : ~0u;
+                        w[i] &= on;
+                        if (FINE) fine[i] &= on;
                     }
                 }
                 d *= b16;
             }
             tmem_store8(out(s + half), w);
+            if (FINE) tmem_store8(out(s + half) + 8, fine);
         }
     }
     tmem_wait_st();
@@ -182,6 +199,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     const int s0 = (int)(seg * a.seg_tokens), s1 = (int)min(a.T, seg * a.seg_tokens + a.seg_tokens);
     const int end = min(s1, (int)len);                         // of the tokens that count
     const int chunks = max(0, end - s0 + kTcC - 1) / kTcC;     // with tokens in them
+    const bool fine = len <= kTcC;  // P and S as two pieces: no block has a second chunk
     const int t_first = p.rev ? s0 + (chunks - 1) * kTcC : s0, t_step = p.rev ? -kTcC : kTcC;
 
     if (warp == 0) tmem_alloc(&tmem_slot, L::tmem_cols);
@@ -289,6 +307,13 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                     for (int k = 0; k < DQ / 16; k++)
                         umma_bf16_ss(tmem + L::o2, dq + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4), ds + k * 128, kIdO,
                                      k > 0);
+                    if (fine) {
+                        const uint64_t lo = umma_desc_sw128(sb + L::s_fine, DQ * 128);
+#pragma unroll 1
+                        for (int k = 0; k < DQ / 16; k++)
+                            umma_bf16_ss(tmem + L::o2, dq + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4), lo + k * 128,
+                                         kIdO, true);
+                    }
                     umma_arrive(&bars.q_free[c % L::nq]);
                     umma_arrive(&bars.s_free);
                     umma_arrive(&bars.o_full);
@@ -316,9 +341,15 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 tcgen05_after();
                 const uint32_t pb = p_cols(c) + (p.rev ? 0u : 64u);  // P in bf16
                 if (elect_lane()) {
+                    if (fine) {
+#pragma unroll 1
+                        for (int k = 0; k < kTcC / 8; k++)
+                            umma_bf16_ts(tmem + L::o1, p_cols(c) + k * 8, dv + k / 2 * 128, kIdO, k > 0);
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < kTcC / 16; k++)
-                        umma_bf16_ts(tmem + L::o1, pb + k * 8, dv + k * 128, kIdO, k > 0);
+                        for (int k = 0; k < kTcC / 16; k++)
+                            umma_bf16_ts(tmem + L::o1, pb + k * 8, dv + k * 128, kIdO, k > 0);
+                    }
                     umma_arrive(&bars.v_free[c % L::nv]);
                 }
                 if (c + L::np < chunks) {
@@ -359,8 +390,10 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             if (!wait_warp(&bars.p_full[group], c / L::np)) break;
             tcgen05_after();
             const uint32_t cols = tmem + lanes + group * 128;
-            if (p.rev) attn_scores<true>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
-            else attn_scores<false>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
+            if (fine && p.rev) attn_scores<true, true>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
+            else if (fine) attn_scores<false, true>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
+            else if (p.rev) attn_scores<true, false>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
+            else attn_scores<false, false>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
             tcgen05_before();
             mbar_arrive(&bars.p_ready[group]);
         }
@@ -468,12 +501,25 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
         }
         auto put_state = [&] {  // its bf16 copy, the B operand of Q S
             if (has_row) {
+                const uint32_t row = (at >> 7) * (DQ * 128) + st * 128;
 #pragma unroll
                 for (int j = 0; j < SC; j += 8)
-                    *reinterpret_cast<uint4 *>(base + L::s + (at >> 7) * (DQ * 128) + st * 128 +
-                                               ((j / 8) ^ (st & 7)) * 16) =
+                    *reinterpret_cast<uint4 *>(base + L::s + row + ((j / 8) ^ (st & 7)) * 16) =
                         make_uint4(pack2_bf16(S[j / 2]), pack2_bf16(S[j / 2 + 1]), pack2_bf16(S[j / 2 + 2]),
                                    pack2_bf16(S[j / 2 + 3]));
+                if (fine) {  // what the copy dropped
+#pragma unroll
+                    for (int j = 0; j < SC; j += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t m = pack2_bf16(S[j / 2 + i]);
+                            w[i] = pack2_bf16(fma2(two(-1.0f, -1.0f), two(bf16_lo(m), bf16_hi(m)), S[j / 2 + i]));
+                        }
+                        *reinterpret_cast<uint4 *>(base + L::s_fine + row + ((j / 8) ^ (st & 7)) * 16) =
+                            make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
             }
             fence_proxy_async_shared();
             mbar_arrive(&bars.s_ready);

@@ -271,3 +271,27 @@ def test_refusals(cuda):
         leaky_attention(q.cpu(), k.cpu(), v.cpu(), ld.cpu())
     with pytest.raises(RuntimeError):
         leaky_attention_step(q[:, 0].clone().requires_grad_(), k[:, 0], v[:, 0], ld, st)
+
+
+@pytest.mark.parametrize("T", [1, 3, 11, 64, 127, 128])
+@pytest.mark.parametrize("H,Hk,Dk,Dv", [(1, 1, 64, 64), (4, 1, 128, 32), (2, 2, 128, 128), (2, 1, 40, 72)])
+def test_few_tokens_bf16_are_rounded_once(cuda, T, H, Hk, Dk, Dv):
+    """One chunk or less: intermediate values have two bf16 pieces (2^-8 each, 2^-16 together), powers of the
+    decay at most 2^-17 (128 products of 2^-24), the rest is fp32; 2^-15 of the sum of the terms' sizes covers
+    them.  What is left is the output's own rounding (half an ulp, 2^-8)."""
+    from hard_resets_compose_b200.leakyattn import leaky_attention
+    g = torch.Generator(device=cuda).manual_seed(T * 1000 + H * 100 + Dk)
+    rand = lambda *s: torch.randn(s, generator=g, device=cuda)  # noqa: E731
+    q, k = rand(2, T, H, Dk).bfloat16(), rand(2, T, Hk, Dk).bfloat16()
+    v, do = rand(2, T, Hk, Dv).bfloat16(), rand(2, T, H, Dv).bfloat16()
+    s0, ds = rand(2, H, Dk, Dv), rand(2, H, Dk, Dv)
+    ld = -torch.rand(H, generator=g, device=cuda)
+    lengths = torch.tensor([T, (T + 1) // 2], dtype=torch.int32, device=cuda)
+    p = [t.clone().requires_grad_(True) for t in (q, k, v, s0)]
+    o, s = leaky_attention(p[0], p[1], p[2], ld, p[3], lengths, return_state=True)
+    got = (o, *torch.autograd.grad((o, s), p[:3], (do, ds)))
+    exact = attention(q, k, v, ld, s0, lengths, do=do, dstate=ds)
+    sizes = attention(q.abs(), k.abs(), v.abs(), ld, s0.abs(), lengths, do=do.abs(), dstate=ds.abs())
+    for name, a, e, z in zip(("o", "dq", "dk", "dv"), got, (exact[0], *exact[2:5]), (sizes[0], *sizes[2:5])):
+        over = (a.double() - e).abs() - (U[torch.bfloat16] * e.abs() + 2.0 ** -15 * z)
+        assert (over <= 0).all(), (name, over.max().item())
