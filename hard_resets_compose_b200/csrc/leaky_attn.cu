@@ -511,7 +511,7 @@ Split split_time(int64_t chains, int64_t T, int64_t room)
 int64_t attn_room(int64_t dq, int64_t dv, int dtype)
 {
     if (dtype == LIFB_BF16 && dq % 8 == 0 && dv % 8 == 0) return kAtSms;
-    if (dtype == LIFB_F32 && dq % 4 == 0 && dv % 4 == 0 && dq <= 64 && dv <= 64) return kAtSms;
+    if (dtype == LIFB_F32 && dq % 4 == 0 && dv % 4 == 0) return kAtSms;
     return kAtSms * 2 / std::max<int64_t>(1, (dv + kAtTile - 1) / kAtTile);
 }
 
@@ -544,7 +544,10 @@ AttnWs carve(void *base, const lifb_leaky_attn &p, bool bwd, const Split &sp)
 
 Split split_of(const lifb_leaky_attn &p, bool bwd)
 {
-    return split_time(p.B * p.H * (bwd ? 3 : 1), p.T, attn_room(p.Dk, p.Dv, p.dtype));
+    // chains of one launch: passes, and in fp32 the parts of their widths
+    int64_t k = 1, v = 1;
+    if (p.dtype == LIFB_F32) k = (p.Dk + kT32W - 1) / kT32W, v = (p.Dv + kT32W - 1) / kT32W;
+    return split_time(p.B * p.H * (bwd ? 2 * k + v : v), p.T, attn_room(p.Dk, p.Dv, p.dtype));
 }
 
 int at_check(const char *what, const lifb_leaky_attn *p)

@@ -41,12 +41,17 @@ struct AttnPass {
     int shift, rev, o_f32;
     float *seg;                   // [B*H][nseg + 1][dq][dv]: each time segment's starting state (0's unused);
                                   // the last is what the final state is joined from
+    // of a pass over a part of the widths (leaky_attn_tc32.cu): elements between two heads' states,
+    // a segment state's row, and whether o is added to
+    int64_t mat, seg_row;
+    int add;
 };
 
 constexpr int kAttnMaxPasses = 3;
 
-struct AttnArgs {
-    AttnPass p[kAttnMaxPasses];
+template <int N>
+struct AttnArgsOf {
+    AttnPass p[N];
     const float *log_decay;       // [H]
     const int32_t *lengths;       // [B], or NULL: every sequence has T tokens
     int64_t B, T, H;
@@ -55,6 +60,7 @@ struct AttnArgs {
     int nseg;                     // time segments, each with a multiple of kAttnSegGrain tokens
     int64_t seg_tokens;
 };
+using AttnArgs = AttnArgsOf<kAttnMaxPasses>;
 
 constexpr int kAttnSegGrain = 128;
 constexpr int kAttnMaxDim = 128;  // of q, k and of v
@@ -101,7 +107,8 @@ bool attn_operand_map(CUtensorMap *m, const void *base, const int64_t (&st)[3], 
                       int64_t B);
 // Whether attn_tc returns this pass's state itself.
 bool attn_tc_returns_state(int dq, int dv);
-// leaky_attn_tc32.cu: the same for fp32 operands in 16-byte aligned vectors, widths up to 64.
+// leaky_attn_tc32.cu: the same for fp32 operands in 16-byte aligned vectors.
+constexpr int kT32W = 64;  // widths of its tiles; wider heads are several
 bool attn_tc32_applies(const AttnArgs &a, int passes, int dtype);
 bool attn_tc32(const AttnArgs &a, int passes, bool state_only, cudaStream_t s);
 

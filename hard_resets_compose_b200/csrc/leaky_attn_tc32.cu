@@ -1,5 +1,14 @@
-// Leaky attention in fp32 on the 5th-generation tensor cores, for heads up to 64
-// wide.  leaky_attn.h has the recurrence, leaky_attn_tc.cu the chunked form in bf16.
+// Leaky attention in fp32 on the 5th-generation tensor cores.  leaky_attn.h has the
+// recurrence, leaky_attn_tc.cu the chunked form in bf16.
+//
+// A block does 64 columns of q and k and 64 of v.  Everything is linear in the products
+// of a column of k with one of v, so wider heads are two or four such parts, each with
+// its own part of the state: the parts over v's columns run together, and those over
+// the second half of q's and k's columns in a launch of their own that adds to o (in a
+// fixed order).  128 x 128 costs a third more multiplications than whole tiles would
+// (Q K^T twice), which would not fit an SM as three pieces.  Measured against the fp32
+// pipe: B 8, T 1024, H 8, 128 x 128: forward 559 -> 136 us, backward 1308 -> 379 us; B 5,
+// T 1336, 8 heads on one k/v head, 32 x 128: 250 -> 73, 688 -> 231 us.
 //
 // Each fp32 operand is the sum of three bf16 pieces, x = x0 + x1 + x2 (8 + 8 + 8 bits),
 // and a product of two operands the six products of pieces down to 2^-16:
@@ -36,7 +45,6 @@ namespace lifb {
 namespace {
 
 constexpr int kT32C = 128, kT32Threads = 768;
-constexpr int kT32W = 64;                        // widths, padded
 constexpr uint32_t kT32Tile = kT32C * 128;       // one piece of 128 rows
 constexpr uint32_t kT32S = kT32W * 128;          // one piece of the state
 constexpr uint32_t kT32Q = 0, kT32K = 3 * kT32Tile, kT32Kw = 6 * kT32Tile, kT32V = 9 * kT32Tile,
@@ -54,6 +62,9 @@ struct T32Bars {
     uint64_t q_ready, k_ready, kw_ready, v_ready, s_ready, p_ready, o_free, ds_free;  // 128 threads each
     uint64_t p_full, o2_full, ds_full, o1_full, done;                                // MMAs
 };
+
+// The parts of one launch.
+using T32Args = AttnArgsOf<4 * kAttnMaxPasses>;
 
 // The piece pairs of a product, small ones first: a nibble each.
 constexpr uint32_t kPieceA = 0x001102, kPieceB = 0x010120;
@@ -116,7 +127,7 @@ struct TileRegs {
 }  // namespace
 
 template <bool STATE_ONLY>
-__global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_constant__ AttnArgs a, int *status)
+__global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_constant__ T32Args a, int *status)
 {
     extern __shared__ unsigned char t32_raw[];
     unsigned char *base = (unsigned char *)(((uintptr_t)t32_raw + 1023) & ~(uintptr_t)1023);
@@ -311,6 +322,12 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
 #pragma unroll 1
                 for (int g = 0; g < kT32W; g += 16) {
                     uint32_t x[16], y[16];
+                    float4 had[4];
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        had[e / 4] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (p.add && st < n && g + e < p.dv) had[e / 4] = *reinterpret_cast<const float4 *>(dst + g + e);
+                    }
                     tmem_load16(tmem + lanes + kT32O1 + g, x);
                     tmem_load16(tmem + lanes + kT32O2 + g, y);
                     tmem_wait_ld();
@@ -325,8 +342,10 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
 #pragma unroll
                             for (int q = 0; q < 4; q++)
                                 f[q] = st < n ? fmaf(w, __uint_as_float(y[e + q]), __uint_as_float(x[e + q])) : 0.0f;
+                            const float4 z = had[e / 4];
                             if (g + e < p.dv)
-                                *reinterpret_cast<float4 *>(dst + g + e) = make_float4(f[0], f[1], f[2], f[3]);
+                                *reinterpret_cast<float4 *>(dst + g + e) =
+                                    make_float4(z.x + f[0], z.y + f[1], z.z + f[2], z.w + f[3]);
                         }
                     }
                     __syncwarp();
@@ -345,7 +364,7 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kT32Regs[kState]));
         const bool has_row = st < kT32W;  // uniform over a warp
         uint64_t S[kT32W / 2];            // pairs of columns of this thread's row
-        const int64_t mat = (int64_t)p.dq * p.dv;
+        const int64_t mat = p.mat;
         {
             const float *s_in = nullptr;
             int64_t row = p.s_row, col = p.s_col;
@@ -354,7 +373,7 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
                     if (p.s_in) s_in = p.s_in + bh * mat;
                 } else {
                     s_in = p.seg + (bh * (a.nseg + 1) + u) * mat;
-                    row = p.dv;
+                    row = p.seg_row;
                     col = 1;
                 }
             }
@@ -409,7 +428,7 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
             mbar_arrive(&bars.ds_free);
         }
         float *s_out = nullptr;
-        int64_t row = p.dv, col = 1;
+        int64_t row = p.seg_row, col = 1;
         if (STATE_ONLY) {
             s_out = p.seg + (bh * (a.nseg + 1) + u + 1) * mat;
         } else if (u == a.nseg - 1 && p.s_out) {
@@ -493,20 +512,56 @@ bool attn_tc32_applies(const AttnArgs &a, int passes, int dtype)
     };
     for (int i = 0; i < passes; i++) {
         const AttnPass &p = a.p[i];
-        if (p.dq > kT32W || p.dv > kT32W || p.dq % 4 || p.dv % 4 || !aligned16(p.o) || !four(p.q, p.qs) ||
+        if (p.dq > kAttnMaxDim || p.dv > kAttnMaxDim || p.dq % 4 || p.dv % 4 || !aligned16(p.o) || !four(p.q, p.qs) ||
             !four(p.k, p.ks) || !four(p.v, p.vs))
             return false;
     }
     return true;
 }
 
+namespace {
+
+// The part of pass p with columns from 64 qi of q and k and 64 vi of v and o.
+AttnPass part_of(const AttnPass &p, int qi, int vi)
+{
+    AttnPass x = p;
+    const int q0 = qi * kT32W, v0 = vi * kT32W;
+    x.q = (const float *)p.q + q0;
+    x.k = (const float *)p.k + q0;
+    x.v = (const float *)p.v + v0;
+    x.o = (float *)p.o + v0;
+    x.dq = std::min(p.dq - q0, kT32W);
+    x.dv = std::min(p.dv - v0, kT32W);
+    x.mat = (int64_t)p.dq * p.dv;
+    x.seg_row = p.dv;
+    if (p.s_in) x.s_in = p.s_in + q0 * p.s_row + v0 * p.s_col;
+    if (p.s_out) x.s_out = p.s_out + q0 * p.s_row + v0 * p.s_col;
+    if (p.seg) x.seg = p.seg + q0 * p.dv + v0;
+    x.add = qi > 0;
+    return x;
+}
+
+}  // namespace
+
 bool attn_tc32(const AttnArgs &a, int passes, bool state_only, cudaStream_t s)
 {
     auto kern = state_only ? k_attn_tc32<true> : k_attn_tc32<false>;
     const size_t smem = kT32Bytes + 1024;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
-    count_launches(1);
-    kern<<<(unsigned)(a.B * a.H * a.nseg * passes), kT32Threads, smem, s>>>(a, device_status_ptr());
+    T32Args b = {};
+    b.log_decay = a.log_decay, b.lengths = a.lengths;
+    b.B = a.B, b.T = a.T, b.H = a.H;
+    b.nseg = a.nseg, b.seg_tokens = a.seg_tokens;
+    for (int qi = 0; qi * kT32W < kAttnMaxDim; qi++) {
+        for (int i = 0; i < passes; i++)
+            if (qi * kT32W < a.p[i].dq)
+                for (int vi = 0; vi * kT32W < a.p[i].dv; vi++) b.p[b.passes++] = part_of(a.p[i], qi, vi);
+        // states alone do not add up: all parts in one launch
+        if (b.passes == 0 || (state_only && (qi + 1) * kT32W < kAttnMaxDim)) continue;
+        count_launches(1);
+        kern<<<(unsigned)(a.B * a.H * a.nseg * b.passes), kT32Threads, smem, s>>>(b, device_status_ptr());
+        b.passes = 0;
+    }
     return true;
 }
 
