@@ -60,8 +60,7 @@ __device__ __forceinline__ void attn_load(float *dst, int ld, const T *src, int6
 // state lives in shared memory in fp32.  Bound by the fp32 pipe: a chunk is 32 (dq (2 64
 // + 16) + 64 16) multiply-adds a block at 128 a cycle (B 64, T 1024, H 4, 64 x 64 forward:
 // 220 us of them, 465 us measured).  What comes here is what the tensor-core kernels do
-// not take: fp32 heads wider than 64, and widths, strides or addresses that are not
-// multiples of 16 bytes.
+// not take: widths, strides or addresses that are not multiples of 16 bytes.
 template <typename T, bool W4>
 __global__ void __launch_bounds__(kAtThreads) k_attn_simt(const __grid_constant__ AttnArgs a, int state_only)
 {

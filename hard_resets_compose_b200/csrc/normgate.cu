@@ -26,6 +26,7 @@
 // the memory waiting a quarter of the time; fp32 [65536, 256] with a row's gate 50 us
 // (42) and 75 us (62).
 #include <algorithm>
+#include <initializer_list>
 
 #include "lifb_common.cuh"
 #include "lifb_internal.h"
@@ -499,21 +500,33 @@ struct NormShape {
 // A row takes as few threads as hold it at 16 (fp32 forward: 8) elements each,
 // in one warp if it can: a row costs each thread some 150 instructions besides its
 // elements (bf16 rows of 2048: forward 150 us with 8 elements a thread, 109 us with 16).
-// Rows that are read element by element take more threads instead.
-bool norm_shape(int64_t D, bool wide, int elem, bool bwd, NormShape &s)
+// Rows that are read element by element take more threads instead, and so do long rows
+// of 8-byte fp32 vectors, whose forward would spill at 16 (8000 rows of 3002: 165 us in
+// 256 threads, 85 in 512; 16-byte vectors: 66 against 82).  Narrower vectors where 16
+// bytes do not fit: bf16 [30000, 1028] with an elementwise gate, by single elements 220
+// us forward and 474 backward, by 8 bytes 123 and 229, by 4 ([30000, 1030]) 184 and 290.
+bool norm_shape(int64_t D, int vec, int elem, bool bwd, NormShape &s)
 {
-    s.vec = wide ? 16 / elem : 1;
+    s.vec = vec;
+    const int widest = 16 / elem;
+    const bool wide = vec > 1;
     const int64_t vecs = (D + s.vec - 1) / s.vec;
     auto spread = [&](int tpr, int elems) {
         s.tpr = tpr;
-        s.nit = wide ? 1 : 4;  // one element a vector: 4 or 16 of them
-        while (s.nit * s.vec < elems && (int64_t)s.tpr * s.nit < vecs) s.nit *= wide ? 2 : 4;
+        // 16-byte vectors: any number of them; single elements: 4, 8 or 16; between: 8 or 16 elements
+        s.nit = vec == widest ? 1 : wide ? 8 / vec : 4;
+        while (s.nit * s.vec < elems && (int64_t)s.tpr * s.nit < vecs) s.nit *= 2;
         return (int64_t)s.tpr * s.nit >= vecs;
     };
     s.threads = kNgThreads;
     for (int tpr = 8; tpr <= kNgThreads; tpr *= 2)
-        if (spread(tpr, tpr < 32 ? s.vec : !wide ? (tpr == 32 ? kNgMaxElems : 4) : elem == 2 || bwd ? kNgMaxElems : 8))
+        if (spread(tpr, tpr < 32 ? (vec == widest || !wide ? s.vec : 8) : !wide ? (tpr == 32 ? kNgMaxElems : tpr == kNgThreads ? 8 : 4) : elem == 2 || bwd ? kNgMaxElems : 8))
             return true;
+    if (!wide || (elem == 4 && vec == 2)) {
+        s.threads = kNgMaxThreads;
+        if (spread(kNgMaxThreads, 8)) return true;
+        s.threads = kNgThreads;
+    }
     if (spread(kNgThreads, kNgMaxElems)) return true;
     s.threads = kNgMaxThreads;
     return spread(kNgMaxThreads, kNgMaxElems);
@@ -546,8 +559,9 @@ template <typename T, int VEC, int NIT>
 void norm_gate(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
 {
     if (sh.threads == kNgMaxThreads) {
-        if constexpr (VEC * NIT == kNgMaxElems) norm_launch<T, VEC, NIT, kNgMaxThreads, -1>(bwd, a, sh, s);
-    } else if constexpr (VEC == 1) {
+        if constexpr (VEC * NIT == kNgMaxElems || (VEC * NIT == 8 && (VEC == 1 || (VEC == 2 && sizeof(T) == 4))))
+            norm_launch<T, VEC, NIT, kNgMaxThreads, -1>(bwd, a, sh, s);
+    } else if constexpr (VEC * sizeof(T) != 16) {
         norm_launch<T, VEC, NIT, kNgThreads, -1>(bwd, a, sh, s);
     } else if (!a.gate) {
         norm_launch<T, VEC, NIT, kNgThreads, 0>(bwd, a, sh, s);
@@ -568,7 +582,16 @@ void norm_run(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
     constexpr int VEC = 16 / sizeof(T);
     if (sh.vec == 1) {
         if (sh.nit == 4) norm_gate<T, 1, 4>(bwd, a, sh, s);
+        else if (sh.nit == 8) norm_gate<T, 1, 8>(bwd, a, sh, s);
         else norm_gate<T, 1, 16>(bwd, a, sh, s);
+    } else if (sh.vec == 2) {
+        if (sh.nit == 4) norm_gate<T, 2, 4>(bwd, a, sh, s);
+        else norm_gate<T, 2, 8>(bwd, a, sh, s);
+    } else if (sh.vec < VEC) {
+        if constexpr (VEC == 8) {
+            if (sh.nit == 2) norm_gate<T, 4, 2>(bwd, a, sh, s);
+            else norm_gate<T, 4, 4>(bwd, a, sh, s);
+        }
     } else if (sh.nit == 1) {
         norm_gate<T, VEC, 1>(bwd, a, sh, s);
     } else if (sh.nit == 2) {
@@ -576,6 +599,19 @@ void norm_run(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
     } else if constexpr (VEC == 4) {
         norm_gate<T, VEC, 4>(bwd, a, sh, s);
     }
+}
+
+// Elements of a vector that D, the strides and the addresses (null: absent) allow.
+int norm_vec(int elem, int64_t D, std::initializer_list<int64_t> strides, std::initializer_list<const void *> ptrs)
+{
+    int vec = 16 / elem;
+    for (; vec > 1; vec /= 2) {
+        bool ok = D % vec == 0;
+        for (int64_t st : strides) ok = ok && st % vec == 0;
+        for (const void *p : ptrs) ok = ok && (uintptr_t)p % (vec * elem) == 0;
+        if (ok) break;
+    }
+    return vec;
 }
 
 int norm_fail(int status, const char *what, const char *why)
@@ -631,13 +667,11 @@ extern "C" int lifb_norm_gate_fwd(const lifb_norm_gate *p, void *xo, void *n, vo
     a.n = n;
     if (!a.x || (a.h && (!a.post || !xo)) || (n && !a.pre) || (p->gate_cols && !p->gate) || (!a.h && !n))
         return norm_fail(LIFB_ERR_INVALID_ARGUMENT, what, "null pointer");
-    const int64_t vec = 16 / dtype_bytes(p->dtype);
-    bool wide = a.D % vec == 0 && a.sx % vec == 0 && aligned16(a.x) && aligned16(xo) && aligned16(n);
-    if (a.h) wide = wide && a.sh % vec == 0 && aligned16(a.h) && aligned16(a.post);
-    if (n) wide = wide && aligned16(a.pre);
-    if (a.gate && !a.gate_row) wide = wide && a.sg % vec == 0 && aligned16(a.gate);
+    const bool gate = a.gate && !a.gate_row;
+    const int elem = (int)dtype_bytes(p->dtype);
+    const int vec = norm_vec(elem, a.D, {a.sx, a.h ? a.sh : 0, gate ? a.sg : 0}, {a.x, xo, n, a.h, gate ? a.gate : nullptr});
     NormShape sh;
-    if (!norm_shape(a.D, wide, (int)dtype_bytes(p->dtype), false, sh))
+    if (!norm_shape(a.D, vec, elem, false, sh))
         return norm_fail(LIFB_ERR_UNSUPPORTED, what, "rows longer than 8192 elements");
     LIFB_BY_DTYPE(p->dtype, T, norm_run<T>(false, a, sh, (cudaStream_t)stream));
     if (cudaGetLastError() != cudaSuccess) return norm_fail(LIFB_ERR_CUDA, what, "launch failed");
@@ -649,10 +683,10 @@ extern "C" size_t lifb_norm_gate_bwd_workspace_bytes(int64_t R, int64_t D, int d
 {
     using namespace lifb;
     if (R <= 0 || D <= 0 || !dtype_bytes(dtype)) return 0;
-    size_t most = 0;  // of the vector and the element form
-    for (int wide = 0; wide < 2; wide++) {
+    size_t most = 0;  // of any vectors
+    for (int vec = 16 / (int)dtype_bytes(dtype); vec > 0; vec /= 2) {
         NormShape sh;
-        if (norm_shape(D, wide != 0, (int)dtype_bytes(dtype), true, sh))
+        if (norm_shape(D, vec, (int)dtype_bytes(dtype), true, sh))
             most = std::max(most, (size_t)norm_blocks(sh, R, true) * 2 * D * 4);
     }
     return most;
@@ -689,14 +723,12 @@ extern "C" int lifb_norm_gate_bwd(const lifb_norm_gate *p, const void *dxo, int6
     if (weights && (!workspace || workspace_bytes < lifb_norm_gate_bwd_workspace_bytes(a.R, a.D, p->dtype)))
         return norm_fail(LIFB_ERR_WORKSPACE, what, "workspace missing or too small");
     a.part = weights ? (float *)workspace : nullptr;
-    const int64_t vec = 16 / dtype_bytes(p->dtype);
-    bool wide = a.D % vec == 0 && a.sx % vec == 0 && aligned16(a.x) && aligned16(dx) && aligned16(dh);
-    if (dxo) wide = wide && dxo_stride % vec == 0 && aligned16(dxo);
-    if (dn) wide = wide && dn_stride % vec == 0 && aligned16(dn) && aligned16(a.pre);
-    if (a.h) wide = wide && a.sh % vec == 0 && aligned16(a.h) && aligned16(a.post);
-    if (a.gate && !a.gate_row) wide = wide && a.sg % vec == 0 && aligned16(a.gate) && aligned16(dgate);
+    const bool gate = a.gate && !a.gate_row;
+    const int elem = (int)dtype_bytes(p->dtype);
+    const int vec = norm_vec(elem, a.D, {a.sx, dxo ? a.sdx : 0, dn ? a.sdn : 0, a.h ? a.sh : 0, gate ? a.sg : 0},
+                             {a.x, dx, dh, dxo, dn, a.h, gate ? a.gate : nullptr, gate ? dgate : nullptr});
     NormShape sh;
-    if (!norm_shape(a.D, wide, (int)dtype_bytes(p->dtype), true, sh))
+    if (!norm_shape(a.D, vec, elem, true, sh))
         return norm_fail(LIFB_ERR_UNSUPPORTED, what, "rows longer than 8192 elements");
     LIFB_BY_DTYPE(p->dtype, T, norm_run<T>(true, a, sh, s));
     if (weights) {

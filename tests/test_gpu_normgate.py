@@ -187,3 +187,28 @@ def test_refusals(cuda):
             bad()
     with pytest.raises(RuntimeError):
         rms_norm(x.cpu(), pre.cpu())
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("R,D,gate", ((9, 12, "full"), (40, 30, "row"), (33, 260, "full"), (21, 1030, "row"),
+                                      (300, 2052, "full"), (200, 5140, "row"), (150, 5142, "full"), (3, 8186, "none")))
+def test_rows_of_narrower_vectors(cuda, dtype, R, D, gate):
+    """Widths that 8 or 4 bytes divide and 16 do not, and addresses that only those fit."""
+    test_against_fp64(cuda, dtype, R, D, gate, "silu")
+
+
+def test_vectors_follow_the_addresses(cuda):
+    """The same rows at every offset: the same values, whatever vectors they are read in (sums in another order)."""
+    from hard_resets_compose_b200.normgate import norm_gate_residual
+    for dtype in (torch.float32, torch.bfloat16):
+        R, D = 50, 512
+        ts = make(R, D, dtype, "full", torch.float32)[:5]
+        rx, rn, _ = reference(ts, 1.0, "silu", 1e-6, *make(R, D, dtype, "full", torch.float32)[5:])
+        for at in (0, 1, 2, 4, 6, 8):
+            def moved(t):
+                wide = torch.full((R, D + 16), float("nan"), device=cuda, dtype=dtype)
+                wide[:, at:at + D] = t
+                return wide[:, at:at + D]
+            with torch.no_grad():
+                x, n = norm_gate_residual(moved(ts[0]), moved(ts[1]), moved(ts[2]), ts[3], ts[4])
+            assert rel(x, rx) <= tol(x) and rel(n, rn) <= tol(n)
