@@ -12,7 +12,7 @@
 // decays), so they are applied where the values are: to P between its two MMAs, to
 // Q S in the epilogue, to k before the state's MMA, to S in registers.
 //
-// Precision: P and S enter their MMAs rounded to bf16, like the inputs are; sequences
+// Precision: P and S enter their MMAs rounded to bf16, like the inputs are; calls
 // of one chunk or less use two pieces of each (a few tokens' roundings need not average
 // out, up to 1.55 times the output's own; such a call's time is latency).  S itself
 // stays in fp32 registers of its warps, one row of the state a thread.  A rounded
@@ -177,7 +177,8 @@ __device__ __forceinline__ void store_32_bytes(void *p, const uint32_t (&m)[8])
                  : "memory");
 }
 
-template <int DQ, int DV, int NP>
+// FINE: P and S as two pieces each; T is at most one chunk.
+template <int DQ, int DV, int NP, bool FINE>
 __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     k_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps maps, int *status)
 {
@@ -199,7 +200,6 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
     const int s0 = (int)(seg * a.seg_tokens), s1 = (int)min(a.T, seg * a.seg_tokens + a.seg_tokens);
     const int end = min(s1, (int)len);                         // of the tokens that count
     const int chunks = max(0, end - s0 + kTcC - 1) / kTcC;     // with tokens in them
-    const bool fine = len <= kTcC;  // P and S as two pieces: no block has a second chunk
     const int t_first = p.rev ? s0 + (chunks - 1) * kTcC : s0, t_step = p.rev ? -kTcC : kTcC;
 
     if (warp == 0) tmem_alloc(&tmem_slot, L::tmem_cols);
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                     for (int k = 0; k < DQ / 16; k++)
                         umma_bf16_ss(tmem + L::o2, dq + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4), ds + k * 128, kIdO,
                                      k > 0);
-                    if (fine) {
+                    if constexpr (FINE) {
                         const uint64_t lo = umma_desc_sw128(sb + L::s_fine, DQ * 128);
 #pragma unroll 1
                         for (int k = 0; k < DQ / 16; k++)
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                 tcgen05_after();
                 const uint32_t pb = p_cols(c) + (p.rev ? 0u : 64u);  // P in bf16
                 if (elect_lane()) {
-                    if (fine) {
+                    if constexpr (FINE) {
 #pragma unroll 1
                         for (int k = 0; k < kTcC / 8; k++)
                             umma_bf16_ts(tmem + L::o1, p_cols(c) + k * 8, dv + k / 2 * 128, kIdO, k > 0);
@@ -390,10 +390,8 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             if (!wait_warp(&bars.p_full[group], c / L::np)) break;
             tcgen05_after();
             const uint32_t cols = tmem + lanes + group * 128;
-            if (fine && p.rev) attn_scores<true, true>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
-            else if (fine) attn_scores<false, true>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
-            else if (p.rev) attn_scores<true, false>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
-            else attn_scores<false, false>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
+            if (p.rev) attn_scores<true, FINE>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
+            else attn_scores<false, FINE>(cols, warp & 3, lane, n, b1, b16, pw, p.p_scale);
             tcgen05_before();
             mbar_arrive(&bars.p_ready[group]);
         }
@@ -507,7 +505,7 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                     *reinterpret_cast<uint4 *>(base + L::s + row + ((j / 8) ^ (st & 7)) * 16) =
                         make_uint4(pack2_bf16(S[j / 2]), pack2_bf16(S[j / 2 + 1]), pack2_bf16(S[j / 2 + 2]),
                                    pack2_bf16(S[j / 2 + 3]));
-                if (fine) {  // what the copy dropped
+                if constexpr (FINE) {  // what the copy dropped
 #pragma unroll
                     for (int j = 0; j < SC; j += 8) {
                         uint32_t w[4];
@@ -647,16 +645,24 @@ namespace {
 
 int width_class(int d) { return d <= 64 ? 64 : 128; }
 
-template <int DQ, int DV, int NP>
-bool launch_tc(const AttnArgs &a, const AttnMaps &m, int passes, cudaStream_t s)
+template <int DQ, int DV, int NP, bool FINE>
+bool launch_kernel(const AttnArgs &a, const AttnMaps &m, int passes, cudaStream_t s)
 {
     using L = TcLayout<DQ, DV, NP>;
     const size_t smem = L::bytes + 1024;
-    auto kern = k_attn_tc<DQ, DV, NP>;
+    auto kern = k_attn_tc<DQ, DV, NP, FINE>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
     count_launches(1);
     kern<<<(unsigned)(a.B * a.H * a.nseg * passes), L::threads, smem, s>>>(a, m, device_status_ptr());
     return true;
+}
+
+// (As a condition in the kernel, the second pieces took 3 to 10% of the longer calls' time.)
+template <int DQ, int DV, int NP>
+bool launch_tc(const AttnArgs &a, const AttnMaps &m, int passes, cudaStream_t s)
+{
+    return a.T <= kTcC ? launch_kernel<DQ, DV, NP, true>(a, m, passes, s)
+                       : launch_kernel<DQ, DV, NP, false>(a, m, passes, s);
 }
 
 }  // namespace
