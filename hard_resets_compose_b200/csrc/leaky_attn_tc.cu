@@ -12,9 +12,17 @@
 // decays), so they are applied where the values are: to P between its two MMAs, to
 // Q S in the epilogue, to k before the state's MMA, to S in registers.
 //
-// Precision: P and S enter their MMAs rounded to bf16, like the inputs are; calls
-// of one chunk or less use two pieces of each (a few tokens' roundings need not average
-// out, up to 1.55 times the output's own; such a call's time is latency).  S itself
+// Precision: P and S enter their MMAs rounded to bf16, like the inputs are: 2^-9 each, as
+// much as the output's own rounding, so that outputs are sqrt(2) times as far off as
+// values rounded once (2.4e-3 against 1.7e-3, relative).  Calls of one chunk, and of
+// 8192 rows (tokens of heads) or less, use two pieces of each, and their outputs are
+// rounded once: roundings of few rows need not average out (one of 130 to 400 tokens and
+// one to four heads in a hundred was 1.5 to 1.56 times as far off as one rounding; from
+// 8192 rows on none was over 1.44), and such a call's time is mostly latency (B 1, T 1024, H 8,
+// 128 x 128: forward 35 -> 37 us, backward 43 -> 45; four of T 256: 12.3 -> 14.4, 12.4 ->
+// 16.5).  Two pieces in every call would cost more than half of
+// the large ones again (B 8, T 4096, H 16, 128 x 128: 104 -> 164 us and 299 -> 494; 64 x 64 at B 16:
+// 132 -> 156 and 443 -> 640).  S itself
 // stays in fp32 registers of its warps, one row of the state a thread.  A rounded
 // weighted k would put 2^-9 into the fp32 state, so b^(C-1-r) k is split into bf16
 // pieces that as many MMAs add up: two (2^-18) where the state only feeds further bf16
@@ -61,19 +69,18 @@ struct AttnMaps {
 // Shared memory of a block: tiles of 64-column blocks.  What an MMA with fewer
 // than 128 rows of A reads past its 64 columns (dq = 64) must lie inside: a piece is
 // never the last tile.
-template <int DQ, int DV, int NP>
+template <int DQ, int DV, int NP, bool FINE>
 struct TcLayout {
     static constexpr uint32_t kQ = DQ / 64 * kTcBlock, kV = DV / 64 * kTcBlock, kS = DV / 64 * DQ * 128;
     static constexpr bool small = DQ == 64 && DV == 64;
     static constexpr int np = small ? 2 : 1;  // P's in flight, in tensor memory
     // tiles in flight: of q one more than P's, so that the next Q K^T need not wait for Q S
-    static constexpr int nq = np + 1, nk = np;
+    // (where S's second piece leaves room for it)
+    static constexpr int nq = FINE && DQ == 128 && DV == 128 ? np : np + 1, nk = np;
     static constexpr int nv = DQ == 128 && DV == 128 ? 1 : 2, nm = small ? 2 : 1;  // nm: sets of pieces
     static constexpr uint32_t pieces = 0, k = nm * NP * kQ, q = k + nk * kQ, v = q + nq * kQ, s = v + nv * kV,
-                              bytes = s + kS;
-    // S's second piece, where there is one: in q's second tile, which one chunk leaves unused
-    static constexpr uint32_t s_fine = q + kQ;
-    static_assert(nq > 1 && kS <= kQ, "it fits there");
+                              s_fine = s + kS,  // S's second piece
+                              bytes = s_fine + (FINE ? kS : 0);
     static_assert(bytes + 1024 + 512 <= 227 * 1024, "tiles fit an SM");
     // columns of tensor memory
     static constexpr uint32_t tmem_cols = 512, o1 = np * 128, o2 = o1 + DV, ds = o2 + DV;
@@ -177,12 +184,12 @@ __device__ __forceinline__ void store_32_bytes(void *p, const uint32_t (&m)[8])
                  : "memory");
 }
 
-// FINE: P and S as two pieces each; T is at most one chunk.
+// FINE: P and S as two pieces each.
 template <int DQ, int DV, int NP, bool FINE>
-__global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
+__global__ void __launch_bounds__((TcLayout<DQ, DV, NP, FINE>::threads), 1)
     k_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps maps, int *status)
 {
-    using L = TcLayout<DQ, DV, NP>;
+    using L = TcLayout<DQ, DV, NP, FINE>;
     extern __shared__ unsigned char tc_raw[];
     unsigned char *base = (unsigned char *)(((uintptr_t)tc_raw + 1023) & ~(uintptr_t)1023);
     __shared__ TcBars bars;
@@ -264,10 +271,16 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
             for (int c = 0; c < chunks; c++) {
                 if (!load(&maps.k[pi], L::k, L::kQ, L::nk, c, hk, bars.k_full, bars.k_free)) break;
                 nk++;
-                if (!load(&maps.q[pi], L::q, L::kQ, L::nq, c, hq, bars.q_full, bars.q_free)) break;
-                nq++;
+                if (L::nq > L::np) {
+                    if (!load(&maps.q[pi], L::q, L::kQ, L::nq, c, hq, bars.q_full, bars.q_free)) break;
+                    nq++;
+                }
                 if (!load(&maps.v[pi], L::v, L::kV, L::nv, c, hv, bars.v_full, bars.v_free)) break;
                 nv++;
+                if (L::nq == L::np) {  // its tile is the last to be free
+                    if (!load(&maps.q[pi], L::q, L::kQ, L::nq, c, hq, bars.q_full, bars.q_free)) break;
+                    nq++;
+                }
             }
             // no copy is left in flight, whatever happened
             for (int c = max(0, nk - L::nk); c < nk; c++) mbar_wait(&bars.k_full[c % L::nk], (c / L::nk) & 1);
@@ -352,12 +365,13 @@ __global__ void __launch_bounds__((TcLayout<DQ, DV, NP>::threads), 1)
                     }
                     umma_arrive(&bars.v_free[c % L::nv]);
                 }
+                if (L::nq == L::np && !carried(c)) return false;  // the next q comes into this one's tile
                 if (c + L::np < chunks) {
                     // P V is done: P's columns are free
                     if (!wait_warp(&bars.v_free[c % L::nv], c / L::nv)) return false;
                     if (!scores(c + L::np)) return false;
                 }
-                return carried(c);
+                return L::nq == L::np || carried(c);
             };
             bool ok = true;
             for (int c = 0; ok && c < L::np && c < chunks; c++) ok = scores(c);
@@ -643,12 +657,15 @@ bool attn_operand_map(CUtensorMap *m, const void *base, const int64_t (&st)[3], 
 
 namespace {
 
+// Rows (tokens of heads) of a call up to which P and S have two pieces, whatever its length.
+constexpr int64_t kTcFineRows = 8192;
+
 int width_class(int d) { return d <= 64 ? 64 : 128; }
 
 template <int DQ, int DV, int NP, bool FINE>
 bool launch_kernel(const AttnArgs &a, const AttnMaps &m, int passes, cudaStream_t s)
 {
-    using L = TcLayout<DQ, DV, NP>;
+    using L = TcLayout<DQ, DV, NP, FINE>;
     const size_t smem = L::bytes + 1024;
     auto kern = k_attn_tc<DQ, DV, NP, FINE>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
@@ -661,8 +678,9 @@ bool launch_kernel(const AttnArgs &a, const AttnMaps &m, int passes, cudaStream_
 template <int DQ, int DV, int NP>
 bool launch_tc(const AttnArgs &a, const AttnMaps &m, int passes, cudaStream_t s)
 {
-    return a.T <= kTcC ? launch_kernel<DQ, DV, NP, true>(a, m, passes, s)
-                       : launch_kernel<DQ, DV, NP, false>(a, m, passes, s);
+    const bool fine = a.T <= kTcC || a.B * a.T * a.H <= kTcFineRows;
+    return fine ? launch_kernel<DQ, DV, NP, true>(a, m, passes, s)
+                : launch_kernel<DQ, DV, NP, false>(a, m, passes, s);
 }
 
 }  // namespace
