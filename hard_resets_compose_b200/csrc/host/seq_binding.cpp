@@ -438,6 +438,7 @@ py::object attention_step(const Tensor &q, const Tensor &k, const Tensor &v, con
                         : state.size(0) < B)
         return py::none();
     const c10::cuda::CUDAGuard guard(q.device());
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();  // who has saved it hears of the change
     Tensor o = torch::empty({B, H, Dv}, q.options());
     lifb_leaky_attn_step_args a{};
     a.q = at(q), a.k = at(k), a.v = at(v), a.log_decay = at_f32(ld), a.slots = at_i32(slots);

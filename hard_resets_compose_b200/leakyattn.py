@@ -179,6 +179,7 @@ def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
         raise RuntimeError(f"{what} is not differentiable: use leaky_attention, or torch.no_grad()")
     q, k, v, log_decay = _last_dense(q), _last_dense(k), _last_dense(v), log_decay.contiguous()
     scale = float(Dk) ** -0.5 if scale is None and Dk > 0 else float(scale or 0.0)
+    torch.autograd.graph.increment_version(state)  # who has saved it hears of the change
     o = q.new_empty((B, H, Dv))
     q0, q1, _ = q.stride()
     k0, k1, _ = k.stride()
