@@ -13,6 +13,7 @@ import threading
 import time
 
 import torch
+from torch.autograd import forward_ad
 
 from . import build as _build
 
@@ -335,6 +336,14 @@ def need_cuda(what: str, names: str, *tensors) -> None:
     name = names.split()[[x is t for x in tensors].index(True)]
     raise RuntimeError(f"{what}: {name} must be a CUDA tensor" if d < 0 else
                        f"{what}: {name} is on {t.device}, not cuda:{dev}")
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raises if one of the tensors (None: absent) is a dual tensor of forward-mode
+    differentiation: dropping its tangent would pass for a derivative of zero."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 _poll_again = 0.0  # when the next poll is due

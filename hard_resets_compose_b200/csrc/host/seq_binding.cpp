@@ -168,6 +168,15 @@ bool wants_grad(std::initializer_list<const Tensor *> ts)
     return false;
 }
 
+// Whether one of them is a dual tensor: no operator has a forward-mode derivative, and the
+// Python functions refuse it
+bool has_tangent(std::initializer_list<const Tensor *> ts)
+{
+    for (const Tensor *t : ts)
+        if (t->defined() && t->_fw_grad(0).defined()) return true;
+    return false;
+}
+
 // ---- embedding
 
 Tensor embed_forward(const Tensor &tokens, const Tensor &weight, double scale)
@@ -215,7 +224,8 @@ py::object embedding(const Tensor &tokens, const Tensor &weight, double scale)
 {
     const auto tt = tokens.scalar_type();
     if (!weight.is_cuda() || weight.dim() != 2 || !weight.is_contiguous() || type_of(weight) < 0 ||
-        !on(tokens, weight.get_device()) || !tokens.is_contiguous() || (tt != torch::kInt && tt != torch::kLong))
+        !on(tokens, weight.get_device()) || !tokens.is_contiguous() || (tt != torch::kInt && tt != torch::kLong) ||
+        has_tangent({&weight}))
         return py::none();
     return py::cast(wants_grad({&weight}) ? EmbedFn::apply(tokens, weight, scale) : embed_forward(tokens, weight, scale));
 }
@@ -298,7 +308,7 @@ py::object norm_gate(const Tensor &x, const OptTensor &h_, const OptTensor &gate
 {
     const Tensor h = h_.value_or(Tensor()), gate = gate_.value_or(Tensor()), post = post_.value_or(Tensor()),
                  pre = pre_.value_or(Tensor());
-    if (!x.is_cuda() || x.dim() < 1 || type_of(x) < 0) return py::none();
+    if (!x.is_cuda() || x.dim() < 1 || type_of(x) < 0 || has_tangent({&x, &h, &gate, &post, &pre})) return py::none();
     const int64_t dev = x.get_device(), D = x.size(-1);
     if (D < 1 || row_stride(x) < 0 || D > 8192 || (!post.defined() && !pre.defined()) || h.defined() != post.defined()) return py::none();
     for (const Tensor *t : {&h, &gate})
@@ -408,7 +418,9 @@ py::object attention(const Tensor &q, const Tensor &k, const Tensor &v, const Te
                      const OptTensor &lengths_, std::optional<double> scale, bool return_state)
 {
     const Tensor state = state_.value_or(Tensor()), lengths = lengths_.value_or(Tensor());
-    if (!attn_fits(q, k, v, ld, 2) || (type_of(q) != LIFB_F32 && type_of(q) != LIFB_BF16)) return py::none();
+    if (!attn_fits(q, k, v, ld, 2) || (type_of(q) != LIFB_F32 && type_of(q) != LIFB_BF16) ||
+        has_tangent({&q, &k, &v, &ld, &state}))
+        return py::none();
     const int64_t dev = q.get_device(), B = q.size(0), H = q.size(2), Dk = q.size(3), Dv = v.size(3);
     if (state.defined() && (!on(state, dev) || state.scalar_type() != torch::kFloat || !state.is_contiguous() ||
                             state.sizes() != at::IntArrayRef({B, H, Dk, Dv})))
@@ -428,7 +440,9 @@ py::object attention_step(const Tensor &q, const Tensor &k, const Tensor &v, con
                           const OptTensor &slots_, std::optional<double> scale)
 {
     const Tensor slots = slots_.value_or(Tensor());
-    if (!attn_fits(q, k, v, ld, 1) || type_of(q) < 0 || wants_grad({&q, &k, &v, &state})) return py::none();
+    if (!attn_fits(q, k, v, ld, 1) || type_of(q) < 0 || wants_grad({&q, &k, &v, &state}) ||
+        has_tangent({&q, &k, &v, &ld, &state}))
+        return py::none();
     const int64_t dev = q.get_device(), B = q.size(0), H = q.size(1), Dk = q.size(2), Dv = v.size(2);
     if (!on(state, dev) || state.dim() != 4 || state.scalar_type() != torch::kFloat || state.size(1) != H ||
         state.size(2) != Dk || state.size(3) != Dv || state.stride(3) != 1 || state.stride(2) != Dv)

@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import DTYPES, addr, check, need_cuda, on_device, raw_stream
+from ._lib import DTYPES, addr, check, need_cuda, on_device, raw_stream, refuse_tangents
 
 
 def _forward(tokens, weight, scale):
@@ -71,6 +71,7 @@ def embedding(tokens, weight, scale=1.0):
     if tokens.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"embedding: tokens must be int32 or int64, got {tokens.dtype}")
     need_cuda("embedding", "tokens weight", tokens, weight)
+    refuse_tangents("embedding", weight)
     tokens = tokens.contiguous()
     if not weight.is_contiguous() and (weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]):
         weight = weight.contiguous()

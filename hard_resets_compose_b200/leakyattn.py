@@ -24,7 +24,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import DTYPES, addr, check, need_cuda, on_device, raw_stream
+from ._lib import DTYPES, addr, check, need_cuda, on_device, raw_stream, refuse_tangents
 
 MAX_WIDTH = 128
 
@@ -128,6 +128,7 @@ def leaky_attention(q, k, v, log_decay, state=None, lengths=None, scale=None, re
     what = "leaky_attention"
     H, _, Dk, Dv = _check(what, q, k, v, log_decay, 2, _SEQ_TYPES)
     need_cuda(what, "q k v log_decay state lengths", q, k, v, log_decay, state, lengths)
+    refuse_tangents(what, q, k, v, log_decay, state)
     B = q.shape[0]
     if state is not None:
         if state.shape != (B, H, Dk, Dv) or state.dtype != torch.float32:
@@ -162,6 +163,7 @@ def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     what = "leaky_attention_step"
     H, Hk, Dk, Dv = _check(what, q, k, v, log_decay, 1, _STEP_TYPES)
     need_cuda(what, "q k v log_decay state slots", q, k, v, log_decay, state, slots)
+    refuse_tangents(what, q, k, v, log_decay, state)
     B = q.shape[0]
     if state.dim() != 4 or state.shape[1:] != (H, Dk, Dv) or state.dtype != torch.float32:
         raise ValueError(f"{what}: state must be [slots, {H}, {Dk}, {Dv}] fp32, got {tuple(state.shape)} {state.dtype}")

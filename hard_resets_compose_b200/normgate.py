@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import DTYPES, addr, check, need_cuda, on_device, raw_stream
+from ._lib import DTYPES, addr, check, need_cuda, on_device, raw_stream, refuse_tangents
 
 ACTS = {"silu": 0, "sigmoid": 1, "none": 2}
 MAX_WIDTH = 8192
@@ -108,6 +108,7 @@ def _run(what, x, h, gate, post, pre, scale, eps, act):
     if dt not in DTYPES:
         raise TypeError(f"{what}: x must be fp32, bf16 or fp16, got {dt}")
     need_cuda(what, "x h gate post_weight pre_weight", x, h, gate, post, pre)
+    refuse_tangents(what, x, h, gate, post, pre)
     for name, t in (("h", h), ("gate", gate)):
         if t is not None:
             if t.dtype != dt:

@@ -2,6 +2,7 @@
 binding and the Python functions)."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from hard_resets_compose_b200 import _lib, embed, leakyattn, normgate
 
@@ -62,3 +63,34 @@ def test_a_cache_made_in_inference_mode(host):
         leakyattn.leaky_attention_step(q, q, q, ld, want)
     leakyattn.leaky_attention_step(q, q, q, ld, cache)
     assert torch.equal(cache, want)
+
+
+CALLS = {
+    "embedding": lambda d: embed.embedding(torch.arange(4, device=DEV), d(4, 8)),
+    "norm_x": lambda d: normgate.norm_gate_residual(d(4, 8), rand(4, 8, seed=2), None, rand(8, seed=3), rand(8, seed=4)),
+    "norm_h": lambda d: normgate.norm_gate_residual(rand(4, 8, seed=2), d(4, 8), None, rand(8, seed=3)),
+    "norm_gate": lambda d: normgate.norm_gate_residual(rand(4, 8, seed=2), rand(4, 8, seed=5), d(4, 1), rand(8, seed=3)),
+    "norm_post": lambda d: normgate.norm_gate_residual(rand(4, 8, seed=2), rand(4, 8, seed=5), None, d(8)),
+    "rms_norm": lambda d: normgate.rms_norm(rand(4, 8, seed=2), d(8)),
+    "attention_q": lambda d: leakyattn.leaky_attention(d(2, 4, 2, 8), *(rand(2, 4, 2, 8, seed=i) for i in (1, 2)),
+                                                       -torch.ones(2, device=DEV)),
+    "attention_decay": lambda d: leakyattn.leaky_attention(*(rand(2, 4, 2, 8, seed=i) for i in (1, 2, 3)), d(2)),
+    "attention_state": lambda d: leakyattn.leaky_attention(*(rand(2, 4, 2, 8, seed=i) for i in (1, 2, 3)),
+                                                           -torch.ones(2, device=DEV), state=d(2, 2, 8, 8)),
+    "step_v": lambda d: leakyattn.leaky_attention_step(rand(2, 2, 8, seed=1), rand(2, 2, 8, seed=2), d(2, 2, 8),
+                                                       -torch.ones(2, device=DEV), rand(2, 2, 8, 8, seed=3)),
+    "step_state": lambda d: leakyattn.leaky_attention_step(*(rand(2, 2, 8, seed=i) for i in (1, 2, 3)),
+                                                           -torch.ones(2, device=DEV), d(2, 2, 8, 8)),
+}
+
+
+@pytest.mark.parametrize("grad", (True, False))
+@pytest.mark.parametrize("call", sorted(CALLS))
+def test_tangents_are_refused(host, call, grad):
+    """No operator has a forward-mode derivative: a dual tensor is refused, not stripped."""
+    with torch.set_grad_enabled(grad), fwAD.dual_level():
+        def dual(*shape):
+            return fwAD.make_dual(-rand(*shape, seed=7).abs(), rand(*shape, seed=8))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            CALLS[call](dual)
+        CALLS[call](lambda *shape: -rand(*shape, seed=7).abs())  # without a tangent it runs
