@@ -436,6 +436,13 @@ py::object attention(const Tensor &q, const Tensor &k, const Tensor &v, const Te
     return py::make_tuple(out[0], out[1]);
 }
 
+// Slots and heads in the usual order, none over another; other orders are looked at in Python
+bool apart(const Tensor &state)
+{
+    const int64_t n = state.size(0), H = state.size(1), mat = state.size(2) * state.size(3);
+    return (H == 1 || state.stride(1) >= mat) && (n == 1 || state.stride(0) >= (H - 1) * state.stride(1) + mat);
+}
+
 py::object attention_step(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &ld, const Tensor &state,
                           const OptTensor &slots_, std::optional<double> scale)
 {
@@ -445,7 +452,7 @@ py::object attention_step(const Tensor &q, const Tensor &k, const Tensor &v, con
         return py::none();
     const int64_t dev = q.get_device(), B = q.size(0), H = q.size(1), Dk = q.size(2), Dv = v.size(2);
     if (!on(state, dev) || state.dim() != 4 || state.scalar_type() != torch::kFloat || state.size(1) != H ||
-        state.size(2) != Dk || state.size(3) != Dv || state.stride(3) != 1 || state.stride(2) != Dv)
+        state.size(2) != Dk || state.size(3) != Dv || state.stride(3) != 1 || state.stride(2) != Dv || !apart(state))
         return py::none();
     if (slots.defined() ? !on(slots, dev) || slots.scalar_type() != torch::kInt || !slots.is_contiguous() ||
                               slots.dim() != 1 || slots.size(0) != B

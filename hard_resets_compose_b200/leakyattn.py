@@ -150,6 +150,17 @@ def leaky_attention(q, k, v, log_decay, state=None, lengths=None, scale=None, re
     return (o, out) if return_state else o
 
 
+def _overlap(n, s0, h, s1, mat):
+    """Whether two of n x h matrices of `mat` elements, at distances s0 and s1, share memory."""
+    if n > 1 and s0 < mat:
+        return True
+    for j in range(1, h):
+        i = min(n - 1, j * s1 // s0) if n > 1 else 0  # the nearest ones below and above
+        if abs(j * s1 - i * s0) < mat or abs(j * s1 - min(i + 1, n - 1) * s0) < mat:
+            return True
+    return False
+
+
 def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     """One token of each sequence: o [B, H, Dv]; `state` is updated in place.
 
@@ -170,6 +181,8 @@ def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     st = state.stride()
     if Dk * Dv > 1 and ((Dv > 1 and st[3] != 1) or (Dk > 1 and st[2] != Dv)):
         raise ValueError(f"{what}: each head's state must be contiguous")
+    if Dk * Dv and state.shape[0] and _overlap(state.shape[0], st[0], H, st[1], Dk * Dv):
+        raise ValueError(f"{what}: slots or heads of the state share memory")
     if slots is None:
         if state.shape[0] < B:
             raise ValueError(f"{what}: {B} sequences but {state.shape[0]} states")

@@ -94,3 +94,25 @@ def test_tangents_are_refused(host, call, grad):
         with pytest.raises(RuntimeError, match="forward-mode"):
             CALLS[call](dual)
         CALLS[call](lambda *shape: -rand(*shape, seed=7).abs())  # without a tangent it runs
+
+
+def test_overlapping_caches_are_refused(host):
+    """Slots or heads that share memory would be written by two sequences at once."""
+    H, D = 2, 8
+    q, ld = rand(3, H, D, seed=2), -torch.ones(2, device=DEV)
+    for state in (rand(1, H, D, D, seed=1).expand(3, H, D, D), rand(3, 1, D, D, seed=1).expand(3, H, D, D),
+                  torch.zeros(4 * H * D * D, device=DEV).as_strided((3, H, D, D), (D * D, D * D, D, 1))):
+        with pytest.raises((ValueError, RuntimeError), match="share memory"):
+            leakyattn.leaky_attention_step(q, q, q, ld, state)
+
+
+def test_caches_in_other_orders(host):
+    """Heads before slots, and slots between the heads of others: nothing overlaps."""
+    n, H, D = 3, 2, 8
+    q, ld, x = rand(n, H, D, seed=2), -torch.ones(2, device=DEV), rand(n, H, D, D, seed=1)
+    want = x.clone()
+    o = leakyattn.leaky_attention_step(q, q, q, ld, want)
+    for strides in ((D * D, n * D * D), (2 * D * D, 7 * D * D)):
+        cache = torch.zeros(20 * D * D, device=DEV).as_strided((n, H, D, D), (*strides, D, 1))
+        cache.copy_(x)
+        assert torch.equal(leakyattn.leaky_attention_step(q, q, q, ld, cache), o) and torch.equal(cache, want)
