@@ -49,6 +49,14 @@ class SeqBlock(nn.Module):
         # memories from a few tokens to thousands
         self.register_buffer("log_decay", torch.log1p(-torch.exp2(-torch.linspace(2.0, 10.0, heads))))
 
+    def _apply(self, fn, recurse=True):
+        """Moves of the module; the decay stays fp32 (1 - 2^-10 is 1 in bf16), bit for bit."""
+        decay = self.log_decay
+        super()._apply(fn, recurse)
+        if self.log_decay.dtype != decay.dtype:
+            self.log_decay = decay.to(self.log_decay.device)
+        return self
+
     def attention_in(self, n):
         q, k, v, g = self.qkvg(n).split(self.splits, -1)
         heads = lambda t, h: t.unflatten(-1, (h, self.dim))  # noqa: E731

@@ -116,3 +116,16 @@ def test_caches_in_other_orders(host):
         cache = torch.zeros(20 * D * D, device=DEV).as_strided((n, H, D, D), (*strides, D, 1))
         cache.copy_(x)
         assert torch.equal(leakyattn.leaky_attention_step(q, q, q, ld, cache), o) and torch.equal(cache, want)
+
+
+def test_bf16_models_run_as_they_come(host):
+    """SeqNet(...).bfloat16() without a word to its buffers."""
+    from hard_resets_compose_b200.seqnet import SeqNet
+    torch.manual_seed(3)
+    net = SeqNet(vocab=50, width=64, heads=4, layers=2).cuda().bfloat16()
+    tok = torch.randint(0, 50, (3, 20), device=DEV)
+    net(tok).float().sum().backward()
+    cache, slots = net.new_cache(4), torch.tensor([1, 0, 3], dtype=torch.int32, device=DEV)
+    n = torch.tensor([20, 3, 7], dtype=torch.int32, device=DEV)
+    assert torch.isfinite(net.prompt(tok, cache, slots, n)).all()
+    assert torch.isfinite(net.step(tok[:, 0], cache, slots)).all()
