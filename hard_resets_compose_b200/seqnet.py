@@ -31,6 +31,28 @@ from .leakyattn import leaky_attention, leaky_attention_step
 from .normgate import norm_gate_residual, rms_norm
 
 
+class _Places:
+    """Where B sequences' states lie in a cache of n slots: slots [B] int32, outside [0, n) an
+    empty place, as for leaky_attention_step.  An empty place is given the slot of a
+    live one and writes what that one writes, so that the cache changes by the live ones
+    alone (by none if there is none) without the host knowing which they are."""
+
+    def __init__(self, slots, n):
+        self.live = (slots >= 0) & (slots < n)
+        self.any = self.live.any()
+        rows = torch.arange(len(slots), device=slots.device)
+        self.source = torch.where(self.live, rows, self.live.long().argmax()) if len(slots) else rows
+        self.at = torch.where(self.any, slots.long()[self.source], 0)
+
+    def get(self, cache):
+        """The live sequences' rows (an empty place's row is some live one's)."""
+        return cache[self.at]
+
+    def put(self, cache, rows, old=None):
+        """Writes the live sequences' rows; old: what get gave."""
+        cache[self.at] = torch.where(self.any, rows[self.source], self.get(cache) if old is None else old)
+
+
 class SeqBlock(nn.Module):
     """Leaky attention and a LIF layer, each followed by its norms, gate and residual."""
 
@@ -118,11 +140,12 @@ class SeqNet(nn.Module):
 
     @torch.no_grad()
     def prompt(self, tokens, cache, slots, lengths):
-        """Runs prompts [B, T] from rest into the slots [B] int32 (lengths [B] int32);
-        logits [B, V] after each one's last token (an empty prompt's are the readout's of zeros)."""
+        """Runs prompts [B, T] from rest into the slots [B] int32, at most one to a slot (outside
+        the cache: the prompt's states are not kept), lengths [B] int32; logits [B, V] after
+        each one's last token (an empty prompt's are the readout's of zeros)."""
         x, n = self._embed(tokens)
         B, T = tokens.shape
-        at = slots.long()
+        places = _Places(slots, cache[0][0].shape[0]) if cache else None
         last = (lengths.long() - 1).clamp(min=0)
         rows = torch.arange(B, device=tokens.device)
         empty = (lengths <= 0)[:, None]
@@ -130,13 +153,13 @@ class SeqNet(nn.Module):
         for i, (states, potentials) in enumerate(cache):
             def attend(b, q, k, v):
                 o, s = leaky_attention(q, k, v, b.log_decay, lengths=lengths, return_state=True)
-                states[at] = s
+                places.put(states, s)
                 return o
 
             def spike(b, current):
                 i = current.transpose(0, 1).reshape(T, B * self.width).contiguous()
                 u, s = L.serial_forward(i, b.beta, self.theta, 0.0, torch.zeros(i.shape[1], device=i.device))
-                potentials[at] = torch.where(empty, 0.0, u.view(T, B, self.width)[last, rows])
+                places.put(potentials, torch.where(empty, 0.0, u.view(T, B, self.width)[last, rows]))
                 return s.view(T, B, self.width).transpose(0, 1)
 
             x, n = self._block(i, x, n, attend, spike)
@@ -144,21 +167,22 @@ class SeqNet(nn.Module):
 
     @torch.no_grad()
     def step(self, tokens, cache, slots):
-        """One token [B] of each sequence (slots [B] int32, all in the cache, at most one
-        sequence to a slot); logits [B, V].  The cache is updated in place."""
+        """One token [B] of each sequence (slots [B] int32, at most one sequence to a slot);
+        logits [B, V].  The cache is updated in place.  A slot outside the cache (-1, say)
+        is an empty place: its logits are zeros and nothing changes."""
         x, n = self._embed(tokens)
         B = tokens.shape[0]
-        at = slots.long()
+        places = _Places(slots, cache[0][0].shape[0]) if cache else None
 
         for i, (states, potentials) in enumerate(cache):
             def attend(b, q, k, v):
                 return leaky_attention_step(q, k, v, b.log_decay, states, slots=slots)
 
             def spike(b, current):
-                u, s = L.serial_forward(current.reshape(1, -1).contiguous(), b.beta, self.theta, 0.0,
-                                        potentials[at].reshape(-1))
-                potentials[at] = u.view(B, self.width)
+                u0 = places.get(potentials)
+                u, s = L.serial_forward(current.reshape(1, -1).contiguous(), b.beta, self.theta, 0.0, u0.reshape(-1))
+                places.put(potentials, u.view(B, self.width), u0)
                 return s.view(B, self.width)
 
             x, n = self._block(i, x, n, attend, spike)
-        return self._logits(n)
+        return self._logits(torch.where(places.live[:, None], n, 0.0) if places else n)

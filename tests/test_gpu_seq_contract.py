@@ -129,3 +129,31 @@ def test_bf16_models_run_as_they_come(host):
     n = torch.tensor([20, 3, 7], dtype=torch.int32, device=DEV)
     assert torch.isfinite(net.prompt(tok, cache, slots, n)).all()
     assert torch.isfinite(net.step(tok[:, 0], cache, slots)).all()
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_the_model_leaves_empty_places_alone(host, dtype):
+    """Prompts and steps of a batch with an empty place: the bits of the same batch with a place for
+    it, and nothing else in the cache changes."""
+    from hard_resets_compose_b200.seqnet import SeqNet
+    torch.manual_seed(3)
+    net = SeqNet(vocab=50, width=64, heads=4, layers=2, kv_heads=2).cuda().to(dtype)
+    tok = torch.randint(0, 50, (3, 20), device=DEV)
+    n = torch.tensor([20, 3, 7], dtype=torch.int32, device=DEV)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+
+    def filled():
+        torch.manual_seed(4)
+        return [tuple(torch.randn_like(t) for t in pair) for pair in net.new_cache(5)]
+    start, all_there, one_empty = filled(), filled(), filled()
+    for slots, empty in ((i32(2, 0, 4), i32(2, -1, 4)), (i32(0, 3, 1), i32(5, 3, 1))):
+        live = empty.clamp(0, 4) == empty
+        for out, got in ((net.prompt(tok, all_there, slots, n), net.prompt(tok, one_empty, empty, n)),
+                         (net.step(tok[:, 0], all_there, slots), net.step(tok[:, 0], one_empty, empty))):
+            assert torch.equal(out[live], got[live])
+    for a, b, was in zip(all_there, one_empty, start):
+        for x, y, w in zip(a, b, was):
+            assert torch.equal(x[1:], y[1:]) and torch.equal(y[0], w[0])
+    before = [tuple(t.clone() for t in pair) for pair in one_empty]
+    assert not net.step(tok[:, 0], one_empty, i32(-1, 5, 99)).any()
+    assert all(torch.equal(x, y) for p, q in zip(before, one_empty) for x, y in zip(p, q))
