@@ -116,3 +116,12 @@ def test_a_prompt_with_empty_places(net):
     for pair, was, ref in zip(cache, before, whole):
         for t, w, r in zip(pair, was, ref):
             assert torch.equal(t[3], r[1]) and torch.equal(t[0], r[2]) and torch.equal(t[1:3], w[1:3])
+
+
+def test_lengths_outside_the_batch(net):
+    """Lengths past T count as T, below zero as zero, as the attention takes them."""
+    tokens = torch.randint(0, 30, (3, 4), generator=torch.Generator().manual_seed(2))
+    a, b = net.new_cache(3), net.new_cache(3)
+    want = net.prompt(tokens, a, i32(0, 1, 2), i32(4, 0, 2))
+    assert torch.equal(net.prompt(tokens, b, i32(0, 1, 2), i32(9, -3, 2)), want)
+    assert all(torch.equal(x, y) for p, q in zip(a, b) for x, y in zip(p, q))
