@@ -143,9 +143,14 @@ class SeqNet(nn.Module):
         """Runs prompts [B, T] from rest into the slots [B] int32, at most one to a slot (outside
         the cache: the prompt's states are not kept), lengths [B] int32, taken into 0..T;
         logits [B, V] after each one's last token (an empty prompt's are the readout's of zeros)."""
-        x, n = self._embed(tokens)
         B, T = tokens.shape
         places = _Places(slots, cache[0][0].shape[0]) if cache else None
+        if T == 0:  # no token: all at rest
+            for pair in cache:
+                for states in pair:
+                    places.put(states, states.new_zeros(B, *states.shape[1:]))
+            return self.embed.new_zeros(B, self.embed.shape[0])
+        x, n = self._embed(tokens)
         last = lengths.long().clamp(max=T).sub(1).clamp(min=0)  # as the attention takes them
         rows = torch.arange(B, device=tokens.device)
         empty = (lengths <= 0)[:, None]

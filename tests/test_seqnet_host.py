@@ -125,3 +125,10 @@ def test_lengths_outside_the_batch(net):
     want = net.prompt(tokens, a, i32(0, 1, 2), i32(4, 0, 2))
     assert torch.equal(net.prompt(tokens, b, i32(0, 1, 2), i32(9, -3, 2)), want)
     assert all(torch.equal(x, y) for p, q in zip(a, b) for x, y in zip(p, q))
+
+
+def test_prompts_without_tokens(net):
+    cache = filled(net, 2)
+    got = net.prompt(torch.zeros(2, 0, dtype=torch.long), cache, i32(0, 1), i32(0, 0))
+    assert got.shape == (2, 30) and not got.any()
+    assert not any(t.any() for pair in cache for t in pair)
