@@ -346,15 +346,14 @@ def refuse_tangents(what: str, *tensors) -> None:
             raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
-_poll_again = 0.0  # when the next poll is due
+_poll_again = {}  # device: when its next poll is due
 
 
 def poll_device_sometimes(what: str) -> None:
     """poll_device, at most every 20 ms: for calls as short as the poll itself."""
-    global _poll_again
-    now = time.monotonic()
-    if now >= _poll_again:
-        _poll_again = now + 0.02
+    now, dev = time.monotonic(), _raw_device()
+    if now >= _poll_again.get(dev, 0.0):
+        _poll_again[dev] = now + 0.02
         poll_device(what)
 
 

@@ -90,19 +90,30 @@ void done(int status, const char *what)
     if (status != LIFB_OK) (*L.check)(status, what);
 }
 
-// A call's status in the autograd engine's thread, which carries torch's own form of a
-// Python exception to the caller; then the library's poll, at most every 20 ms
-void done_in_backward(int status, const char *what)
+// The library's poll of the current device, at most every 20 ms and not while a graph is
+// captured
+int poll_sometimes()
 {
-    static std::atomic<int64_t> again{0};
+    static std::atomic<int64_t> again[64];  // a device each
     const int64_t now = std::chrono::duration_cast<std::chrono::milliseconds>(
                             std::chrono::steady_clock::now().time_since_epoch())
                             .count();
-    if (status == LIFB_OK && now >= again.load(std::memory_order_relaxed) &&
-        c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) {
-        again.store(now + 20, std::memory_order_relaxed);
-        status = L.poll();
-    }
+    auto &due = again[c10::cuda::current_device() & 63];
+    if (now < due.load(std::memory_order_relaxed) ||
+        c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+        return LIFB_OK;
+    due.store(now + 20, std::memory_order_relaxed);
+    return L.poll();
+}
+
+// Before a forward: one that raises has then changed nothing
+void ready(const char *what) { done(poll_sometimes(), what); }
+
+// A call's status in the autograd engine's thread, which carries torch's own form of a
+// Python exception to the caller; then the poll
+void done_in_backward(int status, const char *what)
+{
+    if (status == LIFB_OK) status = poll_sometimes();
     if (status == LIFB_OK) return;
     py::gil_scoped_acquire gil;
     try {
@@ -182,6 +193,7 @@ bool has_tangent(std::initializer_list<const Tensor *> ts)
 Tensor embed_forward(const Tensor &tokens, const Tensor &weight, double scale)
 {
     const c10::cuda::CUDAGuard guard(weight.device());
+    ready("embedding");
     auto shape = tokens.sizes().vec();
     shape.push_back(weight.size(1));
     Tensor y = torch::empty(shape, weight.options());
@@ -250,6 +262,7 @@ variable_list norm_forward(const Tensor &x, const Tensor &h, const Tensor &gate,
                            const Tensor &rstd, double scale, double eps, int64_t act)
 {
     const c10::cuda::CUDAGuard guard(x.device());
+    ready("norm_gate_residual");
     Tensor xo, n;
     if (h.defined()) xo = torch::empty(x.sizes(), x.options());
     if (pre.defined()) n = torch::empty(x.sizes(), x.options());
@@ -352,6 +365,7 @@ variable_list attn_forward(const Tensor &q, const Tensor &k, const Tensor &v, co
                            const Tensor &lengths, double scale, bool return_state)
 {
     const c10::cuda::CUDAGuard guard(q.device());
+    ready("leaky_attention");
     const lifb_leaky_attn a = attn_args(q, k, v, ld, state, lengths, scale);
     variable_list out{torch::empty({a.B, a.T, a.H, a.Dv}, q.options())};
     if (return_state) out.push_back(torch::empty({a.B, a.H, a.Dk, a.Dv}, q.options().dtype(torch::kFloat)));
@@ -459,6 +473,7 @@ py::object attention_step(const Tensor &q, const Tensor &k, const Tensor &v, con
                         : state.size(0) < B)
         return py::none();
     const c10::cuda::CUDAGuard guard(q.device());
+    ready("leaky_attention_step");
     if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();  // who has saved it hears of the change
     Tensor o = torch::empty({B, H, Dv}, q.options());
     lifb_leaky_attn_step_args a{};

@@ -3,8 +3,9 @@
     y = embedding(tokens, weight, scale)      # y[i] = scale * weight[tokens[i]]
 
 Negative tokens are padding: zeros out, no gradient.  A token past the table
-gives zeros too and is reported as a device error (code 102) by the library's
-next poll or by `_lib.check_device`.  The weight's gradient adds the rows of
+gives zeros too and is reported as a device error (code 102): raised by one of the
+next calls of this package's sequence operators (each polls, at most every 20 ms),
+or by `_lib.check_device`.  The weight's gradient adds the rows of
 each token in fp32, in an order that the tokens alone fix, and is rounded
 once: the same bits on every call.  The reference has no such operator.
 """
@@ -21,6 +22,7 @@ def _forward(tokens, weight, scale):
     V, D = weight.shape
     y = weight.new_empty(tokens.shape + (D,))
     with on_device(weight):
+        _lib.poll_device_sometimes("embedding")
         check(_lib.load().lifb_embed_fwd(tokens.data_ptr(), tokens.element_size(), weight.data_ptr(), y.data_ptr(),
                                          tokens.numel(), V, D, max(weight.stride(0), D), scale, DTYPES[weight.dtype],
                                          raw_stream(weight)), "embedding")

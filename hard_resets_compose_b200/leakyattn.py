@@ -48,6 +48,7 @@ def _forward(q, k, v, log_decay, state, lengths, scale, return_state):
     lib = _lib.load()
     args = _pack(q, k, v, log_decay, state, lengths, scale)
     with on_device(q):
+        _lib.poll_device_sometimes("leaky_attention")
         nb = lib.lifb_leaky_attn_workspace_bytes(args, 0)
         ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
         check(lib.lifb_leaky_attn_fwd(args, addr(o), addr(out), addr(ws), nb, raw_stream(q)), "leaky_attention")
@@ -194,7 +195,6 @@ def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
         raise RuntimeError(f"{what} is not differentiable: use leaky_attention, or torch.no_grad()")
     q, k, v, log_decay = _last_dense(q), _last_dense(k), _last_dense(v), log_decay.contiguous()
     scale = float(Dk) ** -0.5 if scale is None and Dk > 0 else float(scale or 0.0)
-    torch.autograd.graph.increment_version(state)  # who has saved it hears of the change
     o = q.new_empty((B, H, Dv))
     q0, q1, _ = q.stride()
     k0, k1, _ = k.stride()
@@ -203,5 +203,7 @@ def leaky_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
                                      Hk, Dk, Dv, state.shape[0], q0, q1, k0, k1, v0, v1, st[0], st[1], scale,
                                      DTYPES[q.dtype])
     with on_device(q):
+        _lib.poll_device_sometimes(what)
+        torch.autograd.graph.increment_version(state)  # who has saved it hears of the change
         check(_lib.load().lifb_leaky_attn_step(args, addr(o), addr(state), raw_stream(q)), what)
     return o

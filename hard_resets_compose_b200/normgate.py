@@ -57,6 +57,7 @@ def _forward(x, h, gate, post, pre, scale, eps, act, keep):
     gate = None if gate is None else _rows(gate, gate.shape[-1])
     rstd = x.new_empty((2, x.shape[0]), dtype=torch.float32) if keep else None
     with on_device(x):
+        _lib.poll_device_sometimes("norm_gate_residual")
         check(_lib.load().lifb_norm_gate_fwd(_pack(x, h, gate, post, pre, rstd, scale, eps, act), addr(xo), addr(n),
                                              raw_stream(x)), "norm_gate_residual")
     return xo, n, (x, h, gate, rstd)
@@ -99,6 +100,7 @@ class NormGateResidual(torch.autograd.Function):
                                          D if dn is None else dn.stride(0), addr(dx), addr(dh), addr(dgate),
                                          addr(dpost), addr(dpre), ws.data_ptr(), nb, raw_stream(x)),
                   "norm_gate_residual")
+            _lib.poll_device_sometimes("norm_gate_residual")
         return dx, dh, dgate, dpost, dpre, None, None, None
 
 

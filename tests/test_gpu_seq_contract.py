@@ -1,5 +1,7 @@
 """What the sequence-model operators owe autograd and their callers, on both host paths (the C++
 binding and the Python functions)."""
+import time
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -157,3 +159,52 @@ def test_the_model_leaves_empty_places_alone(host, dtype):
     before = [tuple(t.clone() for t in pair) for pair in one_empty]
     assert not net.step(tok[:, 0], one_empty, i32(-1, 5, 99)).any()
     assert all(torch.equal(x, y) for p, q in zip(before, one_empty) for x, y in zip(p, q))
+
+
+def test_device_errors_reach_inference(host):
+    """A token past the table, in a program that never runs a backward."""
+    x, w = rand(4, 8, seed=1), rand(8, seed=2)
+    q, ld, state = rand(2, 2, 8, seed=3), -torch.ones(2, device=DEV), rand(2, 2, 8, 8, seed=4)
+    table, good = rand(10, 8, seed=5), torch.tensor([1], device=DEV)
+    calls = (lambda: embed.embedding(good, table), lambda: normgate.rms_norm(x, w),
+             lambda: leakyattn.leaky_attention_step(q, q, q, ld, state),
+             lambda: leakyattn.leaky_attention(q[None], q[None], q[None], ld))
+    _lib.check_device("before")
+    for call in calls:
+        embed.embedding(torch.tensor([99], device=DEV), table)
+        torch.cuda.synchronize()
+        try:
+            with pytest.raises(_lib.LifbError) as e:
+                for _ in range(5):
+                    call()
+                    torch.cuda.synchronize()
+                    time.sleep(0.03)
+            assert e.value.device_code == 102
+        finally:
+            with pytest.raises(_lib.LifbError):
+                _lib.check_device("after", reset=True)
+        _lib.check_device("cleared")
+
+
+def test_a_step_that_reports_an_error_has_not_run(host):
+    table = rand(10, 8, seed=5)
+    q, ld, state = rand(2, 2, 8, seed=3), -torch.ones(2, device=DEV), rand(2, 2, 8, 8, seed=4)
+    _lib.check_device("before")
+    embed.embedding(torch.tensor([99], device=DEV), table)
+    torch.cuda.synchronize()
+    raised = False
+    try:
+        for _ in range(5):
+            was = state.clone()
+            try:
+                leakyattn.leaky_attention_step(q, q, q, ld, state)
+            except _lib.LifbError:
+                raised = True
+                assert torch.equal(state, was)
+                break
+            assert not torch.equal(state, was)
+            time.sleep(0.03)
+    finally:
+        with pytest.raises(_lib.LifbError):
+            _lib.check_device("after", reset=True)
+    assert raised
