@@ -540,65 +540,74 @@ int64_t norm_blocks(const NormShape &s, int64_t R, bool bwd)
 }
 
 template <typename T, int VEC, int NIT, int MAXT, int GATE, int ACT = -1>
-void norm_launch(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
+bool norm_launch(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
 {
     const unsigned blocks = (unsigned)norm_blocks(sh, a.R, bwd);
-    count_launches(1);
     if (bwd) {
         // weights, and each group's sums: 2 * (1 + groups) rows of tpr * VEC * NIT floats
-        const size_t smem = (size_t)2 * (1 + sh.threads / sh.tpr) * sh.tpr * VEC * NIT * 4;  // 128 KB at most
+        const size_t smem = (size_t)2 * (1 + sh.threads / sh.tpr) * sh.tpr * VEC * NIT * 4;
+        // the kernel's limit is the most that any row takes (tpr = MAXT; 128 KB at most): the
+        // limit is one for all threads, and a call's own size could lower it under another's launch
         auto kern = k_norm_bwd<T, VEC, NIT, MAXT, GATE, ACT>;
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * 2 * MAXT * VEC * NIT * 4) !=
+            cudaSuccess)
+            return false;
+        count_launches(1);
         kern<<<blocks, MAXT, smem, s>>>(a, sh.tpr);
     } else {
+        count_launches(1);
         k_norm_fwd<T, VEC, NIT, MAXT, GATE, ACT><<<blocks, MAXT, 0, s>>>(a, sh.tpr);
     }
+    return true;
 }
 
 template <typename T, int VEC, int NIT>
-void norm_gate(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
+bool norm_gate(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
 {
     if (sh.threads == kNgMaxThreads) {
         if constexpr (VEC * NIT == kNgMaxElems || (VEC * NIT == 8 && (VEC == 1 || (VEC == 2 && sizeof(T) == 4))))
-            norm_launch<T, VEC, NIT, kNgMaxThreads, -1>(bwd, a, sh, s);
+            return norm_launch<T, VEC, NIT, kNgMaxThreads, -1>(bwd, a, sh, s);
+        else
+            return false;  // norm_shape gives no such row
     } else if constexpr (VEC * sizeof(T) != 16) {
-        norm_launch<T, VEC, NIT, kNgThreads, -1>(bwd, a, sh, s);
+        return norm_launch<T, VEC, NIT, kNgThreads, -1>(bwd, a, sh, s);
     } else if (!a.gate) {
-        norm_launch<T, VEC, NIT, kNgThreads, 0>(bwd, a, sh, s);
+        return norm_launch<T, VEC, NIT, kNgThreads, 0>(bwd, a, sh, s);
     } else if (a.gate_row) {
-        norm_launch<T, VEC, NIT, kNgThreads, 2>(bwd, a, sh, s);
+        return norm_launch<T, VEC, NIT, kNgThreads, 2>(bwd, a, sh, s);
     } else if (a.act == kActSilu) {
-        norm_launch<T, VEC, NIT, kNgThreads, 1, kActSilu>(bwd, a, sh, s);
+        return norm_launch<T, VEC, NIT, kNgThreads, 1, kActSilu>(bwd, a, sh, s);
     } else if (a.act == kActSigmoid) {
-        norm_launch<T, VEC, NIT, kNgThreads, 1, kActSigmoid>(bwd, a, sh, s);
+        return norm_launch<T, VEC, NIT, kNgThreads, 1, kActSigmoid>(bwd, a, sh, s);
     } else {
-        norm_launch<T, VEC, NIT, kNgThreads, 1, kActLinear>(bwd, a, sh, s);
+        return norm_launch<T, VEC, NIT, kNgThreads, 1, kActLinear>(bwd, a, sh, s);
     }
 }
 
 template <typename T>
-void norm_run(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
+bool norm_run(bool bwd, const NormArgs &a, const NormShape &sh, cudaStream_t s)
 {
     constexpr int VEC = 16 / sizeof(T);
     if (sh.vec == 1) {
-        if (sh.nit == 4) norm_gate<T, 1, 4>(bwd, a, sh, s);
-        else if (sh.nit == 8) norm_gate<T, 1, 8>(bwd, a, sh, s);
-        else norm_gate<T, 1, 16>(bwd, a, sh, s);
+        if (sh.nit == 4) return norm_gate<T, 1, 4>(bwd, a, sh, s);
+        else if (sh.nit == 8) return norm_gate<T, 1, 8>(bwd, a, sh, s);
+        else return norm_gate<T, 1, 16>(bwd, a, sh, s);
     } else if (sh.vec == 2) {
-        if (sh.nit == 4) norm_gate<T, 2, 4>(bwd, a, sh, s);
-        else norm_gate<T, 2, 8>(bwd, a, sh, s);
+        if (sh.nit == 4) return norm_gate<T, 2, 4>(bwd, a, sh, s);
+        else return norm_gate<T, 2, 8>(bwd, a, sh, s);
     } else if (sh.vec < VEC) {
         if constexpr (VEC == 8) {
-            if (sh.nit == 2) norm_gate<T, 4, 2>(bwd, a, sh, s);
-            else norm_gate<T, 4, 4>(bwd, a, sh, s);
+            if (sh.nit == 2) return norm_gate<T, 4, 2>(bwd, a, sh, s);
+            else return norm_gate<T, 4, 4>(bwd, a, sh, s);
         }
     } else if (sh.nit == 1) {
-        norm_gate<T, VEC, 1>(bwd, a, sh, s);
+        return norm_gate<T, VEC, 1>(bwd, a, sh, s);
     } else if (sh.nit == 2) {
-        norm_gate<T, VEC, 2>(bwd, a, sh, s);
+        return norm_gate<T, VEC, 2>(bwd, a, sh, s);
     } else if constexpr (VEC == 4) {
-        norm_gate<T, VEC, 4>(bwd, a, sh, s);
+        return norm_gate<T, VEC, 4>(bwd, a, sh, s);
     }
+    return false;
 }
 
 // Elements of a vector that D, the strides and the addresses (null: absent) allow.
@@ -673,8 +682,9 @@ extern "C" int lifb_norm_gate_fwd(const lifb_norm_gate *p, void *xo, void *n, vo
     NormShape sh;
     if (!norm_shape(a.D, vec, elem, false, sh))
         return norm_fail(LIFB_ERR_UNSUPPORTED, what, "rows longer than 8192 elements");
-    LIFB_BY_DTYPE(p->dtype, T, norm_run<T>(false, a, sh, (cudaStream_t)stream));
-    if (cudaGetLastError() != cudaSuccess) return norm_fail(LIFB_ERR_CUDA, what, "launch failed");
+    bool ok = false;
+    LIFB_BY_DTYPE(p->dtype, T, ok = norm_run<T>(false, a, sh, (cudaStream_t)stream));
+    if (cudaGetLastError() != cudaSuccess || !ok) return norm_fail(LIFB_ERR_CUDA, what, "launch failed");
     set_last_error("");
     return LIFB_OK;
 }
@@ -730,8 +740,9 @@ extern "C" int lifb_norm_gate_bwd(const lifb_norm_gate *p, const void *dxo, int6
     NormShape sh;
     if (!norm_shape(a.D, vec, elem, true, sh))
         return norm_fail(LIFB_ERR_UNSUPPORTED, what, "rows longer than 8192 elements");
-    LIFB_BY_DTYPE(p->dtype, T, norm_run<T>(true, a, sh, s));
-    if (weights) {
+    bool ok = false;
+    LIFB_BY_DTYPE(p->dtype, T, ok = norm_run<T>(true, a, sh, s));
+    if (ok && weights) {
         const int64_t parts = norm_blocks(sh, a.R, true);
         const unsigned blocks = (unsigned)((2 * a.D + 31) / 32);
         count_launches(1);
@@ -739,7 +750,7 @@ extern "C" int lifb_norm_gate_bwd(const lifb_norm_gate *p, const void *dxo, int6
                       (k_norm_weight_grads<T><<<blocks, 32 * kNgReduceRows, 0, s>>>((const float *)workspace, parts,
                                                                                  a.D, dpost, dpre, a.w_f32)));
     }
-    if (cudaGetLastError() != cudaSuccess) return norm_fail(LIFB_ERR_CUDA, what, "launch failed");
+    if (cudaGetLastError() != cudaSuccess || !ok) return norm_fail(LIFB_ERR_CUDA, what, "launch failed");
     set_last_error("");
     return LIFB_OK;
 }
