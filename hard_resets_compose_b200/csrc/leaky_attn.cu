@@ -441,10 +441,15 @@ bool launch_simt(const AttnArgs &a, int passes, bool state_only, cudaStream_t s)
         dq = std::max(dq, (a.p[i].dq + 3) & ~3);
         dv = std::max(dv, a.p[i].dv);
     }
-    const size_t smem = ((size_t)2 * kAtC * (dq + 4) + (size_t)kAtC * kAtSV + (size_t)kAtC * kAtSP +
-                         (size_t)dq * kAtSV) * 4;  // 82 KB at dq = 128
+    auto bytes = [](int dq) {  // 80 KB at dq = 128
+        return ((size_t)2 * kAtC * (dq + 4) + (size_t)kAtC * kAtSV + (size_t)kAtC * kAtSP + (size_t)dq * kAtSV) * 4;
+    };
+    const size_t smem = bytes(dq);
+    // the kernel's limit is the most that any width takes: it is one for all threads, and a
+    // call's own size could lower it under another's launch
     auto kern = k_attn_simt<T, W4>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(kAttnMaxDim)) != cudaSuccess)
+        return false;
     count_launches(1);
     kern<<<dim3((unsigned)(a.B * a.H * a.nseg), (unsigned)((dv + kAtTile - 1) / kAtTile), (unsigned)passes), kAtThreads,
            smem, s>>>(a, state_only);

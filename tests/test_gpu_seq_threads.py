@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from hard_resets_compose_b200 import _lib
-from hard_resets_compose_b200._lib import NORM_GATE
+from hard_resets_compose_b200._lib import LEAKY_ATTN, NORM_GATE
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,17 @@ def test_norm_gradients_of_two_widths(cuda):
         return lambda: (keep, L.lifb_norm_gate_bwd(a, dx.data_ptr(), D, None, D, dh.data_ptr(), None, None, None, None,
                                                    None, 0, s.cuda_stream))[1]
     assert not together([call(512), call(4096), call(512), call(4096)], 5000)
+
+
+def test_attention_of_two_widths(cuda):
+    """Odd widths, on the fp32 pipe: 20 and 80 KB of shared memory."""
+    L = _lib.load()
+
+    def call(D):
+        x, ld, s = torch.randn(2, 8, 1, D, device=cuda), -torch.ones(1, device=cuda), torch.cuda.Stream()
+        o = torch.empty_like(x)
+        torch.cuda.synchronize()
+        a = LEAKY_ATTN.pack(*(x.data_ptr(),) * 3, ld.data_ptr(), 0, 0, 2, 8, 1, 1, D, D, *(8 * D, D, D) * 3, 1.0, 0)
+        keep = (x, ld, s, o)
+        return lambda: (keep, L.lifb_leaky_attn_fwd(a, o.data_ptr(), None, None, 0, s.cuda_stream))[1]
+    assert not together([call(9), call(127), call(9), call(127)], 5000)
