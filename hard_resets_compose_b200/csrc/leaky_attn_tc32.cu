@@ -507,13 +507,14 @@ __global__ void __launch_bounds__(kT32Threads, 1) k_attn_tc32(const __grid_const
 bool attn_tc32_applies(const AttnArgs &a, int passes, int dtype)
 {
     if (dtype != LIFB_F32) return false;
-    auto four = [](const void *p, const int64_t (&st)[3]) {
-        return aligned16(p) && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
+    auto four = [&](const void *p, const int64_t (&st)[3], int group) {  // (one element along it: never used)
+        return aligned16(p) && (a.B == 1 || st[0] % 4 == 0) && (a.T == 1 || st[1] % 4 == 0) &&
+               (a.H == group || st[2] % 4 == 0);
     };
     for (int i = 0; i < passes; i++) {
         const AttnPass &p = a.p[i];
-        if (p.dq > kAttnMaxDim || p.dv > kAttnMaxDim || p.dq % 4 || p.dv % 4 || !aligned16(p.o) || !four(p.q, p.qs) ||
-            !four(p.k, p.ks) || !four(p.v, p.vs))
+        if (p.dq > kAttnMaxDim || p.dv > kAttnMaxDim || p.dq % 4 || p.dv % 4 || !aligned16(p.o) ||
+            !four(p.q, p.qs, p.qg) || !four(p.k, p.ks, p.kg) || !four(p.v, p.vs, p.vg))
             return false;
     }
     return true;

@@ -10,7 +10,11 @@ integrator with a matrix for a state (csrc/leaky_attn.cu).
 q [B, T, H, Dk], k [B, T, Hk, Dk], v [B, T, Hk, Dv] in fp32 or bf16 (the step
 takes fp16 too), H a multiple of Hk (each key/value head serves H / Hk query
 heads), widths up to 128, log_decay [H] fp32 and at most 0 (-inf: no memory),
-states [B, H, Dk, Dv] fp32.  Any strides with a contiguous last dimension.
+states [B, H, Dk, Dv] fp32.  Any strides.  Sequences run on the tensor cores where
+rows of Dk and of Dv elements are whole multiples of 16 bytes (widths of 8 in bf16, 4 in
+fp32); other widths run on the fp32 pipe, some 15 times slower in bf16 and 4 in fp32
+(zero columns added to q, k and v change nothing but the default scale).  An operand or gradient whose last dimension is not dense, whose address or distances are not multiples of
+16 bytes or, in bf16, whose distance is 0 (expand) is copied first.
 fp16 is refused for sequences: a sum over many tokens leaves its range before
 it leaves bf16's.  States and sums are fp32.  In bf16 the outputs of calls of up to 128
 tokens, or up to 8192 tokens of heads in all (B T H), are rounded once; in longer
@@ -31,6 +35,21 @@ MAX_WIDTH = 128
 
 def _last_dense(t):
     return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _rows(t, tc):
+    """t with a dense last dimension; with tc (widths that the tensor-core kernels take) in the
+    16-byte layout that they read: an operand that is not would send the whole call to the fp32 pipe."""
+    t = _last_dense(t)
+    e = t.element_size()
+    if not tc or (t.data_ptr() % 16 == 0 and all(
+            n < 2 or (s * e % 16 == 0 and (e == 4 or s > 0)) for n, s in zip(t.shape[:3], t.stride()[:3]))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _tc_widths(q, v):
+    return q.shape[-1] * q.element_size() % 16 == 0 and v.shape[-1] * v.element_size() % 16 == 0
 
 
 def _pack(q, k, v, log_decay, state, lengths, scale):
@@ -73,7 +92,7 @@ class LeakyAttention(torch.autograd.Function):
         dev = q.device
         if do is None:
             do = torch.zeros(*q.shape[:3], v.shape[3], dtype=q.dtype, device=dev)
-        do = _last_dense(do)
+        do = _rows(do, _tc_widths(q, v))
         dout = None if dout is None else dout.contiguous()
         dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
         ds = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
@@ -141,8 +160,8 @@ def leaky_attention(q, k, v, log_decay, state=None, lengths=None, scale=None, re
             raise ValueError(f"{what}: lengths must be [{B}] int32, got {tuple(lengths.shape)} {lengths.dtype}")
         lengths = lengths.contiguous()
     scale = float(Dk) ** -0.5 if scale is None and Dk > 0 else float(scale or 0.0)
-    args = (_last_dense(q), _last_dense(k), _last_dense(v), log_decay.contiguous(), state, lengths, scale,
-            bool(return_state))
+    tc = _tc_widths(q, v)
+    args = (_rows(q, tc), _rows(k, tc), _rows(v, tc), log_decay.contiguous(), state, lengths, scale, bool(return_state))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (state is not None and state.requires_grad)):
         o, out = LeakyAttention.apply(*args)

@@ -208,3 +208,58 @@ def test_a_step_that_reports_an_error_has_not_run(host):
         with pytest.raises(_lib.LifbError):
             _lib.check_device("after", reset=True)
     assert raised
+
+
+def _layouts(B, T, H, D, dtype, seed):
+    """The same values dense, and in layouts that a tensor map refuses."""
+    x = rand(B, T, H, D, seed=seed, dtype=dtype)
+    wide = torch.zeros(B, T, H, D + 1, device=DEV, dtype=dtype)
+    wide[..., :D] = x
+    off = torch.zeros(x.numel() + 1, device=DEV, dtype=dtype)[1:].view_as(x)
+    off.copy_(x)
+    return x, {"row": wide[..., :D], "address": off}
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("which", ("q", "k", "v", "do"))
+@pytest.mark.parametrize("layout", ("row", "address"))
+def test_layouts_do_not_choose_the_kernel(host, dtype, which, layout):
+    """Operands off the 16-byte grid: the bits of the same call with dense operands."""
+    B, T, H, D = 2, 200, 2, 64
+    ld = -torch.tensor([0.1, 0.01], device=DEV)
+    t = {n: _layouts(B, T, H, D, dtype, i) for i, n in enumerate(("q", "k", "v", "do"))}
+
+    def run(odd):
+        a = {n: (x[1][layout] if odd and n == which else x[0]) for n, x in t.items()}
+        p = [a[n].detach().requires_grad_() for n in ("q", "k", "v")]
+        o, s = leakyattn.leaky_attention(*p, ld, return_state=True)
+        return (o, s, *torch.autograd.grad(o, p, a["do"]))
+    for x, y in zip(run(True), run(False)):
+        assert x.shape == y.shape and torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_expanded_heads_and_gradients(host, dtype):
+    """One key/value head expanded to all, and the gradient of a sum over time."""
+    B, T, H, D = 2, 200, 4, 64
+    q, k, v = rand(B, T, H, D, seed=1, dtype=dtype), rand(B, T, 1, D, seed=2, dtype=dtype), rand(B, T, 1, D, seed=3, dtype=dtype)
+    ld, g = -torch.linspace(0.01, 0.2, H, device=DEV), rand(B, H, D, seed=4, dtype=dtype)
+
+    def run(dense):
+        fit = (lambda x: x.contiguous()) if dense else (lambda x: x)
+        p = [x.detach().requires_grad_() for x in (q, fit(k.expand(B, T, H, D)), fit(v.expand(B, T, H, D)))]
+        o = leakyattn.leaky_attention(*p, ld)
+        return (o, *torch.autograd.grad(o, p, fit(g[:, None].expand(B, T, H, D))))
+    for x, y in zip(run(False), run(True)):
+        assert torch.equal(x, y)
+
+
+def test_one_token_at_an_odd_distance(host):
+    """T = 1: the distance between tokens is never used."""
+    B, H, D = 3, 2, 64
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.zeros(B * H * D, device=DEV, dtype=dtype)
+        x.copy_(rand(B * H * D, seed=1, dtype=dtype))
+        odd = x.as_strided((B, 1, H, D), (H * D, 7, D, 1))
+        ld = -torch.ones(H, device=DEV)
+        assert torch.equal(leakyattn.leaky_attention(odd, odd, odd, ld), leakyattn.leaky_attention(*(x.view(B, 1, H, D),) * 3, ld))
