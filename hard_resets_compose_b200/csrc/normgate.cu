@@ -107,22 +107,34 @@ __device__ __forceinline__ void row_sum(float (&v)[NV], int tpr, float *sh, int 
     }
 }
 
-// sigmoid(g) by the 2-ulp power and the 1-ulp reciprocal: with expf and the division
-// the norms waited for them instead of memory.
-__device__ __forceinline__ float sigmoid(float g) { return rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * g)); }
+// exp(-g).  fp32 rows: expf.  Rows of 16 bits: the 2-ulp power of two; rounding its exponent
+// puts |g| 2^-24 into the result, 2^-17 at |g| = 128, where a bf16 or fp16 output is rounded
+// by 2^-9 or 2^-12 (with expf and the division their norms waited for them instead of memory).
+template <typename T>
+__device__ __forceinline__ float exp_minus(float g)
+{
+    return sizeof(T) == 4 ? expf(-g) : ex2_approx(-1.4426950408889634f * g);
+}
+
+// sigmoid(g), with the 1-ulp reciprocal
+template <typename T>
+__device__ __forceinline__ float sigmoid(float g) { return rcp_approx(1.0f + exp_minus<T>(g)); }
 
 // act(g) and act'(g) of one value, a row's gate
+template <typename T>
 __device__ __forceinline__ float act_value(int act, float g)
 {
-    return act == kActLinear ? g : act == kActSilu ? g * sigmoid(g) : sigmoid(g);
+    return act == kActLinear ? g : act == kActSilu ? g * sigmoid<T>(g) : sigmoid<T>(g);
 }
+template <typename T>
 __device__ __forceinline__ float act_grad(int act, float g)
 {
-    const float sg = sigmoid(g);
+    const float sg = sigmoid<T>(g);
     return act == kActLinear ? 1.0f : act == kActSilu ? sg + g * (sg - sg * sg) : sg - sg * sg;
 }
 
-// The same of a pair: act(g), and with `da` act'(g).
+// The same of a pair (in packed arithmetic): act(g), and with `da` act'(g).
+template <typename T>
 __device__ __forceinline__ uint64_t act_pair(int act, uint64_t g, uint64_t *da)
 {
     if (act == kActLinear) {
@@ -130,8 +142,16 @@ __device__ __forceinline__ uint64_t act_pair(int act, uint64_t g, uint64_t *da)
         return g;
     }
     float z0, z1;
-    both(mul2(g, two(-1.4426950408889634f, -1.4426950408889634f)), z0, z1);
-    both(add2(two(ex2_approx(z0), ex2_approx(z1)), two(1.0f, 1.0f)), z0, z1);
+    if (sizeof(T) == 4) {
+        both(g, z0, z1);
+        z0 = expf(-z0);
+        z1 = expf(-z1);
+    } else {
+        both(mul2(g, two(-1.4426950408889634f, -1.4426950408889634f)), z0, z1);
+        z0 = ex2_approx(z0);
+        z1 = ex2_approx(z1);
+    }
+    both(add2(two(z0, z1), two(1.0f, 1.0f)), z0, z1);
     const uint64_t sg = two(rcp_approx(z0), rcp_approx(z1));
     if (da) {
         const uint64_t d = fma2(mul2(sg, two(-1.0f, -1.0f)), sg, sg);  // sg - sg^2
@@ -246,7 +266,7 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(false, MAXT, VEC, NIT
         nx.get(x);
         nh.get(h);
         if (full_gate) ng.get(gt);
-        const float arow = row_gate ? act_value(a.act, grow) : 1.0f;
+        const float arow = row_gate ? act_value<T>(a.act, grow) : 1.0f;
         fetch(r + stride);
         if (a.h) {
             uint64_t s2 = 0;
@@ -261,7 +281,7 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(false, MAXT, VEC, NIT
 #pragma unroll
             for (int i = 0; i < P; i++) {
                 uint64_t y = mul2(h.v[i], post.v[i]);
-                if (full_gate) y = mul2(y, act_pair(act, gt.v[i], nullptr));
+                if (full_gate) y = mul2(y, act_pair<T>(act, gt.v[i], nullptr));
                 x.v[i] = fma2(kk, y, x.v[i]);
             }
             if (on) store_row(x, a.xo, r * a.D + c0, step, in);
@@ -370,13 +390,13 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT)
         nh.get(hh);
         if (full_gate) ng.get(av);
         if (kAhead) fetch(r + stride);
-        const float arow = row_gate ? act_value(a.act, grow) : 1.0f;
+        const float arow = row_gate ? act_value<T>(a.act, grow) : 1.0f;
         if (a.h) {
             const uint64_t k = two(rh, rh);
 #pragma unroll
             for (int i = 0; i < P; i++) {
                 hh.v[i] = mul2(hh.v[i], k);
-                if (full_gate) av.v[i] = act_pair(act, av.v[i], &da.v[i]);
+                if (full_gate) av.v[i] = act_pair<T>(act, av.v[i], &da.v[i]);
             }
         }
         if (a.dn) {
@@ -443,7 +463,7 @@ __global__ void __launch_bounds__(MAXT, norm_blocks_per_sm(true, MAXT, VEC, NIT)
 #pragma unroll
             for (int i = 0; i < P; i++) t.v[i] = mul2(kh, fma2(hh.v[i], mm, t.v[i]));
             if (on && a.dh) store_row(t, a.dh, r * a.D + c0, step, in);
-            if (row_gate && a.dgate && on && lane == 0) ((T *)a.dgate)[r] = from_f32<T>(m[1] * act_grad(a.act, grow));
+            if (row_gate && a.dgate && on && lane == 0) ((T *)a.dgate)[r] = from_f32<T>(m[1] * act_grad<T>(a.act, grow));
         }
     }
     if (!a.part) return;

@@ -263,3 +263,28 @@ def test_one_token_at_an_odd_distance(host):
         odd = x.as_strided((B, 1, H, D), (H * D, 7, D, 1))
         ld = -torch.ones(H, device=DEV)
         assert torch.equal(leakyattn.leaky_attention(odd, odd, odd, ld), leakyattn.leaky_attention(*(x.view(B, 1, H, D),) * 3, ld))
+
+
+@pytest.mark.parametrize("act", ("silu", "sigmoid"))
+@pytest.mark.parametrize("gate", ("full", "row"))
+def test_fp32_gates_far_from_zero(host, act, gate):
+    """fp32: sigmoid to a few ulps wherever it is not subnormal, also where |gate| is large.  One row
+    of D = 1 columns leaves x' = act(g) * +-1 (h = 2, eps = 0): relative error below 16 2^-24
+    (exp 2 ulps, sum, quotient and products: 8 roundings, each at most 2^-23)."""
+    g = torch.linspace(-80.0, 80.0, 4001, device=DEV)[:, None]
+    if gate == "full":
+        g = torch.cat((g, g.flip(0)), 1)
+    D = g.shape[1] if gate == "full" else 2
+    h, x = torch.full((4001, D), 2.0, device=DEV), torch.zeros(4001, D, device=DEV)
+    got = normgate.norm_gate_residual(x, h, g, torch.ones(D, device=DEV), act=act, eps=0.0).double()
+    s = torch.sigmoid(g.double())
+    want = (s * g.double() if act == "silu" else s).expand(4001, D)
+    assert ((got - want).abs() <= 16 * 2.0 ** -24 * want.abs() + 1e-37).all()
+    # and its derivative: sum over the row of 1 * (+-1) * act'(g)
+    gq = g.clone().requires_grad_()
+    got, = torch.autograd.grad(normgate.norm_gate_residual(x, h, gq, torch.ones(D, device=DEV), act=act, eps=0.0).sum(), gq)
+    d = s * (1 - s) if act == "sigmoid" else s * (1 + g.double() * (1 - s))
+    want = d if gate == "full" else d * D
+    # 1 - s loses what s has rounded away near 1: an absolute 2^-24 of the larger term
+    near = 2.0 ** -22 * (s if act == "sigmoid" else s * (1 + g.double().abs())) * (1 if gate == "full" else D)
+    assert ((got.double() - want).abs() <= 16 * 2.0 ** -24 * want.abs() + near + 1e-37).all()
