@@ -17,7 +17,8 @@ cache of states that sequences have slots in (`new_cache`).
     logits = net.step(next_tokens, cache, slots)           # [B, V]
 
 Attention, norms and embedding run in the weights' type (fp32 or bf16); the LIF
-layer's input, potential and spikes are fp32, as everywhere in this package.
+layer's input, potential and spikes are fp32, as everywhere in this package.  Under
+autocast to bf16 the linear layers, attention and readout run in bf16 around an fp32 stream.
 The reference has no such model.
 """
 from __future__ import annotations
@@ -109,11 +110,12 @@ class SeqNet(nn.Module):
     def _block(self, i, x, n, attend, spike):
         """Block i; attend(block, q, k, v) and spike(block, current) keep its states."""
         b, s = self.blocks[i], self.residual_scale
+        stream = lambda *ts: [t.to(x.dtype) for t in ts]  # noqa: E731 (autocast's linear layers give bf16)
         q, k, v, g = b.attention_in(n)
-        h = b.out(attend(b, q, k, v).flatten(-2))
+        h, g = stream(b.out(attend(b, q, k, v).flatten(-2)), g)
         x, n = norm_gate_residual(x, h, g, b.post_attn, b.pre_lif, residual_scale=s)
         current, g = b.lif_input(n)
-        h = b.lif_out(spike(b, current).to(n.dtype))
+        h, g = stream(b.lif_out(spike(b, current).to(n.dtype)), g)
         return norm_gate_residual(x, h, g, b.post_lif, self.pre[i + 1], residual_scale=s, act="sigmoid")
 
     def _spikes(self, b, current):

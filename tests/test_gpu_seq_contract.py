@@ -288,3 +288,19 @@ def test_fp32_gates_far_from_zero(host, act, gate):
     # 1 - s loses what s has rounded away near 1: an absolute 2^-24 of the larger term
     near = 2.0 ** -22 * (s if act == "sigmoid" else s * (1 + g.double().abs())) * (1 if gate == "full" else D)
     assert ((got.double() - want).abs() <= 16 * 2.0 ** -24 * want.abs() + near + 1e-37).all()
+
+
+def test_the_model_under_autocast(host):
+    """Linear layers in bf16 around an fp32 stream.  Without spikes (a threshold that nothing reaches), whose
+    flips would be large, some ten values on the way to a logit are rounded to bf16, 2^-8 each: below 2^-4."""
+    from hard_resets_compose_b200.seqnet import SeqNet
+    from tests.seq_refs import rel
+    torch.manual_seed(3)
+    net = SeqNet(vocab=50, width=64, heads=4, layers=1).cuda()
+    net.theta = 1e9
+    tok = torch.randint(0, 50, (3, 40), device=DEV)
+    want = net(tok)
+    with torch.autocast("cuda", torch.bfloat16):
+        got = net(tok)
+        got.float().sum().backward()
+    assert rel(got, want) < 2.0 ** -4 and all(torch.isfinite(p.grad).all() for p in net.parameters())
