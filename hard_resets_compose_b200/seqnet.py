@@ -121,6 +121,8 @@ class SeqNet(nn.Module):
     def _spikes(self, b, current):
         """[B, T, D] currents to spikes, from rest."""
         B, T, D = current.shape
+        if current.numel() == 0:
+            return current
         i = current.transpose(0, 1).reshape(T, B * D)
         s = L.lif_tuned(i, torch.zeros(B * D, device=i.device), beta=b.beta, theta=self.theta)
         return s.view(T, B, D).transpose(0, 1)

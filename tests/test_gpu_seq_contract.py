@@ -304,3 +304,21 @@ def test_the_model_under_autocast(host):
         got = net(tok)
         got.float().sum().backward()
     assert rel(got, want) < 2.0 ** -4 and all(torch.isfinite(p.grad).all() for p in net.parameters())
+
+
+
+def test_the_model_without_tokens(host):
+    """No sequence, and sequences without a token, in every form of the model."""
+    from hard_resets_compose_b200.seqnet import SeqNet
+    net = SeqNet(vocab=50, width=64, heads=4, layers=2).cuda()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    tok, cache = torch.zeros(2, 0, dtype=torch.long, device=DEV), net.new_cache(3)
+    for t in (tok, tok[:0], torch.zeros(0, 5, dtype=torch.long, device=DEV)):
+        out = net(t)
+        assert out.shape == (*t.shape, 50)
+        out.sum().backward()
+        assert not any(p.grad is not None and p.grad.any() for p in net.parameters())
+    assert not net.prompt(tok, cache, i32(0, 2), i32(0, 0)).any()
+    assert net.prompt(tok[:0], cache, i32(), i32()).shape == (0, 50)
+    assert net.prompt(torch.zeros(0, 5, dtype=torch.long, device=DEV), cache, i32(), i32()).shape == (0, 50)
+    assert net.step(torch.zeros(0, dtype=torch.long, device=DEV), cache, i32()).shape == (0, 50)
