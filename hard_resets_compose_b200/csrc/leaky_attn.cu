@@ -634,8 +634,8 @@ extern "C" int lifb_leaky_attn_fwd(const lifb_leaky_attn *p, void *o, float *sta
     if (!p->q || !p->k || !p->v) return at_fail(LIFB_ERR_INVALID_ARGUMENT, what, "null pointer");
     const Split sp = split_of(*p, false);
     const AttnWs w = carve(workspace, *p, false, sp);
-    if (w.bytes && (!workspace || workspace_bytes < w.bytes))
-        return at_fail(LIFB_ERR_WORKSPACE, what, "workspace missing or too small");
+    if (w.bytes && (!workspace || !aligned16(workspace) || workspace_bytes < w.bytes))
+        return at_fail(LIFB_ERR_WORKSPACE, what, "workspace missing, misaligned or too small");
     AttnArgs a = {};
     a.log_decay = p->log_decay;
     a.lengths = p->lengths;
@@ -690,8 +690,8 @@ extern "C" int lifb_leaky_attn_bwd(const lifb_leaky_attn *p, const void *d_o, co
         return at_fail(LIFB_ERR_INVALID_ARGUMENT, what, "null pointer");
     const Split sp = split_of(*p, true);
     const AttnWs w = carve(workspace, *p, true, sp);
-    if (w.bytes && (!workspace || workspace_bytes < w.bytes))
-        return at_fail(LIFB_ERR_WORKSPACE, what, "workspace missing or too small");
+    if (w.bytes && (!workspace || !aligned16(workspace) || workspace_bytes < w.bytes))
+        return at_fail(LIFB_ERR_WORKSPACE, what, "workspace missing, misaligned or too small");
     AttnArgs a = {};
     a.log_decay = p->log_decay;
     a.lengths = p->lengths;

@@ -750,8 +750,8 @@ extern "C" int lifb_norm_gate_bwd(const lifb_norm_gate *p, const void *dxo, int6
     a.dgate = dgate;
     if (!a.x || !a.rstd || (a.h && !a.post) || (dn && !a.pre) || (p->gate_cols && !p->gate) || (!dxo && !dn))
         return norm_fail(LIFB_ERR_INVALID_ARGUMENT, what, "null pointer");
-    if (weights && (!workspace || workspace_bytes < lifb_norm_gate_bwd_workspace_bytes(a.R, a.D, p->dtype)))
-        return norm_fail(LIFB_ERR_WORKSPACE, what, "workspace missing or too small");
+    if (weights && (!workspace || !aligned16(workspace) || workspace_bytes < lifb_norm_gate_bwd_workspace_bytes(a.R, a.D, p->dtype)))
+        return norm_fail(LIFB_ERR_WORKSPACE, what, "workspace missing, misaligned or too small");
     a.part = weights ? (float *)workspace : nullptr;
     const bool gate = a.gate && !a.gate_row;
     const int elem = (int)dtype_bytes(p->dtype);

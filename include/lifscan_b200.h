@@ -563,7 +563,8 @@ int lifb_tshard_bwd_fix(const float *I, const float *u_prev, const float *U, con
  * status 102 (lifb_check_device).
  * Gradient: dW [V, D] (contiguous, written whole) = scale * the sum of dY's rows
  * of each token, in an order that the tokens alone fix (same bits each call).
- * Sums in fp32, rounded once.  n < 2^31 - 2^20, V < 2^30. */
+ * Sums in fp32, rounded once.  n < 2^31 - 2^20, V < 2^30.  The workspace is 256-byte
+ * aligned. */
 int lifb_embed_fwd(const void *tokens, int token_bytes, const void *W, void *Y, int64_t n, int64_t V,
                    int64_t D, int64_t w_stride, float scale, int dtype, void *stream);
 size_t lifb_embed_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
@@ -589,7 +590,7 @@ typedef struct lifb_norm_gate {
 int lifb_norm_gate_fwd(const lifb_norm_gate *args, void *xo, void *n, void *stream);
 /* Gradients from dxo and dn (either may be NULL: zero); dx, dh, dgate, dpost and
  * dpre (contiguous) are written where not NULL.  The workspace is for dpost and
- * dpre, whose sums run in a fixed order. */
+ * dpre, whose sums run in a fixed order; it is 16-byte aligned. */
 size_t lifb_norm_gate_bwd_workspace_bytes(int64_t R, int64_t D, int dtype);
 int lifb_norm_gate_bwd(const lifb_norm_gate *args, const void *dxo, int64_t dxo_stride, const void *dn,
                        int64_t dn_stride, void *dx, void *dh, void *dgate, void *dpost, void *dpre,
@@ -601,7 +602,8 @@ int lifb_norm_gate_bwd(const lifb_norm_gate *args, const void *dxo, int64_t dxo_
  * elements for sequence, token and head; the last dimension contiguous), H a
  * multiple of Hk, Dk and Dv <= 128, log_decay [H] fp32, state [B, H, Dk, Dv] fp32
  * (NULL: zeros), lengths [B] (NULL: T each): tokens at and past a sequence's
- * length are not read, change no state and give zeros. */
+ * length are not read, change no state and give zeros.  T < 2^31 - 256, B * H <
+ * 2^16.  Workspaces are 16-byte aligned. */
 typedef struct lifb_leaky_attn {
     const void *q, *k, *v;
     const float *log_decay, *state;
