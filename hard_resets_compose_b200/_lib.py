@@ -9,8 +9,10 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import subprocess
 import threading
 import time
+import warnings
 
 import torch
 from torch.autograd import forward_ad
@@ -213,27 +215,44 @@ def load(build_if_missing: bool = True):
 _fast = None
 
 
+class _NoBinding:
+    """In the place of a binding that cannot be had: leaves every call to Python."""
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def fast():
     """The host binding of the sequence-model operators (csrc/host/seq_binding.cpp), over
     the loaded library: torch autograd nodes without Python in them.  Its functions
-    return None for calls that they leave to the Python functions of the same names."""
+    return None for calls that they leave to the Python functions of the same names,
+    which give the same bits and take twice as long on the host.  All calls go to those,
+    with a warning, where the binding can neither be built nor loaded."""
     global _fast
     if _fast is None:
-        import importlib.util
         L = load()
         with _lock:
             try:
-                path = _build.build_binding()
-            except (RuntimeError, OSError) as e:  # no g++: use the prebuilt binding if present
-                path = _build.binding_path()
-                if not os.path.exists(path):
-                    raise RuntimeError(f"{os.path.basename(path)} is missing and cannot be built: {e}") from e
-            spec = importlib.util.spec_from_file_location("lifb_seq", path)
-            m = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(m)
-            m.bind({name: ctypes.cast(getattr(L, name), c_void_p).value for name in SIGNATURES}, check)
-            _fast = m
+                _fast = _load_binding(L)
+            except (RuntimeError, OSError, ImportError, subprocess.CalledProcessError) as e:
+                warnings.warn(f"no host binding for the sequence operators, small calls will be slower: {e}",
+                              RuntimeWarning, stacklevel=3)
+                _fast = _NoBinding()
     return _fast
+
+
+def _load_binding(L):
+    import importlib.util
+    try:
+        path = _build.build_binding()
+    except (RuntimeError, OSError, subprocess.CalledProcessError):  # no compiler: use the prebuilt one if present
+        path = _build.binding_path()
+        if not os.path.exists(path):
+            raise
+    spec = importlib.util.spec_from_file_location("lifb_seq", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    m.bind({name: ctypes.cast(getattr(L, name), c_void_p).value for name in SIGNATURES}, check)
+    return m
 
 
 def check(status: int, what: str, lib=None) -> None:
