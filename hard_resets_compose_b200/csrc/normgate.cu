@@ -531,25 +531,25 @@ bool norm_shape(int64_t D, int vec, int elem, bool bwd, NormShape &s)
     const int widest = 16 / elem;
     const bool wide = vec > 1;
     const int64_t vecs = (D + s.vec - 1) / s.vec;
-    auto spread = [&](int tpr, int elems) {
+    // the row over `tpr` threads of a block of `threads`, with as few elements each as hold it
+    auto spread = [&](int threads, int tpr, int elems) {
+        s.threads = threads;
         s.tpr = tpr;
         // 16-byte vectors: any number of them; single elements: 4, 8 or 16; between: 8 or 16 elements
         s.nit = vec == widest ? 1 : wide ? 8 / vec : 4;
         while (s.nit * s.vec < elems && (int64_t)s.tpr * s.nit < vecs) s.nit *= 2;
         return (int64_t)s.tpr * s.nit >= vecs;
     };
-    s.threads = kNgThreads;
+    // elements a thread at most before the row takes more threads
+    auto most = [&](int tpr) {
+        if (tpr < 32) return wide && vec < widest ? 8 : vec;  // part of a warp: the fewest there are
+        if (!wide) return tpr == 32 ? kNgMaxElems : tpr < kNgThreads ? 4 : 8;
+        return elem == 2 || bwd ? kNgMaxElems : 8;
+    };
     for (int tpr = 8; tpr <= kNgThreads; tpr *= 2)
-        if (spread(tpr, tpr < 32 ? (vec == widest || !wide ? s.vec : 8) : !wide ? (tpr == 32 ? kNgMaxElems : tpr == kNgThreads ? 8 : 4) : elem == 2 || bwd ? kNgMaxElems : 8))
-            return true;
-    if (!wide || (elem == 4 && vec == 2)) {
-        s.threads = kNgMaxThreads;
-        if (spread(kNgMaxThreads, 8)) return true;
-        s.threads = kNgThreads;
-    }
-    if (spread(kNgThreads, kNgMaxElems)) return true;
-    s.threads = kNgMaxThreads;
-    return spread(kNgMaxThreads, kNgMaxElems);
+        if (spread(kNgThreads, tpr, most(tpr))) return true;
+    if ((!wide || (elem == 4 && vec == 2)) && spread(kNgMaxThreads, kNgMaxThreads, 8)) return true;
+    return spread(kNgThreads, kNgThreads, kNgMaxElems) || spread(kNgMaxThreads, kNgMaxThreads, kNgMaxElems);
 }
 
 int64_t norm_blocks(const NormShape &s, int64_t R, bool bwd)
