@@ -322,3 +322,30 @@ def test_the_model_without_tokens(host):
     assert net.prompt(tok[:0], cache, i32(), i32()).shape == (0, 50)
     assert net.prompt(torch.zeros(0, 5, dtype=torch.long, device=DEV), cache, i32(), i32()).shape == (0, 50)
     assert net.step(torch.zeros(0, dtype=torch.long, device=DEV), cache, i32()).shape == (0, 50)
+
+
+def test_calls_are_captured_into_graphs(host):
+    """The status is not polled inside a capture (even where a poll is due), and replays give the same bits."""
+    B, T, H, D = 2, 150, 2, 64
+    q, k, v = (rand(B, T, H, D, seed=i, dtype=torch.bfloat16) for i in range(3))
+    ld, w, table = -torch.ones(H, device=DEV), rand(D, seed=4), rand(10, D, seed=5)
+    tok, state = torch.arange(6, device=DEV), rand(B, H, D, D, seed=6)
+
+    def run(s):
+        return (*leakyattn.leaky_attention(q, k, v, ld, state=state, return_state=True),
+                leakyattn.leaky_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s), normgate.rms_norm(q, w),
+                embed.embedding(tok, table), s)
+    want = run(state.clone())
+    s, side = state.clone(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(s)  # warm up
+    torch.cuda.current_stream().wait_stream(side)
+    time.sleep(0.03)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run(s)
+    s.copy_(state)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
