@@ -107,7 +107,8 @@ struct TcBars {
 // This thread's row of P: scores from tensor memory, times p_scale * b^distance
 // where the other token is not in the future (and is one of the n), else zero;
 // packed to bf16 into 64 of the same 128 columns.  Powers of b run from the
-// diagonal outwards (pw: of 16 columns, in their order).  Forward passes walk the columns
+// diagonal outwards, a product each (at most 128 of them: 2^-17, below the 2^-16 of two
+// pieces) (pw: of 16 columns, in their order).  Forward passes walk the columns
 // downwards and pack into the upper half, backward passes the other way round, so
 // that nothing unread is overwritten.  FINE: two bf16 pieces (2^-18) in place of one,
 // each 16 columns of scores becoming 8 of the first and 8 of the second.

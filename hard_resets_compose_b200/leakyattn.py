@@ -13,14 +13,15 @@ heads), widths up to 128, log_decay [H] fp32 and at most 0 (-inf: no memory),
 states [B, H, Dk, Dv] fp32.  Any strides.  Sequences run on the tensor cores where
 rows of Dk and of Dv elements are whole multiples of 16 bytes (widths of 8 in bf16, 4 in
 fp32); other widths run on the fp32 pipe, some 15 times slower in bf16 and 4 in fp32
-(zero columns added to q, k and v change nothing but the default scale).  An operand or gradient whose last dimension is not dense, whose address or distances are not multiples of
-16 bytes or, in bf16, whose distance is 0 (expand) is copied first.
+(zero columns added to q, k and v change nothing but the default scale).  An operand or
+gradient whose last dimension is not dense, whose address or distances are not multiples
+of 16 bytes or, in bf16, whose distance is 0 (expand) is copied first.  B H < 2^16.
 fp16 is refused for sequences: a sum over many tokens leaves its range before
 it leaves bf16's.  States and sums are fp32.  In bf16 the outputs of calls of up to 128
-tokens, or up to 8192 tokens of heads in all (B T H), are rounded once; in longer
+tokens, or up to 8192 tokens of heads in all (B T H), are rounded once; in larger
 ones the decayed scores and the state are rounded to bf16 before they meet v and q
-too (relative error 2.4e-3 in place of 1.7e-3; fp32 inputs: 3e-7).  The decay is a constant: it gets no gradient.  The reference
-has no such operator.
+too (relative error 2.4e-3 in place of 1.7e-3; fp32 inputs: 3e-7).  The decay is a
+constant: it gets no gradient.  The reference has no such operator.
 """
 from __future__ import annotations
 
