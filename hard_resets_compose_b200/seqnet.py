@@ -70,7 +70,8 @@ class SeqBlock(nn.Module):
         self.lif_out = nn.Linear(width, width, bias=False)
         self.post_attn, self.pre_lif, self.post_lif = (nn.Parameter(torch.ones(width)) for _ in range(3))
         # memories from a few tokens to thousands
-        self.register_buffer("log_decay", torch.log1p(-torch.exp2(-torch.linspace(2.0, 10.0, heads))))
+        memory = torch.linspace(2.0, 10.0, heads, dtype=torch.float32)
+        self.register_buffer("log_decay", torch.log1p(-torch.exp2(-memory)))
 
     def _apply(self, fn, recurse=True):
         """Moves of the module; the decay stays fp32 (1 - 2^-10 is 1 in bf16), bit for bit."""
@@ -124,7 +125,7 @@ class SeqNet(nn.Module):
         if current.numel() == 0:
             return current
         i = current.transpose(0, 1).reshape(T, B * D)
-        s = L.lif_tuned(i, torch.zeros(B * D, device=i.device), beta=b.beta, theta=self.theta)
+        s = L.lif_tuned(i, i.new_zeros(B * D), beta=b.beta, theta=self.theta)
         return s.view(T, B, D).transpose(0, 1)
 
     def forward(self, tokens, lengths=None):
@@ -138,9 +139,8 @@ class SeqNet(nn.Module):
     def new_cache(self, slots):
         """States of `slots` sequences at rest: for each block the attention's and
         the LIF layer's potentials."""
-        dev = self.embed.device
-        return [(torch.zeros(slots, b.heads, b.dim, b.dim, device=dev), torch.zeros(slots, self.width, device=dev))
-                for b in self.blocks]
+        zeros = lambda *shape: torch.zeros(slots, *shape, device=self.embed.device, dtype=torch.float32)  # noqa: E731
+        return [(zeros(b.heads, b.dim, b.dim), zeros(self.width)) for b in self.blocks]
 
     @torch.no_grad()
     def prompt(self, tokens, cache, slots, lengths):
@@ -167,7 +167,7 @@ class SeqNet(nn.Module):
 
             def spike(b, current):
                 i = current.transpose(0, 1).reshape(T, B * self.width).contiguous()
-                u, s = L.serial_forward(i, b.beta, self.theta, 0.0, torch.zeros(i.shape[1], device=i.device))
+                u, s = L.serial_forward(i, b.beta, self.theta, 0.0, i.new_zeros(i.shape[1]))
                 places.put(potentials, torch.where(empty, 0.0, u.view(T, B, self.width)[last, rows]))
                 return s.view(T, B, self.width).transpose(0, 1)
 

@@ -132,3 +132,17 @@ def test_prompts_without_tokens(net):
     got = net.prompt(torch.zeros(2, 0, dtype=torch.long), cache, i32(0, 1), i32(0, 0))
     assert got.shape == (2, 30) and not got.any()
     assert not any(t.any() for pair in cache for t in pair)
+
+
+def test_a_model_built_in_bf16(net):
+    """Under another default type: the weights have it, the decay and the cache stay fp32."""
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        n = seqnet.SeqNet(vocab=30, width=16, heads=2, layers=2)
+        cache = n.new_cache(2)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert n.embed.dtype == torch.bfloat16
+    for a, b in zip(n.blocks, net.blocks):
+        assert torch.equal(a.log_decay, b.log_decay)
+    assert all(t.dtype == torch.float32 for pair in cache for t in pair)
